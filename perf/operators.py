@@ -216,21 +216,15 @@ def prepare(case, seed):
 # ---------------------------------------------------------------------------------------------------------------------
 
 def quantise(rows, bits, D):
-    """(codes int8 [rows, heads, D], scales bf16 [rows, heads, D / 32]) of rows [rows, heads * D], a few rows at a time."""
+    """(codes int8 [rows, heads, D], scales bf16 [rows, heads, D / 32]) of rows [rows, heads * D]."""
     top = 7 if bits == 4 else 127
-    codes = torch.empty((rows.shape[0], rows.shape[1] // D, D), dtype=torch.int8, device=rows.device)
-    scales = torch.empty((*codes.shape[:2], D // GROUP), dtype=torch.bfloat16, device=rows.device)
-    step = max(1, (1 << 27) // rows.shape[1])
-    for a in range(0, rows.shape[0], step):
-        x = rows[a:a + step].float().view(-1, codes.shape[1], D // GROUP, GROUP)
-        most = x.abs().amax(-1)
-        # (by a tensor: torch divides by a number as a product with its reciprocal, which rounds twice)
-        s = torch.where(torch.isfinite(most), most / torch.full_like(most, top), torch.nan).to(torch.bfloat16)
-        by = s.float().unsqueeze(-1)
-        q = torch.where(by > 0, torch.round(x / by), 0.0).clamp(-top, top)
-        codes[a:a + step] = q.view(q.shape[0], codes.shape[1], D).to(torch.int8)
-        scales[a:a + step] = s
-    return codes, scales
+    x = rows.float().view(rows.shape[0], -1, D // GROUP, GROUP)
+    most = x.abs().amax(-1)
+    # (by a tensor: torch divides by a number as a product with its reciprocal, which rounds twice)
+    scales = torch.where(torch.isfinite(most), most / torch.full_like(most, top), torch.nan).to(torch.bfloat16)
+    by = scales.float().unsqueeze(-1)
+    codes = torch.where(by > 0, torch.round(x / by), 0.0).clamp(-top, top)
+    return codes.view(*scales.shape[:2], D).to(torch.int8), scales
 
 
 def values(codes, scales):
@@ -239,56 +233,48 @@ def values(codes, scales):
     return x.view(codes.shape)
 
 
+def tokens_of(held, at):
+    """Values [B, n, G, D] of the tokens at [B, n] (places before the first are those of the first)."""
+    who = torch.arange(at.shape[0], device="cuda").unsqueeze(1)
+    return values(*(t[who, at.clamp(min=0)] for t in held))
+
+
 def plain_attend(st):
-    c, (q,), out = st["c"], st["rows"], []
-    m, H, G, D = c["m"], c["H"], c["G"], c["D"]
-    (kc, ks), (vc, vs) = st["k"], st["v"]
-    q = q.float().view(c["B"], m, G, H // G, D)
-    for b, n in enumerate(st["lens"]):
-        first = max(0, n - m + 1 - c["window"]) if c["window"] else 0
-        if n == 0:
-            out.append(torch.zeros((m, H * D), dtype=DTYPES[c["dtype"]], device="cuda"))
-            continue
-        k, v = values(kc[b, first:n], ks[b, first:n]), values(vc[b, first:n], vs[b, first:n])   # [tokens, G, D]
-        s = torch.einsum("mgrd,tgd->grmt", q[b], k) * D ** -0.5
-        if c["softcap"]:
-            s = c["softcap"] * torch.tanh(s / c["softcap"])
-        p = torch.arange(n - m, n, device="cuda").unsqueeze(1)
-        t = torch.arange(first, n, device="cuda").unsqueeze(0)
-        if st["slopes"] is not None:
-            s = s - st["slopes"].view(G, H // G, 1, 1) * (p - t).float()
-        seen = (t <= p) & (p - t < c["window"]) if c["window"] else t <= p
-        s = torch.where(seen, s, -torch.inf)
-        most = s.amax(-1, keepdim=True)
-        e = torch.exp(s - torch.where(torch.isinf(most), 0.0, most))
-        total = e.sum(-1, keepdim=True)
-        o = torch.einsum("grmt,tgd->mgrd", e / torch.where(total > 0, total, 1.0), v)
-        out.append(o.reshape(m, H * D).to(DTYPES[c["dtype"]]))
-    return torch.cat(out)
+    c, (q,) = st["c"], st["rows"]
+    B, m, H, G, D = c["B"], c["m"], c["H"], c["G"], c["D"]
+    ends = torch.tensor(st["lens"], device="cuda").unsqueeze(1)
+    span = max(1, max(visible(c, n) for n in st["lens"]))
+    t = ends - span + torch.arange(span, device="cuda")                      # [B, span]: every token that some query of the sequence sees
+    far = (ends - m + torch.arange(m, device="cuda")).unsqueeze(2) - t.unsqueeze(1)   # [B, m, span]
+    s = torch.einsum("bmgrd,btgd->bgrmt", q.float().view(B, m, G, H // G, D), tokens_of(st["k"], t)) * D ** -0.5
+    if c["softcap"]:
+        s = c["softcap"] * torch.tanh(s / c["softcap"])
+    if st["slopes"] is not None:
+        s = s - st["slopes"].view(G, H // G, 1, 1) * far.float()[:, None, None]
+    seen = (far >= 0) & (t >= 0).unsqueeze(1) & (far < (c["window"] or span + m))
+    s = torch.where(seen[:, None, None], s, -torch.inf)
+    most = s.amax(-1, keepdim=True)
+    e = torch.exp(s - torch.where(torch.isinf(most), 0.0, most))
+    total = e.sum(-1, keepdim=True)
+    o = torch.einsum("bgrmt,btgd->bmgrd", e / torch.where(total > 0, total, 1.0), tokens_of(st["v"], t))
+    return o.reshape(B * m, H * D).to(q.dtype)
 
 
 def plain_write(st):
     c, got = st["c"], []
+    who = torch.arange(c["B"], device="cuda").unsqueeze(1)
+    at = torch.tensor(st["lens"], device="cuda").unsqueeze(1) + torch.arange(c["m"], device="cuda")
     for which, new, bits in (("k", st["rows"][0], c["kb"]), ("v", st["rows"][1], c["vb"])):
-        codes, scales = quantise(new, bits, c["D"])
-        codes, scales = codes.view(c["B"], c["m"], c["G"], -1), scales.view(c["B"], c["m"], c["G"], -1)
-        for b, n in enumerate(st["lens"]):
-            st[which][0][b, n:n + c["m"]] = codes[b]
-            st[which][1][b, n:n + c["m"]] = scales[b]
-        back = [values(st[which][0][b, n:n + c["m"]], st[which][1][b, n:n + c["m"]]).to(new.dtype) for b, n in enumerate(st["lens"])]
-        got.append(torch.stack(back))
+        for held, t in zip(st[which], quantise(new, bits, c["D"])):
+            held[who, at] = t.view(c["B"], c["m"], c["G"], -1)
+        got.append(tokens_of(st[which], at).to(new.dtype))
     return got
 
 
 def plain_read(st):
-    c, got = st["c"], []
-    for which in "kv":
-        codes, scales = st[which]
-        back = torch.zeros(codes.shape, dtype=DTYPES[c["dtype"]], device="cuda")
-        for b, n in enumerate(st["lens"]):
-            back[b, :n] = values(codes[b, :n], scales[b, :n]).to(back.dtype)
-        got.append(back)
-    return got
+    c = st["c"]
+    inside = torch.arange(capacity(c), device="cuda") < torch.tensor(st["lens"], device="cuda").unsqueeze(1)
+    return [torch.where(inside[..., None, None], values(*st[which]), 0.0).to(DTYPES[c["dtype"]]) for which in "kv"]
 
 
 # ---------------------------------------------------------------------------------------------------------------------
