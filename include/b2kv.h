@@ -609,6 +609,72 @@ int b2kv_moe_combine(float* x, int64_t ld_x, const void* y, int64_t ld_y, const 
                      int top, int dim, int dtype, void* stream);
 
 /*
+ * A cache of quantised keys and values.  A row (one token of one key / value head, D elements) is cut into groups of 32 elements;
+ * a group is whole numbers of `bits` = 4 or 8 bits and one bfloat16 scale:
+ *   scale = bf16(max |x| / L), L = 7 or 127;  code = x / scale to the nearest whole number, ties to even, within -L .. L, 0 where
+ *   the scale is 0;  value = code * scale.
+ * A group with an infinity or a NaN has a NaN for its scale: it reads back as NaN.  No counterpart in the reference, whose cache
+ * is fp32 (simple-llm/src/gpu/gpu_kv_cache.py:66-78).
+ *
+ * Rows of a head lie one behind the other: token t of sequence b, head g is row (b * G + g) * T_max + t of the codes and of the
+ * scales; through a block table (max_blocks per sequence, n_blocks in the pool) row (block * G + g) * block_size + t % block_size.  Inside a row
+ * the elements lie as the matrix instructions of b2kv_qcache_attend take them, so that nothing is moved between lanes there:
+ *   keys    element 32 u + 8 o + i is code i of unit o * (D / 32) + u, units of 8 codes;
+ *   values  element 32 u + 4 o + i is code i of unit o * (D / 32) + u, units of 4 codes;
+ *   codes   lowest bits first, stored as code + 8 or code + 128;
+ *   scales  scale of group u at u of b2kv_qcache_scale_row(D) bfloat16 per row (the rest is not used).
+ * D is 32, 64, 96, 128 or 256.  (k_bits, v_bits) is (4, 4), (8, 4) or (8, 8): keys are what suffers from few bits.
+ * dtype is the type of the rows that are written, read back and attended with.  seq_lens (device, B entries) or len are the tokens
+ * that each sequence holds; T_max bounds them (through a block table too).
+ */
+typedef struct b2kv_qcache {
+    void* k_codes;  /* rows of D * k_bits / 8 bytes */
+    void* v_codes;  /* rows of D * v_bits / 8 bytes */
+    void* k_scales; /* rows of b2kv_qcache_scale_row(D) bfloat16 */
+    void* v_scales;
+    const int32_t* block_table; /* [B, max_blocks], or NULL: contiguous */
+    const int32_t* seq_lens;    /* [B], or NULL: len for every sequence */
+    int32_t len, B, G, D, T_max, max_blocks, block_size, n_blocks, k_bits, v_bits, dtype;
+} b2kv_qcache;
+int b2kv_qcache_scale_row(int D); /* 0: not a D of this cache */
+
+/*
+ * Quantises n rows per sequence into places len_b .. len_b + n - 1: row b * n + i of k and v ([B * n, G * D], ld elements from one to
+ * the next) is place len_b + i of sequence b.  No length is advanced.  A place outside [0, T_max) or a bad table entry is skipped
+ * and recorded in dev_status.
+ */
+int b2kv_qcache_write(const b2kv_qcache* cache, const void* k, int64_t ld_k, const void* v, int64_t ld_v, int n, int32_t* dev_status,
+                      void* stream);
+
+/*
+ * Reads rows back: out [B, n, G, D] of `which` (0 keys, 1 values).  Row i of sequence b is the token at place i, or with last != 0 at
+ * place len_b + len_bias - n + i; places before 0 or from len_b + len_bias (at most T_max) on give zeros.
+ */
+int b2kv_qcache_read(const b2kv_qcache* cache, int which, void* out, int n, int last, int len_bias, int32_t* dev_status, void* stream);
+
+/*
+ * Attention of the last m tokens of every sequence over its n_b = min(max(len_b + len_bias, 0), T_upper) tokens, T_upper <= T_max a bound that the
+ * host knows.  q and out are [B * m, H * D] (ld elements between rows), row b * m + i stands at place p = n_b - m + i; head h reads
+ * key / value head h / (H / G) and sees the tokens t <= p, with window > 0 only those with p - t < window:
+ *   score = cap(scale * q . k) - slopes[h] * (p - t),  cap(x) = softcap * tanh(x / softcap) where softcap > 0,  out = softmax(score) v.
+ * A row that sees nothing (an empty sequence, p < 0) is zeros.  slopes (fp32, H) may be NULL.  1 <= m <= B2KV_QCACHE_MAX_ROWS.
+ * `workspace` takes b2kv_qcache_attend_workspace_bytes bytes (16-byte aligned), needs no initialisation and carries nothing between
+ * calls; calls that may run at the same time need one each.
+ */
+#define B2KV_QCACHE_MAX_ROWS 64
+typedef struct b2kv_qcache_attend_args {
+    const void* q;
+    void* out;
+    const float* slopes;
+    int64_t ld_q, ld_out;
+    int32_t H, m, T_upper, len_bias, window;
+    float scale, softcap;
+} b2kv_qcache_attend_args;
+size_t b2kv_qcache_attend_workspace_bytes(const b2kv_qcache* cache, const b2kv_qcache_attend_args* args);
+int b2kv_qcache_attend(const b2kv_qcache* cache, const b2kv_qcache_attend_args* args, void* workspace, size_t workspace_bytes,
+                       int32_t* dev_status, void* stream);
+
+/*
  * Tuning hook for experiments (process-global and unsynchronised: set knobs before launching work, never while
  * another thread is inside a b2kv call): sets an integer knob by name ("decode_variant",
  * "decode_grid_per_sm", "decode_l2_keep", "decode_no_tensor_map", "decode_dynamic_chunks": small chunks of the

@@ -82,6 +82,20 @@ class GlaArgs(ctypes.Structure):
                 ("eps", _f)]
 
 
+class QCache(ctypes.Structure):
+    """``b2kv_qcache``."""
+
+    _fields_ = [("k_codes", _vp), ("v_codes", _vp), ("k_scales", _vp), ("v_scales", _vp), ("block_table", _vp), ("seq_lens", _vp)] + [
+        (name, ctypes.c_int32) for name in ("len", "B", "G", "D", "T_max", "max_blocks", "block_size", "n_blocks", "k_bits", "v_bits", "dtype")]
+
+
+class QCacheAttendArgs(ctypes.Structure):
+    """``b2kv_qcache_attend_args``."""
+
+    _fields_ = [("q", _vp), ("out", _vp), ("slopes", _vp), ("ld_q", _i64), ("ld_out", _i64), ("H", ctypes.c_int32), ("m", ctypes.c_int32),
+                ("T_upper", ctypes.c_int32), ("len_bias", ctypes.c_int32), ("window", ctypes.c_int32), ("scale", _f), ("softcap", _f)]
+
+
 # name -> (restype, argtypes); kept in the order of include/b2kv.h
 SIGNATURES = {
     "b2kv_strerror": (ctypes.c_char_p, [_i]),
@@ -148,6 +162,11 @@ SIGNATURES = {
     "b2kv_route": (_i, [_vp, _i64, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "b2kv_moe_plan": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i64, _vp, _i64, _i, _i, _vp]),
     "b2kv_moe_combine": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "b2kv_qcache_scale_row": (_i, [_i]),
+    "b2kv_qcache_write": (_i, [ctypes.POINTER(QCache), _vp, _i64, _vp, _i64, _i, _vp, _vp]),
+    "b2kv_qcache_read": (_i, [ctypes.POINTER(QCache), _i, _vp, _i, _i, _i, _vp, _vp]),
+    "b2kv_qcache_attend_workspace_bytes": (_sz, [ctypes.POINTER(QCache), ctypes.POINTER(QCacheAttendArgs)]),
+    "b2kv_qcache_attend": (_i, [ctypes.POINTER(QCache), ctypes.POINTER(QCacheAttendArgs), _vp, _sz, _vp, _vp]),
     "b2kv_tune": (_i, [ctypes.c_char_p, _i]),
 }
 
@@ -225,6 +244,9 @@ lib = _load()
 _LINEAR_ARGS = struct.Struct("5P5q" + "P2q2i" * MAX_SEGMENTS + "8if4x")
 _LINEAR_OPTIONS = struct.Struct("P2i")
 assert _LINEAR_ARGS.size == ctypes.sizeof(LinearArgs) and _LINEAR_OPTIONS.size == ctypes.sizeof(LinearOptions)
+_QCACHE = struct.Struct("6P11i4x")
+_QCACHE_ATTEND_ARGS = struct.Struct("3P2q5i2f4x")
+assert _QCACHE.size == ctypes.sizeof(QCache) and _QCACHE_ATTEND_ARGS.size == ctypes.sizeof(QCacheAttendArgs)
 _NO_SEGMENT = (0, 0, 0, 0, 0)
 
 
@@ -245,6 +267,16 @@ def linear_args(x, w, residual, bias, group_rows, ld_x, group_x, ld_w, group_w, 
 def linear_options(group_x_rows: int, x_rows: int, flags: int):
     """``b2kv_linear_options`` for ``lib``."""
     return _structure(LinearOptions, _LINEAR_OPTIONS.pack(group_x_rows, x_rows, flags))
+
+
+def qcache(*fields):
+    """``b2kv_qcache`` for ``lib``; the fields in order, pointers as integers (0: none)."""
+    return _structure(QCache, _QCACHE.pack(*fields))
+
+
+def qcache_attend_args(*fields):
+    """``b2kv_qcache_attend_args`` for ``lib``, likewise."""
+    return _structure(QCacheAttendArgs, _QCACHE_ATTEND_ARGS.pack(*fields))
 
 
 def check(status: int) -> None:

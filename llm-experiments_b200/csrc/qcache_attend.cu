@@ -1,0 +1,85 @@
+// Attention over a quantised cache: checks, how the work is cut, and which instance runs.
+#include "qcache_attend.cuh"
+
+#include <math.h>
+
+#include <algorithm>
+
+namespace b2kv {
+namespace qcache {
+namespace {
+
+int check_attend(const b2kv_qcache* c, const b2kv_qcache_attend_args* a) {
+    const int rc = check(c);
+    if (rc != B2KV_OK) return rc;
+    if (a == nullptr || !a->q || !a->out) return B2KV_ERR_BAD_ARG;
+    if (a->H <= 0 || a->H % c->G != 0 || a->m <= 0 || a->T_upper < 0 || a->T_upper > c->T_max || a->window < 0) return B2KV_ERR_BAD_ARG;
+    if (a->m > B2KV_QCACHE_MAX_ROWS) return B2KV_ERR_UNSUPPORTED;
+    if (!isfinite(a->scale) || !(a->softcap >= 0.0f) || !isfinite(a->softcap)) return B2KV_ERR_BAD_ARG;
+    const int64_t cols = static_cast<int64_t>(a->H) * c->D;
+    if (a->ld_q < cols || a->ld_out < cols) return B2KV_ERR_BAD_ARG;
+    const int es = elt_bytes(c->dtype);
+    if (!aligned16(a->q) || !aligned16(a->out) || !stride_ok(a->ld_q, es) || !stride_ok(a->ld_out, es)) return B2KV_ERR_ALIGN;
+    return B2KV_OK;
+}
+
+bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& plan) {
+    const int columns = a.m * (a.H / c.G);
+    plan.cols = c.dtype == B2KV_DTYPE_F32 || columns <= 8 ? 8 : 16;
+    plan.col_tiles = (columns + plan.cols - 1) / plan.cols;
+    plan.pairs = static_cast<int64_t>(c.B) * c.G * plan.col_tiles;
+    if (plan.pairs > 0x7fffffff) return false;
+    const int most = a.window > 0 ? std::min(a.T_upper, a.window + a.m - 1) : a.T_upper;
+    plan.share = 1024;
+    plan.n_splits = std::max(1, (most + plan.share - 1) / plan.share);
+    if (plan.n_splits > 65535) return false;
+    const size_t slots = plan.n_splits > 1 ? static_cast<size_t>(plan.pairs) * plan.n_splits : 0;
+    plan.workspace = slots * plan.cols * (c.D + 1) * sizeof(float);
+    return true;
+}
+
+}  // namespace
+}  // namespace qcache
+}  // namespace b2kv
+
+using namespace b2kv;
+
+extern "C" {
+
+size_t b2kv_qcache_attend_workspace_bytes(const b2kv_qcache* cache, const b2kv_qcache_attend_args* args) {
+    qcache::Plan plan;
+    return qcache::check_attend(cache, args) == B2KV_OK && qcache::make_plan(*cache, *args, plan) ? plan.workspace : 0;
+}
+
+int b2kv_qcache_attend(const b2kv_qcache* cache, const b2kv_qcache_attend_args* args, void* workspace, size_t workspace_bytes, int32_t* dev_status,
+                       void* stream) {
+    using namespace qcache;
+    const int rc = check_attend(cache, args);
+    if (rc != B2KV_OK) return rc;
+    const b2kv_qcache& c = *cache;
+    const b2kv_qcache_attend_args& a = *args;
+    Plan plan;
+    if (!make_plan(c, a, plan)) return B2KV_ERR_UNSUPPORTED;
+    if (plan.workspace > 0) {
+        if (workspace == nullptr || workspace_bytes < plan.workspace) return B2KV_ERR_WORKSPACE;
+        if (!aligned16(workspace)) return B2KV_ERR_ALIGN;
+    }
+    AttendParams p{};
+    p.c = c;
+    p.q = a.q, p.out = a.out, p.slopes = a.slopes, p.dev_status = dev_status;
+    p.ld_q = a.ld_q, p.ld_out = a.ld_out;
+    p.R = a.H / c.G, p.m = a.m, p.col_tiles = plan.col_tiles, p.T_upper = a.T_upper, p.len_bias = a.len_bias, p.window = a.window;
+    p.n_splits = plan.n_splits, p.share = plan.share;
+    p.scale = a.scale, p.softcap = a.softcap;
+    p.ws_o = static_cast<float*>(workspace);
+    p.ws_lse = p.ws_o + static_cast<size_t>(plan.pairs) * plan.n_splits * plan.cols * c.D;
+    switch (c.D) {
+        case 32: return attend_32(p, plan, stream);
+        case 64: return attend_64(p, plan, stream);
+        case 96: return attend_96(p, plan, stream);
+        case 128: return attend_128(p, plan, stream);
+        default: return attend_256(p, plan, stream);
+    }
+}
+
+}  // extern "C"

@@ -33,10 +33,18 @@ from .kv_cache import (
 from .latent import latent_append, latent_decode, latent_prefill
 from .moe import moe_feed_forward
 from .projection import linear, matmul, qkv_project_append
+from .quant_cache import (
+    attention_with_quant_cache,
+    quant_cache_create,
+    quant_cache_gather,
+    quant_cache_reset,
+    quant_cache_set_lengths,
+    quant_cache_update,
+)
 from .recurrent import gated_linear_attention
 from .registry import architectures, load_model
 from .step_tail import argmax, embedding, embedding_rows, extract_last_tokens, layernorm, layernorm_rows, rms_norm, softmax
-from .types import GPUBuffer1D, GPUBuffer2D, GPUConfig, GPUContext, KVCache, KVCacheConfig, KVCacheLayer
+from .types import GPUBuffer1D, GPUBuffer2D, GPUConfig, GPUContext, KVCache, KVCacheConfig, KVCacheLayer, QuantKVCache, QuantKVCacheConfig
 
 __all__ = [
     "GPUBuffer1D", "GPUBuffer2D", "GPUConfig", "GPUContext", "KVCache", "KVCacheConfig", "KVCacheLayer",
@@ -54,5 +62,7 @@ __all__ = [
     # extensions: building blocks of decoders with a 32-bit residual stream, and models from folders
     "linear", "embedding_rows", "rms_norm", "latent_append", "latent_decode", "latent_prefill", "moe_feed_forward",
     "layernorm_rows", "gqa_append", "gqa_decode", "gqa_prefill", "gated_linear_attention",
+    "QuantKVCache", "QuantKVCacheConfig", "quant_cache_create", "quant_cache_reset", "quant_cache_set_lengths", "quant_cache_update",
+    "quant_cache_gather", "attention_with_quant_cache",
     "architectures", "load_model",
 ]

@@ -165,3 +165,45 @@ class KVCacheConfig:
     block_size: int = 0  # > 0: paged cache with blocks of this many tokens
     n_blocks: int = 0  # pool size in blocks (paged)
     v_head_dim: int = 0  # > 0: V rows are this wide (latent layers; contiguous caches only)
+
+
+@dataclass
+class QuantKVCacheLayer:
+    """Codes and scales of one layer's keys and values, a row per token of a key / value head (``b2kv_qcache`` in include/b2kv.h)."""
+
+    k_codes: GPUBuffer2D
+    v_codes: GPUBuffer2D
+    k_scales: GPUBuffer2D
+    v_scales: GPUBuffer2D
+
+
+@dataclass
+class QuantKVCache:
+    layers: List[QuantKVCacheLayer]
+    batch_size: int
+    max_seq_len: int
+    current_len: int  # host-side length; with seq_lens set it is the upper bound of all lengths
+    n_kv_heads: int
+    head_dim: int
+    dtype: torch.dtype  # of the rows written, read back and attended with
+    k_bits: int
+    v_bits: int
+    seq_lens: Optional[torch.Tensor] = None  # int32[B] on the device: per-sequence lengths
+    block_table: Optional[torch.Tensor] = None  # int32[B, max_blocks] on the device
+    block_size: int = 0
+    n_blocks: int = 0
+
+
+@dataclass
+class QuantKVCacheConfig:
+    batch_size: int
+    max_seq_len: int
+    n_layers: int
+    n_kv_heads: int
+    head_dim: int  # 32, 64, 96, 128 or 256
+    dtype: torch.dtype = torch.bfloat16
+    k_bits: int = 4  # (k_bits, v_bits): (4, 4), (8, 4) or (8, 8)
+    v_bits: int = 4
+    ragged: bool = False  # keep per-sequence lengths on the device
+    block_size: int = 0  # > 0: paged cache with blocks of this many tokens
+    n_blocks: int = 0  # pool size in blocks (paged)

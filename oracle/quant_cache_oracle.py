@@ -1,0 +1,79 @@
+"""CPU oracle (numpy, float64) of the quantised key / value cache: what a cache holds for rows, and attention over it.  TEST
+INFRASTRUCTURE ONLY.  The reference has no such cache (simple-llm/src/gpu/gpu_kv_cache.py:66-78 is fp32); this is the definition."""
+from __future__ import annotations
+
+import numpy as np
+
+GROUP = 32
+
+
+def to_bf16(x: np.ndarray) -> np.ndarray:
+    """float64 rounded once to the nearest bfloat16 (ties to even), as float64."""
+    x = np.asarray(x, dtype=np.float64)
+    out = x.copy()
+    some = np.isfinite(x) & (x != 0)
+    m, e = np.frexp(x[some])                       # x = m * 2^e, 0.5 <= |m| < 1
+    step = np.ldexp(1.0, np.maximum(e - 8, -133))  # 8 bits, subnormals down to 2^-133
+    out[some] = np.rint(x[some] / step) * step
+    return np.where(np.abs(out) >= 2.0 ** 128, np.copysign(np.inf, out), out)
+
+
+def quantise(x: np.ndarray, bits: int):
+    """(codes, scales) of rows [..., D]: codes [..., D] whole numbers, scales [..., D / 32]."""
+    top = 7 if bits == 4 else 127
+    g = np.asarray(x, dtype=np.float64).reshape(*x.shape[:-1], -1, GROUP)
+    most = np.abs(g).max(-1)
+    scales = np.where(np.isfinite(most), to_bf16(np.where(np.isfinite(most), most, 0) / top), np.nan)
+    s = scales[..., None]
+    with np.errstate(all="ignore"):
+        codes = np.where(s > 0, np.clip(np.rint(g / s), -top, top), 0)
+    return codes.reshape(x.shape), scales
+
+
+def held(x: np.ndarray, bits: int) -> np.ndarray:
+    codes, scales = quantise(x, bits)
+    return codes * np.repeat(scales, GROUP, axis=-1)
+
+
+def attention(q, k, v, scale, softcap=0.0, window=0, slopes=None):
+    """One sequence.  q [m, H, D], k and v [n, G, D] (what the cache holds), query i at place n - m + i -> (out [m, H, D], the mean magnitude
+    sum_t w_t |v_t| of what was averaged, and per query and head scale * sum_d |q_d| max |k| over d's group, which bounds what a score was made of)."""
+    m, H, D = q.shape
+    n, G = k.shape[:2]
+    out, mean, size = np.zeros((m, H, D)), np.zeros((m, H, D)), np.zeros((m, H, 1))
+    for i in range(m):
+        p = n - m + i
+        first = max(0, p + 1 - window) if window else 0
+        if p < 0:
+            continue
+        t = np.arange(first, p + 1)
+        for h in range(H):
+            kk, vv = k[t, h // (H // G)], v[t, h // (H // G)]
+            s = kk @ q[i, h] * scale
+            most = np.nan_to_num(np.abs(kk)).max(0).reshape(-1, min(GROUP, D)).max(-1)  # of a group: its codes are steps of that
+            size[i, h] = np.repeat(most, min(GROUP, D)) @ np.abs(q[i, h]) * abs(scale)
+            if softcap:
+                s = softcap * np.tanh(s / softcap)
+            if slopes is not None:
+                s = s - slopes[h] * (p - t)
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            out[i, h], mean[i, h] = w @ vv, w @ np.abs(vv)
+    return out, mean, size
+
+
+def tolerance(out, mean, size, n, dtype: str, extra: float = 0.0, largest: float = 0.0):
+    """How far an output element may be off, from the formulas' roundings:
+    - the output's own rounding: half a step, 2^-8 (bfloat16) or 2^-24 of the value;
+    - a probability times a value scale is held in 11 (fp32: 22) bits: 2^-11 (2^-21) of the mean magnitude;
+    - a score is a sum in fp32 of products of whole codes up to twice (4 bits: 15 / 7) what they stand for: 2^-20 of the sum of magnitudes
+      `size` twice over, which scales probabilities above and below the line;
+    - the sums over n tokens in fp32, 16 tokens at a time: 2^-23 of the mean magnitude each, and as much for their reunion.
+    `extra` is an absolute error of scores beyond that (bias, cap).
+    - fp16 numbers below 2^-14 lie 2^-24 apart.  A probability (relative to a score that was seen, so their sum is at least 1) times a
+      value scale s is held as a multiple p s / 2^(E - 6), 2^E <= the largest scale: off by up to half of 2^-24 * 2^(E - 6) = 2^-31 2^E beyond the
+      relative error, times a code up to L, over a sum of at least 1.  L 2^E <= `largest`, the largest magnitude held: 2^-31 * largest per token.
+      (It shows where one token has nearly all the weight and a code of zero, and what is left is below 2^-31 of the values.)"""
+    half, held_in = (2.0 ** -8, 2.0 ** -11) if dtype == "bf16" else (2.0 ** -24, 2.0 ** -21)
+    score = 2.0 ** -20 * 2.2 * size + extra
+    return half * np.abs(out) + (held_in + 2 * score + 2.0 ** -23 * (n / 16 + 32)) * mean + n * 2.0 ** -31 * largest
