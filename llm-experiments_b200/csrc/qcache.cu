@@ -86,7 +86,7 @@ __device__ __forceinline__ uint2 quantise(const float (&f)[8], __nv_bfloat16& sc
 template <int BITS, bool kValues>
 __device__ __forceinline__ void store_codes(uint8_t* row, int groups, int u, int o, uint2 w) {
     if (!kValues && BITS == 4) {
-        reinterpret_cast<uint32_t*>(row)[o * groups + u] = w.x;
+        reinterpret_cast<uint32_t*>(row)[o * groups + u] = __funnelshift_l(w.x, w.x, 2);
     } else if (!kValues) {
         reinterpret_cast<uint2*>(row)[o * groups + u] = w;
     } else if (BITS == 4) {
@@ -99,7 +99,10 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int groups, int u, int
 }
 template <int BITS, bool kValues>
 __device__ __forceinline__ uint2 load_codes(const uint8_t* row, int groups, int u, int o) {
-    if (!kValues && BITS == 4) return make_uint2(reinterpret_cast<const uint32_t*>(row)[o * groups + u], 0);
+    if (!kValues && BITS == 4) {
+        const uint32_t w = reinterpret_cast<const uint32_t*>(row)[o * groups + u];
+        return make_uint2(__funnelshift_r(w, w, 2), 0);
+    }
     if (!kValues) return reinterpret_cast<const uint2*>(row)[o * groups + u];
     if (BITS == 4) {
         const uint32_t a = reinterpret_cast<const uint16_t*>(row)[2 * o * groups + u];

@@ -30,11 +30,18 @@ bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& pla
     plan.pairs = static_cast<int64_t>(c.B) * c.G * plan.col_tiles;
     if (plan.pairs > 0x7fffffff) return false;
     const int most = a.window > 0 ? std::min(a.T_upper, a.window + a.m - 1) : a.T_upper;
-    plan.share = 1024;
-    plan.n_splits = std::max(1, (most + plan.share - 1) / plan.share);
-    if (plan.n_splits > 65535) return false;
-    const size_t slots = plan.n_splits > 1 ? static_cast<size_t>(plan.pairs) * plan.n_splits : 0;
-    plan.workspace = slots * plan.cols * (c.D + 1) * sizeof(float);
+    // CTAs that run at the same time: two per SM for one tile of columns and heads up to 128, else one (Ring).
+    const int at_once = device_sm_count() * (c.dtype != B2KV_DTYPE_F32 && plan.cols == 8 && c.D <= 128 ? 2 : 1);
+    plan.cluster = 1;
+    while (plan.cluster < 8 && plan.pairs * plan.cluster * 2 <= at_once && most > plan.cluster * 256) plan.cluster *= 2;
+    plan.workspace = 0;
+    if (static_cast<int64_t>(most) * plan.pairs > static_cast<int64_t>(at_once) * 1024) {
+        plan.cluster = 0;
+        plan.ctas = at_once;
+        plan.workspace = static_cast<size_t>(at_once) * 2 * plan.cols * (c.D + 1) * sizeof(float);
+    } else {
+        plan.ctas = static_cast<int>(plan.pairs) * plan.cluster;
+    }
     return true;
 }
 
@@ -69,10 +76,10 @@ int b2kv_qcache_attend(const b2kv_qcache* cache, const b2kv_qcache_attend_args* 
     p.q = a.q, p.out = a.out, p.slopes = a.slopes, p.dev_status = dev_status;
     p.ld_q = a.ld_q, p.ld_out = a.ld_out;
     p.R = a.H / c.G, p.m = a.m, p.col_tiles = plan.col_tiles, p.T_upper = a.T_upper, p.len_bias = a.len_bias, p.window = a.window;
-    p.n_splits = plan.n_splits, p.share = plan.share;
+    p.cluster = plan.cluster;
     p.scale = a.scale, p.softcap = a.softcap;
     p.ws_o = static_cast<float*>(workspace);
-    p.ws_lse = p.ws_o + static_cast<size_t>(plan.pairs) * plan.n_splits * plan.cols * c.D;
+    p.ws_lse = p.ws_o + static_cast<size_t>(plan.ctas) * 2 * plan.cols * c.D;
     switch (c.D) {
         case 32: return attend_32(p, plan, stream);
         case 64: return attend_64(p, plan, stream);

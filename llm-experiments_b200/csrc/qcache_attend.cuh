@@ -4,27 +4,31 @@
 // arithmetic has to be hidden behind 23 bytes per clock and SM, and with 4 bits 46 elements per clock have to be widened.  Plain
 // fp32 arithmetic cannot (128 FMAs per clock and SM, one per element and query head); the tensor cores can, if widening is cheap:
 //
-//   * Codes become fp16 numbers by masking alone: a code c in the low bits of a 16-bit half is the fp16 subnormal c * 2^-24, one in
-//     the next four bits is c * 2^-20, and tensor cores and half-precision adds take subnormals at full speed.  Two codes per
-//     instruction, no conversion.
+//   * Codes become fp16 numbers by masking: a key's code c in bits 2 .. 5 or 6 .. 9 of a 16-bit half is the fp16 subnormal c * 2^-22 or c * 2^-18, two
+//     codes per instruction, and tensor cores take subnormals at full speed.  They add products by the exponents as they stand, so
+//     that a number whose first bit is k places below the tenth loses k bits of the sum: at most 4 here, which is why the keys' words are kept
+//     turned by two bits (bits 0 .. 3 and 4 .. 7 lost 7 and 3).  fp32 queries, and values, have the mask's result put behind the exponent of 1024
+//     by the same instruction and the centre taken off by a second one.
 //   * Both products have the cache's rows as the operand of many rows: S[token, column] = K q (16 tokens by 8 columns per MMA, m16n8k16)
 //     and O[element, column] += V^T P.  A column is one (new token, query head) pair of the key / value head.  The cache's
 //     layout gives a lane the codes that it needs as one piece, the query is permuted to match, and P goes from the accumulator's
 //     layout to the operand's by an 8 x 8 transpose within the warp.  The rows go through tcgen05 only if they were first widened into
 //     shared memory at 16 bits per element, which is four times the traffic of reading them; as register operands they are widened in place.
-//   * Key codes are taken as stored (c + 8, c + 128); the accumulator of a group starts at minus 8 (128) times the group's sum of the query.
-//     A group's sum is multiplied by its key scale in fp32.  Value codes are centred (one half-precision add per two), because over thousands
-//     of tokens the sum of uncentred ones grows far beyond what is left when the centre is taken off.
+//   * Uncentred key codes (c + 8, c + 128): the accumulator of a group starts at minus 8 (128) times the group's sum of the query.  A group's sum is
+//     multiplied by its key scale in fp32.  Value codes are centred, because over thousands of tokens the sum of uncentred ones grows far beyond
+//     what is left when the centre is taken off.
 //   * A probability times a value scale is rounded to fp16 (11 bits; the output has 8).  To keep it in range whatever the scales
 //     are, it is taken relative to the largest scale's exponent so far, and the accumulators are rescaled when that grows: below 2^15
 //     always, and full precision down to scales 2^20 below the largest.
-//   * fp32 queries and probabilities are sums of two fp16 numbers (22 bits), in columns of their own.
+//   * fp32 queries and probabilities are sums of two fp16 numbers (22 bits), in columns of their own, and only 16 tokens' products are
+//     added up in the tensor core, whose sums are cut off and not rounded.
 //   * Softmax: scores in the log2 domain, reference maxima that move only when a score has outgrown its reference by more than 2^8 (one vote
-//     per 32 tokens), sums per lane until the end, all in fp32.
+//     per stage), sums per lane until the end, all in fp32.
 #pragma once
 
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "qcache.cuh"
@@ -37,18 +41,17 @@ struct AttendParams {
     const void* q;
     void* out;
     const float* slopes;
-    float* ws_o;   // [slots, kCols, D]: normalised
-    float* ws_lse; // [slots, kCols]: log2 of the sum of exponentials
+    float* ws_o;    // [2 * CTAs, kCols, D]: what a CTA has of its first (sequence, head) and of its last, normalised
+    float* ws_lse;  // [2 * CTAs, kCols]: log2 of the sum of exponentials
     int32_t* dev_status;
     int64_t ld_q, ld_out;
     int R, m, col_tiles, T_upper, len_bias, window;
-    int n_splits, share;  // pieces of a (sequence, head) and tokens in one
+    int cluster;      // > 0: a cluster of this many CTAs per (sequence, head, column tile); 0: all tokens laid end to end and cut into gridDim.x pieces
     float scale, softcap;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_huge_valf();
-constexpr int kStageTokens = 32;
 constexpr int kScaleExpMin = 17;  // (biased) smaller exponents of value scales are taken for this one: 2^-110
 
 __device__ __forceinline__ float ex2(float x) {
@@ -125,20 +128,43 @@ struct Words {
     }
 };
 
+// The first token that any query of a sequence of n tokens sees.
+__device__ __forceinline__ int first_seen(const AttendParams& p, int n) { return p.window > 0 ? max(n - p.m + 1 - p.window, 0) : 0; }
+
+// What a warp's ring holds: stages of 16 or 32 tokens, as many as fit with two CTAs per SM (one, where the registers leave room for no more).
+template <int NG, int KB, int VB, int NT>
+struct Ring {
+    static constexpr int kWarps = 8;
+    static constexpr int kCtas = NT == 1 && NG <= 4 ? 2 : 1;
+    static constexpr int kToken = NG * 4 * (KB + VB) + 4 * scale_row(NG);
+    static constexpr int kRoom = (kCtas == 2 ? 113 : 225) * 1024 / kWarps;
+    static constexpr int kTokens = 3 * 32 * kToken <= kRoom ? 32 : 16;
+    static constexpr int kFit = kRoom / (kTokens * kToken);
+    static constexpr int kStages = kFit > 6 ? 6 : kFit;
+    static_assert(kStages >= 3, "");
+};
+
 // T: type of queries and outputs; NG groups of 32 elements; KB, VB bits; NT tiles of 8 columns (fp32: 2, the second for what fp16 leaves
-// of the first); WARPS per CTA, STAGES of 32 tokens in each warp's ring.
-template <typename T, int NG, int KB, int VB, int NT, int WARPS, int STAGES>
+// of the first).
+template <typename T, int NG, int KB, int VB, int NT>
 struct Attend {
+    using R = Ring<NG, KB, VB, NT>;
+    static constexpr int WARPS = R::kWarps, STAGES = R::kStages, kTok = R::kTokens, MT = kTok / 16;
     static constexpr bool kF32 = std::is_same<T, float>::value;
     static_assert(!kF32 || NT == 2, "");
     static constexpr int D = NG * kGroup, kCols = kF32 ? 8 : 8 * NT, kThreads = WARPS * 32;
     static constexpr int kKRow = D * KB / 8, kVRow = D * VB / 8, kSRow = scale_row(NG) * 2;
-    static constexpr int kKBytes = kStageTokens * kKRow, kVBytes = kStageTokens * kVRow, kSBytes = kStageTokens * kSRow;
+    static constexpr int kKBytes = kTok * kKRow, kVBytes = kTok * kVRow, kSBytes = kTok * kSRow;
     static constexpr int kStage = (kKBytes + kVBytes + 2 * kSBytes + 15) / 16 * 16;
     static constexpr int kRing = WARPS * STAGES * kStage;
-    static constexpr int kMerge = WARPS * kCols * (D + 2) * 4;
-    static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+    // Results are put together in a stage of each warp's ring, as many columns at a time as go into one.
+    static constexpr int kRoundCols = kCols * D * 4 <= kStage ? kCols : kCols * D * 2 <= kStage ? kCols / 2 : kCols / 4;
+    static constexpr int kRounds = kCols / kRoundCols;
+    static_assert(kRoundCols * D * 4 <= kStage && kRoundCols % 2 == 0, "");
+    static constexpr int kMl = WARPS * kCols * 2 * 4;
+    static constexpr int kSmem = kRing + kMl + WARPS * 4;
     static constexpr int kKOff = KB == 4 ? 8 : 128;  // what is added to a key's code
+    static constexpr float kKeyUnit = (KB == 4 ? 4.0f : 1.0f) * (kF32 ? 1.0f : 0x1p-24f);
 
     // Where 16-byte piece ch of row r lies in a stage: moved about so that the lanes that read together meet different banks.
     __device__ static __forceinline__ int k_place(int r, int ch) {
@@ -205,8 +231,8 @@ struct Attend {
             // q = qn * 2^e with the largest |qn| in [2^14, 2^15): exact, and no fp16 overflow
             const int biased = min(max(__float_as_int(most) >> 23, 27), 254);
             const float down = __int_as_float((254 + 14 - biased) << 23);
-            // 2^(e - 14 + 24) * scale, the 24 for the codes' 2^-24
-            const float f = p.scale * kLog2e * 1024.0f * __int_as_float(biased << 23);
+            // scale * 2^(e - 14) over what a code of one is in the product
+            const float f = p.scale * kLog2e * 0x1p-14f / kKeyUnit * __int_as_float(biased << 23);
             float part[2][NG];
 #pragma unroll
             for (int u = 0; u < NG; ++u) {
@@ -239,7 +265,7 @@ struct Attend {
                     float s = part[l][u];
                     s += __shfl_xor_sync(~0u, s, 1);
                     s += __shfl_xor_sync(~0u, s, 2);
-                    s *= -static_cast<float>(kKOff) * 0x1p-24f;
+                    s *= kF32 ? 0.0f : -static_cast<float>(kKOff) * kKeyUnit;
                     w.off[nt + l][u][0] = __shfl_sync(~0u, s, from0);
                     w.off[nt + l][u][1] = __shfl_sync(~0u, s, from1);
                 }
@@ -273,53 +299,83 @@ struct Attend {
         w.scale_exp = kScaleExpMin;
     }
 
-    // Starts the copies of tokens t0 .. t0 + 31 (below t1) of a sequence and head; a bit for each token that is there.
-    __device__ static __forceinline__ uint32_t issue(const AttendParams& p, uint32_t stage, int b, int g, int t0, int t1) {
-        const int lane = threadIdx.x & 31, t = t0 + lane;
-        const int64_t row = t < t1 ? row_of(p.c, b, g, t, p.dev_status) : -1;
+    // Where a lane's token of a tile lies: its row, -1 where there is none or no query sees it.
+    __device__ static __forceinline__ int64_t find(const AttendParams& p, int b, int g, int t0, int n) {
+        const int lane = threadIdx.x & 31, t = t0 + (lane & (kTok - 1));
+        return t < n && t >= first_seen(p, n) ? row_of(p.c, b, g, t, p.dev_status) : -1;
+    }
+
+    // Starts the copies of a tile whose rows `find` gave (zeros where there is none); a bit for each token that is there.
+    __device__ static __forceinline__ uint32_t issue(const AttendParams& p, uint32_t stage, int64_t row) {
+        const int lane = threadIdx.x & 31;
         const uint32_t there = __ballot_sync(~0u, row >= 0);
         const int64_t at = row >= 0 ? row : 0;
         const uint32_t ks = stage + kKBytes + kVBytes;
-        copy_small<kSRow>(ks + lane * kSRow, static_cast<const uint8_t*>(p.c.k_scales) + at * kSRow, row >= 0);
-        copy_small<kSRow>(ks + kSBytes + lane * kSRow, static_cast<const uint8_t*>(p.c.v_scales) + at * kSRow, row >= 0);
-        copy_rows<kKRow>(stage, static_cast<const uint8_t*>(p.c.k_codes), at, there, [](int r, int ch) { return k_place(r, ch); });
-        copy_rows<kVRow>(stage + kKBytes, static_cast<const uint8_t*>(p.c.v_codes), at, there, [](int r, int ch) { return v_place(r, ch); });
+        if (kTok == 32 || lane < kTok) {
+            copy_small<kSRow>(ks + lane * kSRow, static_cast<const uint8_t*>(p.c.k_scales) + at * kSRow, row >= 0);
+            copy_small<kSRow>(ks + kSBytes + lane * kSRow, static_cast<const uint8_t*>(p.c.v_scales) + at * kSRow, row >= 0);
+        }
+        copy_rows<kKRow>(p, stage, static_cast<const uint8_t*>(p.c.k_codes), at, there, [](int r, int ch) { return k_place(r, ch); });
+        copy_rows<kVRow>(p, stage + kKBytes, static_cast<const uint8_t*>(p.c.v_codes), at, there, [](int r, int ch) { return v_place(r, ch); });
         return there;
     }
     template <int ROW, typename F>
-    __device__ static __forceinline__ void copy_rows(uint32_t dst, const uint8_t* src, int64_t mine, uint32_t there, F&& place) {
-        constexpr int kCh = ROW / 16;
+    __device__ static __forceinline__ void copy_rows(const AttendParams& p, uint32_t dst, const uint8_t* src, int64_t mine, uint32_t there, F&& place) {
+        constexpr int kCh = ROW / 16, kPieces = kCh * kTok, kPer = (kPieces + 31) / 32;
         const int lane = threadIdx.x & 31;
+        if (p.c.block_table == nullptr) {  // rows follow one another
+            const int some = there != 0 ? __ffs(there) - 1 : 0;  // (tokens before the first one seen have no row here)
+            const uint8_t* const from = src + (__shfl_sync(~0u, mine, some) - some) * ROW + lane * 16;
 #pragma unroll
-        for (int i = 0; i < kCh; ++i) {
-            const int idx = i * 32 + lane, r = idx / kCh, ch = idx - r * kCh;
-            const int64_t row = __shfl_sync(~0u, mine, r);
-            copy16(dst + place(r, ch), src + row * ROW + ch * 16, (there >> r) & 1u);
+            for (int i = 0; i < kPer; ++i) {
+                const int idx = i * 32 + lane, r = idx / kCh, ch = idx - r * kCh;
+                if (kPieces % 32 == 0 || idx < kPieces) {
+                    const bool is = (there >> r) & 1u;
+                    copy16(dst + place(r, ch), is ? from + i * 512 : src, is);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int idx = i * 32 + lane, r = idx / kCh, ch = idx - r * kCh;
+                const int64_t row = __shfl_sync(~0u, mine, r & 31);
+                if (kPieces % 32 == 0 || idx < kPieces) copy16(dst + place(r, ch), src + row * ROW + ch * 16, (there >> r) & 1u);
+            }
         }
     }
 
-    // Two rows' codes of half a group as operand pieces (a0 and a1 of two rows; a2 and a3 likewise).
+    // Codes in bits 0 .. 3 or 4 .. 7 of 16-bit halves, or in bytes, as centred fp16 numbers (the higher ones times 16).
+    __device__ static __forceinline__ uint32_t centred4(uint32_t x, bool high) {
+        return high ? half_sub((x & 0x00f000f0u) | 0x64006400u, 0x64806480u) : half_sub((x & 0x000f000fu) | 0x64006400u, 0x64086408u);
+    }
+    __device__ static __forceinline__ uint32_t centred8(uint32_t x, int sel) { return half_sub(__byte_perm(x, 0x64646464u, sel), 0x64806480u); }
+
+    // A row's codes of half a group as operand pieces (a0 and a2, or a1 and a3).
     template <int STEP>
     __device__ static __forceinline__ void k_piece(const uint32_t* w, uint32_t& first, uint32_t& second) {
         if constexpr (KB == 4) {
-            const uint32_t x = STEP == 0 ? w[0] : w[0] >> 8;
-            first = x & 0x000f000fu;
-            second = x & 0x00f000f0u;
+            const uint32_t x = STEP == 0 ? w[0] : __funnelshift_r(w[0], w[0], 8);
+            first = x & 0x003c003cu;
+            second = x & 0x03c003c0u;
+            if constexpr (kF32) {
+                first = half_sub(first | 0x64006400u, 0x64206420u);    // 1024 + 4 c less 1024 + 32
+                second = half_sub(second | 0x64006400u, 0x66006600u);  // 1024 + 64 c less 1024 + 512
+            }
         } else {
-            first = __byte_perm(w[STEP], 0, 0x4140);
-            second = __byte_perm(w[STEP], 0, 0x4342);
+            first = kF32 ? centred8(w[STEP], 0x4140) : __byte_perm(w[STEP], 0, 0x4140);
+            second = kF32 ? centred8(w[STEP], 0x4342) : __byte_perm(w[STEP], 0, 0x4342);
         }
     }
 
-    // The 32 tokens of a stage.
+    // The tokens of a stage, t0 the first.
     __device__ static __forceinline__ void fold(const AttendParams& p, Warp& w, uint32_t stage, int t0, uint32_t there) {
         const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
         const uint32_t ks = stage + kKBytes + kVBytes, vs = ks + kSBytes, vc = stage + kKBytes;
         constexpr int kKPiece = NG * KB, kVPiece = NG * VB / 2;  // bytes of a row that a lane reads
         constexpr int NS = kF32 ? 1 : NT;                        // tiles of scores
-        float s[2][NS][4];
+        float s[MT][NS][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < MT; ++h) {
             const int r = h * 16 + gid;
             Words<kKPiece> k0, k1;
             load_k(k0, stage, r, tig);
@@ -361,7 +417,7 @@ struct Attend {
         if (p.softcap > 0.0f) {
             const float down = 1.0f / (p.softcap * kLog2e), up = p.softcap * kLog2e;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < MT; ++h)
 #pragma unroll
                 for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
@@ -369,7 +425,7 @@ struct Attend {
         }
         if (p.slopes != nullptr) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < MT; ++h)
 #pragma unroll
                 for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
@@ -377,11 +433,11 @@ struct Attend {
                         s[h][nt][e] -= w.slope[nt][e & 1] * static_cast<float>(w.lim[nt][e & 1] - 1 - (t0 + h * 16 + (e >> 1) * 8 + gid));
         }
         // Masks, where the stage has a token that some column does not see.
-        const bool masked = there != ~0u || t0 < w.all_lo || t0 + kStageTokens > w.all_lim;
+        const bool masked = there != ~0u || t0 < w.all_lo || t0 + kTok > w.all_lim;
         uint32_t hidden = 0;  // a bit per score of this lane
         if (masked) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < MT; ++h)
 #pragma unroll
                 for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
@@ -389,14 +445,14 @@ struct Attend {
                         const int r = h * 16 + (e >> 1) * 8 + gid, t = t0 + r;
                         if (!((there >> r) & 1u) || t < w.lo[nt][e & 1] || t >= w.lim[nt][e & 1]) {
                             s[h][nt][e] = kNegInf;
-                            hidden |= 1u << (h * 8 + nt * 4 + e);
+                            hidden |= 1u << ((h * NS + nt) * 4 + e);
                         }
                     }
         }
         // The references, where a score has outgrown its own by more than 2^8.
         bool grown = false;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < MT; ++h)
 #pragma unroll
             for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
@@ -406,7 +462,9 @@ struct Attend {
             for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float top = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+                    float top = kNegInf;
+#pragma unroll
+                    for (int h = 0; h < MT; ++h) top = fmaxf(top, fmaxf(s[h][nt][e], s[h][nt][e + 2]));
 #pragma unroll
                     for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
                     top = fmaxf(top, w.top[nt][e]);
@@ -425,7 +483,7 @@ struct Attend {
             for (int e = 0; e < 2; ++e) {
                 const float top = w.top[nt][e] == kNegInf ? 0.0f : w.top[nt][e];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < MT; ++h) {
                     s[h][nt][e] = ex2(s[h][nt][e] - top);
                     s[h][nt][e + 2] = ex2(s[h][nt][e + 2] - top);
                     w.sum[nt][e] += s[h][nt][e] + s[h][nt][e + 2];
@@ -434,7 +492,7 @@ struct Attend {
         // The largest exponent of a value scale (NaN groups have none).
         {
             Words<kSRow> mine;
-            mine.load(vs + lane * kSRow);
+            mine.load(vs + (lane & (kTok - 1)) * kSRow);
             uint32_t most = 0;
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
@@ -455,7 +513,7 @@ struct Attend {
         }
         const float vf = __int_as_float((260 - w.scale_exp) << 23);  // 2^(6 - exponent)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < MT; ++h) {
             const int r = h * 16 + gid;
             Words<kSRow> s0, s1;
             s0.load(vs + r * kSRow);
@@ -473,7 +531,7 @@ struct Attend {
                     float x[4] = {s[h][nt][0] * f0, s[h][nt][1] * f0, s[h][nt][2] * f1, s[h][nt][3] * f1};
                     if (masked) {  // (0 times a NaN scale)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = (hidden >> (h * 8 + nt * 4 + e)) & 1u ? 0.0f : x[e];
+                        for (int e = 0; e < 4; ++e) x[e] = (hidden >> ((h * NS + nt) * 4 + e)) & 1u ? 0.0f : x[e];
                     }
                     const uint32_t p0 = pack_half(x[0], x[1]), p1 = pack_half(x[2], x[3]);
                     b[nt][0] = transpose8x8(p0);
@@ -487,10 +545,18 @@ struct Attend {
                 uint32_t a[2][4];
                 v_pieces(v, u, a);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma(w.o[nt][2 * u], a[0][0], a[0][1], a[0][2], a[0][3], b[nt][0], b[nt][1]);
-                    mma(w.o[nt][2 * u + 1], a[1][0], a[1][1], a[1][2], a[1][3], b[nt][0], b[nt][1]);
-                }
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        if constexpr (kF32) {
+                            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma(d, a[j][0], a[j][1], a[j][2], a[j][3], b[nt][0], b[nt][1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w.o[nt][2 * u + j][e] += d[e];
+                        } else {
+                            mma(w.o[nt][2 * u + j], a[j][0], a[j][1], a[j][2], a[j][3], b[nt][0], b[nt][1]);
+                        }
+                    }
             }
         }
     }
@@ -503,19 +569,19 @@ struct Attend {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t x = __byte_perm(v[2 * i].w[u >> 1], v[2 * i + 1].w[u >> 1], sel);
-                a[0][2 * i] = half_sub(x & 0x000f000fu, 0x00080008u);
-                a[0][2 * i + 1] = half_sub(x & 0x00f000f0u, 0x00800080u);
-                a[1][2 * i] = half_sub((x >> 8) & 0x000f000fu, 0x00080008u);
-                a[1][2 * i + 1] = half_sub((x >> 8) & 0x00f000f0u, 0x00800080u);
+                a[0][2 * i] = centred4(x, false);
+                a[0][2 * i + 1] = centred4(x, true);
+                a[1][2 * i] = centred4(x >> 8, false);
+                a[1][2 * i + 1] = centred4(x >> 8, true);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t x = __byte_perm(v[2 * i].w[u], v[2 * i + 1].w[u], 0x5410), y = __byte_perm(v[2 * i].w[u], v[2 * i + 1].w[u], 0x7632);
-                a[0][2 * i] = half_sub(x & 0x00ff00ffu, 0x00800080u);
-                a[0][2 * i + 1] = half_sub(__byte_perm(x, 0, 0x4341), 0x00800080u);
-                a[1][2 * i] = half_sub(y & 0x00ff00ffu, 0x00800080u);
-                a[1][2 * i + 1] = half_sub(__byte_perm(y, 0, 0x4341), 0x00800080u);
+                a[0][2 * i] = centred8(x, 0x4240);
+                a[0][2 * i + 1] = centred8(x, 0x4341);
+                a[1][2 * i] = centred8(y, 0x4240);
+                a[1][2 * i + 1] = centred8(y, 0x4341);
             }
         }
     }
@@ -546,22 +612,33 @@ struct Attend {
         }
     }
 
-    // This warp's result into `o` [kCols][D] (normalised) and `ml` [kCols][2] (reference, sum).
-    __device__ static __forceinline__ void leave(Warp& w, float* o, float* ml) {
+    // This warp's reference and sum of each column into ml [kCols][2]; sums of all lanes are left in w.sum.
+    __device__ static __forceinline__ void leave_sums(Warp& w, float* ml) {
         const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-        constexpr int NS = kF32 ? 1 : NT;
-        // the accumulators are in units of 2^-24 * 2^(6 - exponent)
-        const float up = __int_as_float(w.scale_exp << 23);
 #pragma unroll
-        for (int nt = 0; nt < NS; ++nt)
+        for (int nt = 0; nt < (kF32 ? 1 : NT); ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float sum = w.sum[nt][e];
 #pragma unroll
-                for (int d = 4; d <= 16; d <<= 1) sum += __shfl_xor_sync(~0u, sum, d);
-                const int col = col_of(nt, 2 * tig + e);
-                const float by = sum == 0.0f ? 0.0f : 0x1p18f / sum;
-                if (gid == 0) ml[col * 2] = w.top[nt][e], ml[col * 2 + 1] = sum;
+                for (int d = 4; d <= 16; d <<= 1) w.sum[nt][e] += __shfl_xor_sync(~0u, w.sum[nt][e], d);
+                if (gid == 0) {
+                    float* const to = ml + col_of(nt, 2 * tig + e) * 2;
+                    to[0] = w.top[nt][e], to[1] = w.sum[nt][e];
+                }
+            }
+    }
+    // Its normalised result for columns c0 .. c0 + kRoundCols - 1 into o [kRoundCols][D].
+    __device__ static __forceinline__ void leave(const Warp& w, uint32_t o, int c0) {
+        const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+        // the accumulators are in units of 2^(exponent - 6)
+        const float up = __int_as_float(w.scale_exp << 23);
+#pragma unroll
+        for (int nt = 0; nt < (kF32 ? 1 : NT); ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int col = col_of(nt, 2 * tig + e) - c0;
+                if (col < 0 || col >= kRoundCols) continue;
+                const float sum = w.sum[nt][e], by = sum == 0.0f ? 0.0f : 0x1p-6f / sum;
 #pragma unroll
                 for (int u = 0; u < NG; ++u) {
                     float x[4];
@@ -571,122 +648,357 @@ struct Attend {
                         const float y = kF32 ? w.o[0][j][at] + w.o[NT - 1][j][at] : w.o[nt][j][at];
                         x[i] = y * by * (VB == 4 && (i & 1) ? 0.0625f : 1.0f) * up;
                     }
-                    *reinterpret_cast<float4*>(o + col * D + u * kGroup + gid * 4) = make_float4(x[0], x[1], x[2], x[3]);
+                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(o + (col * D + u * kGroup + gid * 4) * 4), "f"(x[0]), "f"(x[1]), "f"(x[2]),
+                                 "f"(x[3])
+                                 : "memory");
                 }
             }
     }
 
-    __device__ static __forceinline__ void store(T* out, float x) { *out = Elt<T>::from_float(x); }
+    __device__ static __forceinline__ void store(T* out, const float (&x)[4]) {
+        if constexpr (kF32) {
+            *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
+            __nv_bfloat162 h[2] = {__floats2bfloat162_rn(x[0], x[1]), __floats2bfloat162_rn(x[2], x[3])};
+            *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(h);
+        }
+    }
+    __device__ static __forceinline__ T* out_row(const AttendParams& p, int b, int g, int mine) {
+        const int i = mine / p.R, h = g * p.R + mine - i * p.R;
+        return static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.m + i) * p.ld_out + static_cast<int64_t>(h) * D;
+    }
+};
 
-    // The warps' results put together: into the output rows, or into the workspace as piece `slot`.
-    __device__ static __forceinline__ void merge(const AttendParams& p, const float* o, const float* ml, int b, int g, int ct, int slot) {
-        for (int idx = threadIdx.x; idx < kCols * D; idx += kThreads) {
-            const int col = idx / D, d = idx - col * D;
-            const int mine = ct * kCols + col;
-            if (mine >= p.m * p.R) break;
-            float top = kNegInf;
+// Tokens of sequence b, and the first one that any query of it sees, rounded down to a whole number of tiles.
+template <int TOK>
+__device__ __forceinline__ int attended(const AttendParams& p, int b, int& first) {
+    const int n = min(max(tokens_held(p.c, b) + p.len_bias, 0), p.T_upper);
+    first = first_seen(p, n) / TOK * TOK;
+    return n;
+}
+template <int TOK>
+__device__ __forceinline__ int tiles_of(const AttendParams& p, int b) {  // at least one: an empty sequence's rows are written too
+    int first;
+    const int n = attended<TOK>(p, b, first);
+    return max(1, (n - first + TOK - 1) / TOK);
+}
+
+// How the tiles of all (sequence, head, column tile) pairs, laid end to end, are cut into pieces of the same size.  Every thread takes the same
+// stretch of sequences, whose sums are scanned; part[i] is what lies before stretch i.
+template <int TOK, int THREADS>
+struct Cut {
+    const int64_t* part;
+    int64_t total;
+    int stretch;
+
+    __device__ static Cut make(const AttendParams& p, int64_t* part) {
+        __shared__ int64_t sums[THREADS / 32];
+        Cut c{part, 0, (p.c.B + THREADS - 1) / THREADS};
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const int from = threadIdx.x * c.stretch;
+        int64_t mine = 0;
+        for (int b = from; b < min(from + c.stretch, p.c.B); ++b) mine += tiles_of<TOK>(p, b);
+        int64_t sum = mine;
 #pragma unroll
-            for (int i = 0; i < WARPS; ++i) top = fmaxf(top, ml[(i * kCols + col) * 2]);
-            const float ref = top == kNegInf ? 0.0f : top;
-            float sum = 0.0f, x = 0.0f;
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t other = __shfl_up_sync(~0u, sum, d);
+            if (lane >= d) sum += other;
+        }
+        if (lane == 31) sums[warp] = sum;
+        __syncthreads();
+        int64_t before = 0;
 #pragma unroll
-            for (int i = 0; i < WARPS; ++i) {
-                const float l = ml[(i * kCols + col) * 2 + 1] * ex2(ml[(i * kCols + col) * 2] - ref);
-                sum += l;
-                x += l * o[(i * kCols + col) * D + d];
-            }
-            x = sum == 0.0f ? 0.0f : x / sum;
-            if (slot >= 0) {
-                p.ws_o[(static_cast<int64_t>(slot) * kCols + col) * D + d] = x;
-                if (d == 0) p.ws_lse[static_cast<int64_t>(slot) * kCols + col] = sum == 0.0f ? kNegInf : ref + log2f(sum);
-            } else {
-                const int i = mine / p.R, h = g * p.R + mine - i * p.R;
-                store(static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.m + i) * p.ld_out + static_cast<int64_t>(h) * D + d, x);
-            }
+        for (int i = 0; i < THREADS / 32; ++i) {
+            if (i < warp) before += sums[i];
+            c.total += sums[i];
+        }
+        part[threadIdx.x] = before + sum - mine;
+        __syncthreads();
+        c.total *= pairs_each(p);
+        return c;
+    }
+    __device__ static __forceinline__ int pairs_each(const AttendParams& p) { return p.c.G * p.col_tiles; }
+    // First tile of piece i of `pieces`.
+    __device__ __forceinline__ int64_t start(int i, int pieces) const { return total / pieces * i + min(static_cast<int64_t>(i), total % pieces); }
+    // The piece that tile u lies in.
+    __device__ __forceinline__ int piece_of(int64_t u, int pieces) const {
+        const int64_t each = total / pieces, more = total % pieces;  // the first `more` have one more
+        return static_cast<int>(u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each);
+    }
+    // The sequence that tile u lies in, and its first tile.
+    __device__ __forceinline__ int sequence_of(const AttendParams& p, int64_t u, int64_t& first) const {
+        const int each = pairs_each(p);
+        int lo = 0, hi = THREADS - 1;
+        while (lo < hi) {  // the last stretch that begins at or before u
+            const int mid = (lo + hi + 1) >> 1;
+            if (part[mid] * each <= u) lo = mid; else hi = mid - 1;
+        }
+        int b = lo * stretch;
+        first = part[lo] * each;
+        for (;;) {
+            const int64_t next = first + static_cast<int64_t>(tiles_of<TOK>(p, b)) * each;
+            if (u < next || b + 1 >= p.c.B) return b;
+            first = next, ++b;
         }
     }
 };
 
-// Tokens of sequence b, and the first one that any query of it sees.
-__device__ __forceinline__ int attended(const AttendParams& p, int b, int& first) {
-    const int n = min(max(tokens_held(p.c, b) + p.len_bias, 0), p.T_upper);
-    first = p.window > 0 ? max(n - p.m + 1 - p.window, 0) : 0;
-    return n;
-}
+// A place in a CTA's run of tiles: tiles tile .. end - 1 of the pair (b, pair) are its next ones.
+template <int TOK>
+struct Walk {
+    int b, pair, n, first, tiles, tile, end;
+    int64_t left;  // tiles of the run, from `tile` on
 
-// One CTA per (sequence, head, column tile) and share of its tokens; the warps take its stages in turn.
-template <typename T, int NG, int KB, int VB, int NT, int WARPS, int STAGES>
-__global__ void __launch_bounds__(WARPS * 32) attend_kernel(const AttendParams p) {
-    using A = Attend<T, NG, KB, VB, NT, WARPS, STAGES>;
+    __device__ __forceinline__ void at_sequence(const AttendParams& p) {
+        n = attended<TOK>(p, b, first);
+        tiles = max(1, (n - first + TOK - 1) / TOK);
+    }
+    __device__ __forceinline__ void limit() { end = static_cast<int>(min(static_cast<int64_t>(tiles), tile + left)); }
+    __device__ __forceinline__ bool next(const AttendParams& p) {
+        left -= end - tile;
+        if (left <= 0) return false;
+        tile = 0;
+        if (++pair == p.c.G * p.col_tiles) pair = 0, ++b, at_sequence(p);
+        limit();
+        return true;
+    }
+};
+
+template <typename T, int NG, int KB, int VB, int NT>
+__global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB, VB, NT>::kCtas) attend_kernel(const AttendParams p) {
+    using A = Attend<T, NG, KB, VB, NT>;
+    constexpr int kTok = A::kTok, S = A::STAGES, W = A::WARPS, kThreads = A::kThreads, D = A::D;
     extern __shared__ __align__(128) uint8_t smem[];
+    float* const ml = reinterpret_cast<float*>(smem + A::kRing);
+    uint32_t* const left_at = reinterpret_cast<uint32_t*>(smem + A::kRing + A::kMl);
+    const int warp = threadIdx.x >> 5;
+    const uint32_t ring = smem_u32(smem) + warp * S * A::kStage;
     grid_dependency_wait();
-    const int pair = blockIdx.x, split = blockIdx.y, warp = threadIdx.x >> 5;
-    const int ct = pair % p.col_tiles, bg = pair / p.col_tiles, b = bg / p.c.G, g = bg - b * p.c.G;
-    int first;
-    const int n = attended(p, b, first);
-    const int t_begin = first + split * p.share, t_end = min(n, t_begin + p.share);
-    typename A::Warp w;
-    A::begin(p, w, b, g, ct, n);
-    const uint32_t ring = smem_u32(smem) + warp * STAGES * A::kStage;
-    uint32_t there[STAGES];
-    const int stages = t_end > t_begin ? (t_end - t_begin + kStageTokens - 1) / kStageTokens : 0;
-    for (int i = warp; i < stages; i += WARPS) {
-        const int t0 = t_begin + i * kStageTokens;
-        there[0] = A::issue(p, ring, b, g, t0, t_end);
-        copy_commit();
-        copy_wait<0>();
-        __syncwarp();
-        A::fold(p, w, ring, t0, there[0]);
-        __syncwarp();
+
+    // This CTA's run of tiles, and which of a pair's tiles are this warp's.
+    Walk<kTok> w;
+    int step = W, skip = warp;
+    if (p.cluster > 0) {
+        const int at = blockIdx.x / p.cluster, each = p.c.G * p.col_tiles;
+        w.b = at / each, w.pair = at - w.b * each, w.tile = 0;
+        w.at_sequence(p);
+        w.left = w.tiles;
+        step *= p.cluster;
+        skip += W * (blockIdx.x - at * p.cluster);
+    } else {
+        const auto cut = Cut<kTok, kThreads>::make(p, reinterpret_cast<int64_t*>(smem));
+        const int64_t from = cut.start(blockIdx.x, gridDim.x);
+        w.left = cut.start(blockIdx.x + 1, gridDim.x) - from;
+        int64_t first;
+        w.b = cut.sequence_of(p, from, first);
+        w.at_sequence(p);
+        w.pair = static_cast<int>((from - first) / w.tiles);
+        w.tile = static_cast<int>((from - first) % w.tiles);
+        __syncthreads();  // (the scan lies where the ring does)
     }
-    __syncthreads();
-    float* const o = reinterpret_cast<float*>(smem);
-    float* const ml = o + WARPS * A::kCols * A::D;
-    A::leave(w, o + warp * A::kCols * A::D, ml + warp * A::kCols * 2);
-    __syncthreads();
-    A::merge(p, o, ml, b, g, ct, p.n_splits > 1 ? pair * p.n_splits + split : -1);
+    if (w.left <= 0) return;
+    w.limit();
+
+    // Copies run ahead of the arithmetic, across pairs too: `ahead` is the place of the next tile to be copied, `row` where this lane's token of it lies.
+    Walk<kTok> ahead = w;
+    int tile = ahead.tile + skip;
+    int64_t row = -1;
+    bool more = true;
+    const auto look = [&] {
+        while (tile >= ahead.end) {
+            if (!ahead.next(p)) {
+                more = false;
+                row = -1;
+                return;
+            }
+            tile = ahead.tile + skip;
+        }
+        row = A::find(p, ahead.b, ahead.pair / p.col_tiles, ahead.first + tile * kTok, ahead.n);
+    };
+    uint32_t there[S];  // [0]: of the stage that is next in the arithmetic
+    const auto copy = [&](int slot) {
+        uint32_t is = 0;
+        if (more) {
+            is = A::issue(p, ring + slot * A::kStage, row);
+            tile += step;
+            look();
+        }
+        copy_commit();
+        return is;
+    };
+    look();
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) there[i] = copy(i);
+
+    typename A::Warp q;
+    int slot = 0;
+    bool first_of_run = true;
+    for (;;) {
+        const int g = w.pair / p.col_tiles, ct = w.pair - g * p.col_tiles;
+        A::begin(p, q, w.b, g, ct, w.n);
+        for (int t = w.tile + skip; t < w.end; t += step) {
+            copy_wait<S - 2>();
+            __syncwarp();
+            there[S - 1] = copy(slot == 0 ? S - 1 : slot - 1);
+            A::fold(p, q, ring + slot * A::kStage, w.first + t * kTok, there[0]);
+#pragma unroll
+            for (int i = 0; i < S - 1; ++i) there[i] = there[i + 1];
+            slot = slot == S - 1 ? 0 : slot + 1;
+        }
+        // The warps' results, in the stage of each ring that the next copy goes to.
+        const uint32_t mine = static_cast<uint32_t>((warp * S + (slot == 0 ? S - 1 : slot - 1)) * A::kStage);
+        __syncwarp();
+        A::leave_sums(q, ml + warp * A::kCols * 2);
+        if ((threadIdx.x & 31) == 0) left_at[warp] = mine;
+        const bool whole = p.cluster == 1 || (p.cluster == 0 && w.tile == 0 && w.end == w.tiles);
+        const int used = min(p.m * p.R - ct * A::kCols, A::kCols);
+        constexpr int kQuads = A::kRoundCols * D / 4, kPer = (kQuads + kThreads - 1) / kThreads;
+        float kept[A::kRounds * kPer][4];
+        float kept_lse[A::kRounds * kPer];
+#pragma unroll
+        for (int r = 0; r < A::kRounds; ++r) {
+            A::leave(q, smem_u32(smem) + mine, r * A::kRoundCols);
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                const int i = threadIdx.x + k * kThreads;
+                const int in_round = i / (D / 4), col = r * A::kRoundCols + in_round, d = (i - in_round * (D / 4)) * 4;
+                float (&x)[4] = kept[r * kPer + k];
+                x[0] = x[1] = x[2] = x[3] = 0.0f;
+                kept_lse[r * kPer + k] = kNegInf;
+                if ((kQuads % kThreads == 0 || i < kQuads) && col < used) {
+                    float top = kNegInf, total = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) top = fmaxf(top, ml[(j * A::kCols + col) * 2]);
+                    const float ref = top == kNegInf ? 0.0f : top;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) {
+                        const float l = ml[(j * A::kCols + col) * 2 + 1] * ex2(ml[(j * A::kCols + col) * 2] - ref);
+                        const float4 y = *reinterpret_cast<const float4*>(smem + left_at[j] + (in_round * D + d) * 4);
+                        total += l;
+                        x[0] += l * y.x, x[1] += l * y.y, x[2] += l * y.z, x[3] += l * y.w;
+                    }
+                    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] *= by;
+                    kept_lse[r * kPer + k] = total == 0.0f ? kNegInf : ref + log2f(total);
+                    if (whole) {
+                        A::store(A::out_row(p, w.b, g, ct * A::kCols + col) + d, x);
+                    } else if (p.cluster == 0) {
+                        const int64_t at = 2ll * blockIdx.x + (first_of_run ? 0 : 1);
+                        *reinterpret_cast<float4*>(p.ws_o + (at * A::kCols + col) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+                        if (d == 0) p.ws_lse[at * A::kCols + col] = kept_lse[r * kPer + k];
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (p.cluster > 1) {
+            // One pair per cluster: the CTAs' results, each left at the start of its ring, and each CTA puts its share of the columns together.
+            float* const o = reinterpret_cast<float*>(smem);
+            float* const lse = o + A::kCols * D;
+            static_assert(A::kCols * (D + 1) * 4 <= A::kRing, "");
+#pragma unroll
+            for (int k = 0; k < A::kRounds * kPer; ++k) {
+                const int i = threadIdx.x + k % kPer * kThreads;
+                const int in_round = i / (D / 4), col = k / kPer * A::kRoundCols + in_round, d = (i - in_round * (D / 4)) * 4;
+                if (kQuads % kThreads == 0 || i < kQuads) {
+                    *reinterpret_cast<float4*>(o + col * D + d) = make_float4(kept[k][0], kept[k][1], kept[k][2], kept[k][3]);
+                    if (d == 0) lse[col] = kept_lse[k];
+                }
+            }
+            cluster_sync();
+            const uint32_t o_at = smem_u32(o), lse_at = smem_u32(lse);
+            const int rank = static_cast<int>(cluster_rank());
+            for (int i = threadIdx.x + rank * kThreads; i < used * (D / 2); i += kThreads * p.cluster) {
+                const int col = i / (D / 2), d = (i - col * (D / 2)) * 2;
+                float top = kNegInf, total = 0.0f, x0 = 0.0f, x1 = 0.0f;
+                for (int j = 0; j < p.cluster; ++j) top = fmaxf(top, __int_as_float(peer_load1(peer_address(lse_at + col * 4, j))));
+                const float ref = top == kNegInf ? 0.0f : top;
+                for (int j = 0; j < p.cluster; ++j) {
+                    const float l = ex2(__int_as_float(peer_load1(peer_address(lse_at + col * 4, j))) - ref);
+                    const float2 y = peer_load2(peer_address(o_at + (col * D + d) * 4, j));
+                    total += l;
+                    x0 += l * y.x, x1 += l * y.y;
+                }
+                const float by = total == 0.0f ? 0.0f : 1.0f / total;
+                T* const out = A::out_row(p, w.b, g, ct * A::kCols + col) + d;
+                out[0] = Elt<T>::from_float(x0 * by), out[1] = Elt<T>::from_float(x1 * by);
+            }
+            cluster_sync();  // nobody leaves while its results are read
+        }
+        first_of_run = false;
+        if (p.cluster > 0 || !w.next(p)) break;
+    }
+    copy_wait<0>();
 }
 
-// One CTA per column: its pieces put together.
-template <typename T, int D, int COLS>
-__global__ void __launch_bounds__(D < 64 ? 64 : D) merge_kernel(const AttendParams p) {
+// Pairs that were cut, put together: one CTA per cut and column; the first cut of a pair has it.
+template <typename T, int D, int COLS, int TOK>
+__global__ void __launch_bounds__(256) merge_kernel(const AttendParams p, int pieces) {
+    __shared__ int64_t part[256];
+    __shared__ float sums[256 / (D / 4)][D + 1];
     grid_dependency_wait();
-    const int pair = blockIdx.x, col = blockIdx.y, d = threadIdx.x;
-    const int ct = pair % p.col_tiles, bg = pair / p.col_tiles, b = bg / p.c.G, g = bg - b * p.c.G;
-    const int mine = ct * COLS + col;
-    if (mine >= p.m * p.R || d >= D) return;
-    const int64_t slot0 = static_cast<int64_t>(pair) * p.n_splits;
+    const auto cut = Cut<TOK, 256>::make(p, part);
+    const int c0 = blockIdx.x;  // the cut is between pieces c0 and c0 + 1
+    const int64_t at_cut = cut.start(c0 + 1, pieces);
+    if (at_cut >= cut.total) return;
+    int64_t first;
+    const int b = cut.sequence_of(p, at_cut, first), tiles = tiles_of<TOK>(p, b);
+    const int pair = static_cast<int>((at_cut - first) / tiles), g = pair / p.col_tiles, ct = pair - g * p.col_tiles;
+    first += static_cast<int64_t>(pair) * tiles;
+    const int64_t before = cut.start(c0, pieces);
+    const int mine = ct * COLS + blockIdx.y;
+    if (first == at_cut || before > first || mine >= p.m * p.R) return;
+    const int c1 = cut.piece_of(first + tiles - 1, pieces);
+    // the first CTA has it as its last pair, unless it is its first one too
+    const auto place = [&](int c) { return (2ll * c + (c == c0 && before < first ? 1 : 0)) * COLS + blockIdx.y; };
     float top = kNegInf;
-    for (int i = 0; i < p.n_splits; ++i) top = fmaxf(top, p.ws_lse[(slot0 + i) * COLS + col]);
+    for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.ws_lse[place(c)]);
     const float ref = top == kNegInf ? 0.0f : top;
-    float sum = 0.0f, x = 0.0f;
-    for (int i = 0; i < p.n_splits; ++i) {
-        const float l = ex2(p.ws_lse[(slot0 + i) * COLS + col] - ref);
-        sum += l;
-        x += l * p.ws_o[((slot0 + i) * COLS + col) * D + d];
+    constexpr int kLanes = D / 4, kRows = 256 / kLanes;
+    const int lane = threadIdx.x % kLanes, r = threadIdx.x / kLanes;
+    float total = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (r < kRows)
+        for (int c = c0 + r; c <= c1; c += kRows) {
+            const int64_t at = place(c);
+            const float l = ex2(p.ws_lse[at] - ref);
+            const float4 y = *reinterpret_cast<const float4*>(p.ws_o + at * D + lane * 4);
+            total += l;
+            x[0] += l * y.x, x[1] += l * y.y, x[2] += l * y.z, x[3] += l * y.w;
+        }
+    if (r < kRows) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[r][lane * 4 + e] = x[e];
+        if (lane == 0) sums[r][D] = total;
     }
-    x = sum == 0.0f ? 0.0f : x / sum;
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= D) return;
+    float y = 0.0f, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) y += sums[i][d], l += sums[i][D];
+    y = l == 0.0f ? 0.0f : y / l;
     const int i = mine / p.R, h = g * p.R + mine - i * p.R;
-    static_cast<T*>(p.out)[(static_cast<int64_t>(b) * p.m + i) * p.ld_out + static_cast<int64_t>(h) * D + d] = Elt<T>::from_float(x);
+    static_cast<T*>(p.out)[(static_cast<int64_t>(b) * p.m + i) * p.ld_out + static_cast<int64_t>(h) * D + d] = Elt<T>::from_float(y);
 }
 
 struct Plan {
-    int cols, col_tiles, n_splits, share;
+    int cols, col_tiles, cluster, ctas;
     int64_t pairs;
     size_t workspace;
 };
 
 template <typename T, int NG, int KB, int VB, int NT>
 int launch_attend(const AttendParams& p, const Plan& plan, void* stream) {
-    constexpr int kWarps = 8, kStages = 1;
-    using A = Attend<T, NG, KB, VB, NT, kWarps, kStages>;
-    auto kernel = attend_kernel<T, NG, KB, VB, NT, kWarps, kStages>;
+    using A = Attend<T, NG, KB, VB, NT>;
+    auto kernel = attend_kernel<T, NG, KB, VB, NT>;
     B2KV_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, A::kSmem));
-    OverlapLaunch launch(dim3(static_cast<unsigned>(plan.pairs), plan.n_splits), kWarps * 32, A::kSmem, stream);
+    OverlapLaunch launch(dim3(static_cast<unsigned>(plan.ctas)), A::kThreads, A::kSmem, stream, plan.cluster > 1 ? plan.cluster : 1);
     B2KV_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, kernel, p));
-    if (plan.n_splits > 1) {
-        OverlapLaunch second(dim3(static_cast<unsigned>(plan.pairs), A::kCols), A::D < 64 ? 64 : A::D, 0, stream);
-        B2KV_CUDA_TRY(cudaLaunchKernelEx(&second.cfg, merge_kernel<T, A::D, A::kCols>, p));
+    if (plan.cluster == 0) {
+        OverlapLaunch second(dim3(plan.ctas - 1, std::min(A::kCols, p.m * p.R)), 256, 0, stream);
+        B2KV_CUDA_TRY(cudaLaunchKernelEx(&second.cfg, merge_kernel<T, A::D, A::kCols, A::kTok>, p, plan.ctas));
     }
     return B2KV_OK;
 }
