@@ -141,7 +141,12 @@ __global__ void __launch_bounds__(kThreads) write_kernel(b2kv_qcache c, const T*
         store_codes<VB, true>(static_cast<uint8_t*>(c.v_codes) + row * (c.D * VB / 8), groups, u, o, w);
     else
         store_codes<KB, false>(static_cast<uint8_t*>(c.k_codes) + row * (c.D * KB / 8), groups, u, o, w);
-    if (o == 0) static_cast<__nv_bfloat16*>(values ? c.v_scales : c.k_scales)[row * scale_row(groups) + u] = scale;
+    if (o == 0) {
+        __nv_bfloat16* const to = static_cast<__nv_bfloat16*>(values ? c.v_scales : c.k_scales) + row * scale_row(groups);
+        to[u] = scale;
+        if (u == groups - 1)  // the rest takes part in products, with zeros
+            for (int r = groups; r < scale_row(groups); ++r) to[r] = __float2bfloat16_rn(0.0f);
+    }
 }
 
 // Thread = octet of the output.

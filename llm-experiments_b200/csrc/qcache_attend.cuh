@@ -14,8 +14,8 @@
 //     layout gives a lane the codes that it needs as one piece, the query is permuted to match, and P goes from the accumulator's
 //     layout to the operand's by an 8 x 8 transpose within the warp.  The rows go through tcgen05 only if they were first widened into
 //     shared memory at 16 bits per element, which is four times the traffic of reading them; as register operands they are widened in place.
-//   * Uncentred key codes (c + 8, c + 128): the accumulator of a group starts at minus 8 (128) times the group's sum of the query.  A group's sum is
-//     multiplied by its key scale in fp32.  Value codes are centred, because over thousands of tokens the sum of uncentred ones grows far beyond
+//   * Key codes stay uncentred (c + 8, c + 128); a group's sum is multiplied by its key scale in fp32, and what the centre comes to is one more small
+//     product, of the key scales and the query's sums over the groups, which the scores start from.  Value codes are centred, because over thousands of tokens the sum of uncentred ones grows far beyond
 //     what is left when the centre is taken off.
 //   * A probability times a value scale is rounded to fp16 (11 bits; the output has 8).  To keep it in range whatever the scales
 //     are, it is taken relative to the largest scale's exponent so far, and the accumulators are rescaled when that grows: below 2^15
@@ -65,6 +65,11 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -73,6 +78,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 __device__ __forceinline__ uint32_t half_sub(uint32_t a, uint32_t b) {
     uint32_t y;
     asm("sub.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+    return y;
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {  // one instruction
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
     return y;
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
@@ -89,6 +99,13 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there
 template <int BYTES>
 __device__ __forceinline__ void copy_small(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_small(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -163,6 +180,9 @@ struct Attend {
     static_assert(kRoundCols * D * 4 <= kStage && kRoundCols % 2 == 0, "");
     static constexpr int kMl = WARPS * kCols * 2 * 4;
     static constexpr int kSmem = kRing + kMl + WARPS * 4;
+    // The centre of the keys costs -kKOff * sum over groups of (key scale) * (sum of the group's query): a product over the groups, the sums
+    // in three bfloat16 parts (16 places: part k / kSG of group k % kSG; with 8 groups in two products).
+    static constexpr int kSG = scale_row(NG), kOffs = kF32 ? 1 : kSG == 8 ? 4 : 2;
     static constexpr int kKOff = KB == 4 ? 8 : 128;  // what is added to a key's code
     static constexpr float kKeyUnit = (KB == 4 ? 4.0f : 1.0f) * (kF32 ? 1.0f : 0x1p-24f);
 
@@ -182,7 +202,7 @@ struct Attend {
 
     struct Warp {
         uint32_t q[NT][NG][2][2];  // the query as the second operand of S = K q
-        float off[NT][NG][2];      // what a group's accumulator starts at, columns 2 tig and 2 tig + 1
+        uint32_t off[NT][kOffs];   // what the key's centre comes to, as the second operand of a product with the key scales (not for fp32)
         float f[NT][2];            // score = sum * f
         float slope[NT][2];        // log2 e times the column's slope
         int lo[NT][2], lim[NT][2]; // the column sees tokens lo <= t < lim
@@ -233,10 +253,10 @@ struct Attend {
             const float down = __int_as_float((254 + 14 - biased) << 23);
             // scale * 2^(e - 14) over what a code of one is in the product
             const float f = p.scale * kLog2e * 0x1p-14f / kKeyUnit * __int_as_float(biased << 23);
-            float part[2][NG];
+            float part[NG];  // the quad's shares of the groups' sums, of what the products see
 #pragma unroll
             for (int u = 0; u < NG; ++u) {
-                part[0][u] = part[1][u] = 0.0f;
+                part[u] = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[u][e] *= down;
                 // elements in the order of the codes in a word's halves: 4 bits (0,4) (1,5) (2,6) (3,7), the odd ones 16 times too
@@ -248,27 +268,39 @@ struct Attend {
                     const uint32_t h = pack_half(a, c);
                     const float2 got = unpack_half(h);
                     w.q[nt][u][j >> 1][j & 1] = h;
-                    part[0][u] += (got.x + got.y) / by;
+                    part[u] += (got.x + got.y) / by;
                     if constexpr (kF32) {
-                        const uint32_t l = pack_half(a - got.x, c - got.y);
-                        const float2 low = unpack_half(l);
-                        w.q[1][u][j >> 1][j & 1] = l;
-                        part[1][u] += (low.x + low.y) / by;
+                        w.q[1][u][j >> 1][j & 1] = pack_half(a - got.x, c - got.y);
                     }
                 }
             }
             const int from0 = 8 * tig, from1 = 8 * tig + 4;  // lanes that loaded columns 2 tig and 2 tig + 1
-#pragma unroll
-            for (int l = 0; l < (kF32 ? 2 : 1); ++l)
+            if constexpr (!kF32) {
+                float sum[NG];
 #pragma unroll
                 for (int u = 0; u < NG; ++u) {
-                    float s = part[l][u];
-                    s += __shfl_xor_sync(~0u, s, 1);
-                    s += __shfl_xor_sync(~0u, s, 2);
-                    s *= kF32 ? 0.0f : -static_cast<float>(kKOff) * kKeyUnit;
-                    w.off[nt + l][u][0] = __shfl_sync(~0u, s, from0);
-                    w.off[nt + l][u][1] = __shfl_sync(~0u, s, from1);
+                    sum[u] = part[u];
+                    sum[u] += __shfl_xor_sync(~0u, sum[u], 1);
+                    sum[u] += __shfl_xor_sync(~0u, sum[u], 2);
+                    sum[u] *= -static_cast<float>(kKOff) * kKeyUnit;
                 }
+#pragma unroll
+                for (int i = 0; i < kOffs; ++i) {
+                    float x[2] = {0.0f, 0.0f};
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int k = 2 * tig + e + 8 * i, which = k / kSG;
+#pragma unroll
+                        for (int u = 0; u < NG; ++u) {
+                            const float high = __bfloat162float(__float2bfloat16_rn(sum[u]));
+                            const float middle = __bfloat162float(__float2bfloat16_rn(sum[u] - high));
+                            if (k % kSG == u) x[e] = which == 0 ? high : which == 1 ? middle : which == 2 ? sum[u] - high - middle : 0.0f;
+                        }
+                    }
+                    const __nv_bfloat162 both = __floats2bfloat162_rn(x[0], x[1]);
+                    w.off[nt][i] = *reinterpret_cast<const uint32_t*>(&both);
+                }
+            }
             w.f[nt][0] = __shfl_sync(~0u, f, from0);
             w.f[nt][1] = __shfl_sync(~0u, f, from1);
 #pragma unroll
@@ -300,13 +332,13 @@ struct Attend {
     }
 
     // Where a lane's token of a tile lies: its row, -1 where there is none or no query sees it.
-    __device__ static __forceinline__ int64_t find(const AttendParams& p, int b, int g, int t0, int n) {
+    __device__ static __forceinline__ int64_t find(const AttendParams& p, int b, int g, int t0, int seen, int n) {
         const int lane = threadIdx.x & 31, t = t0 + (lane & (kTok - 1));
-        return t < n && t >= first_seen(p, n) ? row_of(p.c, b, g, t, p.dev_status) : -1;
+        return t < n && t >= seen ? row_of(p.c, b, g, t, p.dev_status) : -1;
     }
 
     // Starts the copies of a tile whose rows `find` gave (zeros where there is none); a bit for each token that is there.
-    __device__ static __forceinline__ uint32_t issue(const AttendParams& p, uint32_t stage, int64_t row) {
+    __device__ static __forceinline__ uint32_t copy_paged(const AttendParams& p, uint32_t stage, int64_t row) {
         const int lane = threadIdx.x & 31;
         const uint32_t there = __ballot_sync(~0u, row >= 0);
         const int64_t at = row >= 0 ? row : 0;
@@ -315,38 +347,75 @@ struct Attend {
             copy_small<kSRow>(ks + lane * kSRow, static_cast<const uint8_t*>(p.c.k_scales) + at * kSRow, row >= 0);
             copy_small<kSRow>(ks + kSBytes + lane * kSRow, static_cast<const uint8_t*>(p.c.v_scales) + at * kSRow, row >= 0);
         }
-        copy_rows<kKRow>(p, stage, static_cast<const uint8_t*>(p.c.k_codes), at, there, [](int r, int ch) { return k_place(r, ch); });
-        copy_rows<kVRow>(p, stage + kKBytes, static_cast<const uint8_t*>(p.c.v_codes), at, there, [](int r, int ch) { return v_place(r, ch); });
+        pieces_paged<kKRow>(stage, static_cast<const uint8_t*>(p.c.k_codes), at, there, [](int r, int ch) { return k_place(r, ch); });
+        pieces_paged<kVRow>(stage + kKBytes, static_cast<const uint8_t*>(p.c.v_codes), at, there, [](int r, int ch) { return v_place(r, ch); });
         return there;
     }
     template <int ROW, typename F>
-    __device__ static __forceinline__ void copy_rows(const AttendParams& p, uint32_t dst, const uint8_t* src, int64_t mine, uint32_t there, F&& place) {
+    __device__ static __forceinline__ void pieces_paged(uint32_t dst, const uint8_t* src, int64_t mine, uint32_t there, F&& place) {
         constexpr int kCh = ROW / 16, kPieces = kCh * kTok, kPer = (kPieces + 31) / 32;
         const int lane = threadIdx.x & 31;
-        if (p.c.block_table == nullptr) {  // rows follow one another
-            const int some = there != 0 ? __ffs(there) - 1 : 0;  // (tokens before the first one seen have no row here)
-            const uint8_t* const from = src + (__shfl_sync(~0u, mine, some) - some) * ROW + lane * 16;
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int idx = i * 32 + lane, r = idx / kCh, ch = idx - r * kCh;
-                if (kPieces % 32 == 0 || idx < kPieces) {
-                    const bool is = (there >> r) & 1u;
-                    copy16(dst + place(r, ch), is ? from + i * 512 : src, is);
-                }
+        for (int i = 0; i < kPer; ++i) {
+            const int idx = i * 32 + lane, r = idx / kCh, ch = idx - r * kCh;
+            const int64_t row = __shfl_sync(~0u, mine, r & 31);
+            if (kPieces % 32 == 0 || idx < kPieces) copy16(dst + place(r, ch), src + row * ROW + ch * 16, (there >> r) & 1u);
+        }
+    }
+
+    // The same for rows that follow one another, the sequence's first one at row `row`: tokens t0 .., those from `seen` to n - 1.
+    __device__ static __forceinline__ uint32_t copy_run(const AttendParams& p, uint32_t stage, int64_t row, int t0, int seen, int n) {
+        const int lane = threadIdx.x & 31;
+        const int64_t at = row + t0;
+        const uint32_t ks = stage + kKBytes + kVBytes + lane * kSRow;
+        const uint8_t* const k = static_cast<const uint8_t*>(p.c.k_codes) + at * kKRow;
+        const uint8_t* const v = static_cast<const uint8_t*>(p.c.v_codes) + at * kVRow;
+        const uint8_t* const k_scale = static_cast<const uint8_t*>(p.c.k_scales) + (at + lane) * kSRow;
+        const uint8_t* const v_scale = static_cast<const uint8_t*>(p.c.v_scales) + (at + lane) * kSRow;
+        uint32_t there = ~0u;
+        if (t0 >= seen && t0 + kTok <= n) {  // nearly always
+            if (kTok == 32 || lane < kTok) {
+                copy_small<kSRow>(ks, k_scale);
+                copy_small<kSRow>(ks + kSBytes, v_scale);
             }
+            pieces_run<kKRow, true>(stage, k, there, [](int r, int ch) { return k_place(r, ch); });
+            pieces_run<kVRow, true>(stage + kKBytes, v, there, [](int r, int ch) { return v_place(r, ch); });
         } else {
+            const int t = t0 + (lane & (kTok - 1));
+            const bool is = t >= seen && t < n;
+            there = __ballot_sync(~0u, is);
+            if (kTok == 32 || lane < kTok) {
+                copy_small<kSRow>(ks, is ? k_scale : static_cast<const uint8_t*>(p.c.k_scales), is);
+                copy_small<kSRow>(ks + kSBytes, is ? v_scale : static_cast<const uint8_t*>(p.c.v_scales), is);
+            }
+            pieces_run<kKRow, false>(stage, k, there, [](int r, int ch) { return k_place(r, ch); });
+            pieces_run<kVRow, false>(stage + kKBytes, v, there, [](int r, int ch) { return v_place(r, ch); });
+        }
+        return there;
+    }
+    template <int ROW, bool kAll, typename F>
+    __device__ static __forceinline__ void pieces_run(uint32_t dst, const uint8_t* src, uint32_t there, F&& place) {
+        constexpr int kCh = ROW / 16, kPieces = kCh * kTok, kPer = (kPieces + 31) / 32;
+        const int lane = threadIdx.x & 31;
+        const uint8_t* const from = src + lane * 16;
+        const uint8_t* const some = src + (there != 0 ? __ffs(there) - 1 : 0) * ROW;  // a row that is there, for the address of those that are not
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int idx = i * 32 + lane, r = idx / kCh, ch = idx - r * kCh;
-                const int64_t row = __shfl_sync(~0u, mine, r & 31);
-                if (kPieces % 32 == 0 || idx < kPieces) copy16(dst + place(r, ch), src + row * ROW + ch * 16, (there >> r) & 1u);
+        for (int i = 0; i < kPer; ++i) {
+            const int idx = i * 32 + lane, r = idx / kCh, ch = idx - r * kCh;
+            if (kPieces % 32 == 0 || idx < kPieces) {
+                if constexpr (kAll) {
+                    copy16(dst + place(r, ch), from + i * 512);
+                } else {
+                    const bool is = (there >> r) & 1u;
+                    copy16(dst + place(r, ch), is ? from + i * 512 : some, is);
+                }
             }
         }
     }
 
     // Codes in bits 0 .. 3 or 4 .. 7 of 16-bit halves, or in bytes, as centred fp16 numbers (the higher ones times 16).
     __device__ static __forceinline__ uint32_t centred4(uint32_t x, bool high) {
-        return high ? half_sub((x & 0x00f000f0u) | 0x64006400u, 0x64806480u) : half_sub((x & 0x000f000fu) | 0x64006400u, 0x64086408u);
+        return high ? half_sub(and_or(x, 0x00f000f0u, 0x64006400u), 0x64806480u) : half_sub(and_or(x, 0x000f000fu, 0x64006400u), 0x64086408u);
     }
     __device__ static __forceinline__ uint32_t centred8(uint32_t x, int sel) { return half_sub(__byte_perm(x, 0x64646464u, sel), 0x64806480u); }
 
@@ -355,11 +424,12 @@ struct Attend {
     __device__ static __forceinline__ void k_piece(const uint32_t* w, uint32_t& first, uint32_t& second) {
         if constexpr (KB == 4) {
             const uint32_t x = STEP == 0 ? w[0] : __funnelshift_r(w[0], w[0], 8);
-            first = x & 0x003c003cu;
-            second = x & 0x03c003c0u;
             if constexpr (kF32) {
-                first = half_sub(first | 0x64006400u, 0x64206420u);    // 1024 + 4 c less 1024 + 32
-                second = half_sub(second | 0x64006400u, 0x66006600u);  // 1024 + 64 c less 1024 + 512
+                first = half_sub(and_or(x, 0x003c003cu, 0x64006400u), 0x64206420u);   // 1024 + 4 c less 1024 + 32
+                second = half_sub(and_or(x, 0x03c003c0u, 0x64006400u), 0x66006600u);  // 1024 + 64 c less 1024 + 512
+            } else {
+                first = x & 0x003c003cu;
+                second = x & 0x03c003c0u;
             }
         } else {
             first = kF32 ? centred8(w[STEP], 0x4140) : __byte_perm(w[STEP], 0, 0x4140);
@@ -388,6 +458,16 @@ struct Attend {
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
+            if constexpr (!kF32) {
+                uint32_t a0, a1;  // key scales of the two rows, groups 2 tig and 2 tig + 1 of as many as there are
+                const uint32_t at = ks + r * kSRow + tig % (kSG / 2) * 4;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(a0) : "r"(at) : "memory");
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(a1) : "r"(at + 8 * kSRow) : "memory");
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < kOffs; i += 2) mma_bf16(acc[nt], a0, a1, a0, a1, w.off[nt][i], w.off[nt][i + 1]);
+            }
 #pragma unroll
             for (int u = 0; u < NG; ++u) {
                 uint32_t a[2][4];
@@ -400,7 +480,7 @@ struct Attend {
                 const float f1 = __uint_as_float(u & 1 ? s1.w[u >> 1] & 0xffff0000u : s1.w[u >> 1] << 16);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float d[4] = {w.off[nt][u][0], w.off[nt][u][1], w.off[nt][u][0], w.off[nt][u][1]};
+                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     mma(d, a[0][0], a[0][1], a[0][2], a[0][3], w.q[nt][u][0][0], w.q[nt][u][0][1]);
                     mma(d, a[1][0], a[1][1], a[1][2], a[1][3], w.q[nt][u][1][0], w.q[nt][u][1][1]);
                     acc[nt][0] = fmaf(f0, d[0], acc[nt][0]);
@@ -511,7 +591,15 @@ struct Attend {
                         for (int e = 0; e < 4; ++e) w.o[nt][j][e] *= by;
             }
         }
-        const float vf = __int_as_float((260 - w.scale_exp) << 23);  // 2^(6 - exponent)
+        {
+            const float vf = __int_as_float((260 - w.scale_exp) << 23);  // 2^(6 - exponent)
+#pragma unroll
+            for (int h = 0; h < MT; ++h)
+#pragma unroll
+                for (int nt = 0; nt < NS; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[h][nt][e] *= vf;
+        }
 #pragma unroll
         for (int h = 0; h < MT; ++h) {
             const int r = h * 16 + gid;
@@ -523,8 +611,8 @@ struct Attend {
             for (int i = 0; i < 4; ++i) load_v(v[i], vc, h * 16 + 2 * tig + (i & 1) + (i >> 1) * 8, gid);
 #pragma unroll
             for (int u = 0; u < NG; ++u) {
-                const float f0 = vf * __uint_as_float(u & 1 ? s0.w[u >> 1] & 0xffff0000u : s0.w[u >> 1] << 16);
-                const float f1 = vf * __uint_as_float(u & 1 ? s1.w[u >> 1] & 0xffff0000u : s1.w[u >> 1] << 16);
+                const float f0 = __uint_as_float(u & 1 ? s0.w[u >> 1] & 0xffff0000u : s0.w[u >> 1] << 16);
+                const float f1 = __uint_as_float(u & 1 ? s1.w[u >> 1] & 0xffff0000u : s1.w[u >> 1] << 16);
                 uint32_t b[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NS; ++nt) {
@@ -743,10 +831,10 @@ struct Cut {
     }
 };
 
-// A place in a CTA's run of tiles: tiles tile .. end - 1 of the pair (b, pair) are its next ones.
+// A place in a CTA's run of tiles: tiles tile .. end - 1 of the pair (b, g, ct) are its next ones.
 template <int TOK>
 struct Walk {
-    int b, pair, n, first, tiles, tile, end;
+    int b, g, ct, n, first, tiles, tile, end;
     int64_t left;  // tiles of the run, from `tile` on
 
     __device__ __forceinline__ void at_sequence(const AttendParams& p) {
@@ -758,7 +846,10 @@ struct Walk {
         left -= end - tile;
         if (left <= 0) return false;
         tile = 0;
-        if (++pair == p.c.G * p.col_tiles) pair = 0, ++b, at_sequence(p);
+        if (++ct == p.col_tiles) {
+            ct = 0;
+            if (++g == p.c.G) g = 0, ++b, at_sequence(p);
+        }
         limit();
         return true;
     }
@@ -780,7 +871,8 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
     int step = W, skip = warp;
     if (p.cluster > 0) {
         const int at = blockIdx.x / p.cluster, each = p.c.G * p.col_tiles;
-        w.b = at / each, w.pair = at - w.b * each, w.tile = 0;
+        w.b = at / each, w.tile = 0;
+        w.g = (at - w.b * each) / p.col_tiles, w.ct = at - w.b * each - w.g * p.col_tiles;
         w.at_sequence(p);
         w.left = w.tiles;
         step *= p.cluster;
@@ -792,34 +884,39 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
         int64_t first;
         w.b = cut.sequence_of(p, from, first);
         w.at_sequence(p);
-        w.pair = static_cast<int>((from - first) / w.tiles);
-        w.tile = static_cast<int>((from - first) % w.tiles);
+        const int pair = static_cast<int>((from - first) / w.tiles);
+        w.tile = static_cast<int>((from - first) - static_cast<int64_t>(pair) * w.tiles);
+        w.g = pair / p.col_tiles, w.ct = pair - w.g * p.col_tiles;
         __syncthreads();  // (the scan lies where the ring does)
     }
     if (w.left <= 0) return;
     w.limit();
 
-    // Copies run ahead of the arithmetic, across pairs too: `ahead` is the place of the next tile to be copied, `row` where this lane's token of it lies.
+    // Copies run ahead of the arithmetic, across pairs too: `ahead` is the place of the next tile to be copied, `row` where this lane's token of it lies
+    // (contiguous: only the pair's first row is kept).
     Walk<kTok> ahead = w;
-    int tile = ahead.tile + skip;
-    int64_t row = -1;
+    int tile = ahead.tile + skip, seen = first_seen(p, ahead.n);
+    const bool paged = p.c.block_table != nullptr;
+    int64_t row = paged ? 0 : row_of(p.c, ahead.b, ahead.g, 0, nullptr);
     bool more = true;
     const auto look = [&] {
         while (tile >= ahead.end) {
             if (!ahead.next(p)) {
                 more = false;
-                row = -1;
                 return;
             }
             tile = ahead.tile + skip;
+            seen = first_seen(p, ahead.n);
+            if (!paged) row = row_of(p.c, ahead.b, ahead.g, 0, nullptr);
         }
-        row = A::find(p, ahead.b, ahead.pair / p.col_tiles, ahead.first + tile * kTok, ahead.n);
+        if (paged) row = A::find(p, ahead.b, ahead.g, ahead.first + tile * kTok, seen, ahead.n);
     };
     uint32_t there[S];  // [0]: of the stage that is next in the arithmetic
     const auto copy = [&](int slot) {
         uint32_t is = 0;
         if (more) {
-            is = A::issue(p, ring + slot * A::kStage, row);
+            const uint32_t to = ring + slot * A::kStage;
+            is = paged ? A::copy_paged(p, to, row) : A::copy_run(p, to, row, ahead.first + tile * kTok, seen, ahead.n);
             tile += step;
             look();
         }
@@ -834,7 +931,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
     int slot = 0;
     bool first_of_run = true;
     for (;;) {
-        const int g = w.pair / p.col_tiles, ct = w.pair - g * p.col_tiles;
+        const int g = w.g, ct = w.ct;
         A::begin(p, q, w.b, g, ct, w.n);
         for (int t = w.tile + skip; t < w.end; t += step) {
             copy_wait<S - 2>();
