@@ -621,7 +621,7 @@ int b2kv_moe_combine(float* x, int64_t ld_x, const void* y, int64_t ld_y, const 
  * the elements lie as the matrix instructions of b2kv_qcache_attend take them, so that nothing is moved between lanes there:
  *   keys    element 32 u + 8 o + i is code i of unit o * (D / 32) + u, units of 8 codes;
  *   values  element 32 u + 4 o + i is code i of unit o * (D / 32) + u, units of 4 codes;
- *   codes   lowest bits first, stored as code + 8 or code + 128; the 32-bit units of 4-bit keys are turned left by two bits;
+ *   codes   lowest bits first, stored as code + 8 or code + 128; units of 4-bit codes (32 bits of keys, 16 of values) are turned left by two bits;
  *   scales  scale of group u at u of b2kv_qcache_scale_row(D) bfloat16 per row, the rest is zeros.
  * D is 32, 64, 96, 128 or 256.  (k_bits, v_bits) is (4, 4), (8, 4) or (8, 8): keys are what suffers from few bits.
  * dtype is the type of the rows that are written, read back and attended with.  seq_lens (device, B entries) or len are the tokens

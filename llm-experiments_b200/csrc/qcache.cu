@@ -90,6 +90,7 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int groups, int u, int
     } else if (!kValues) {
         reinterpret_cast<uint2*>(row)[o * groups + u] = w;
     } else if (BITS == 4) {
+        w.x = ((w.x << 2) & 0xfffcfffcu) | ((w.x >> 14) & 0x00030003u);
         reinterpret_cast<uint16_t*>(row)[2 * o * groups + u] = static_cast<uint16_t>(w.x);
         reinterpret_cast<uint16_t*>(row)[(2 * o + 1) * groups + u] = static_cast<uint16_t>(w.x >> 16);
     } else {
@@ -105,8 +106,9 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t* row, int groups, int 
     }
     if (!kValues) return reinterpret_cast<const uint2*>(row)[o * groups + u];
     if (BITS == 4) {
-        const uint32_t a = reinterpret_cast<const uint16_t*>(row)[2 * o * groups + u];
-        return make_uint2(a | static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[(2 * o + 1) * groups + u]) << 16, 0);
+        const uint32_t w = reinterpret_cast<const uint16_t*>(row)[2 * o * groups + u] |
+                           static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[(2 * o + 1) * groups + u]) << 16;
+        return make_uint2(((w >> 2) & 0x3fff3fffu) | ((w << 14) & 0xc000c000u), 0);
     }
     return make_uint2(reinterpret_cast<const uint32_t*>(row)[2 * o * groups + u], reinterpret_cast<const uint32_t*>(row)[(2 * o + 1) * groups + u]);
 }

@@ -4,26 +4,25 @@
 // arithmetic has to be hidden behind 23 bytes per clock and SM, and with 4 bits 46 elements per clock have to be widened.  Plain
 // fp32 arithmetic cannot (128 FMAs per clock and SM, one per element and query head); the tensor cores can, if widening is cheap:
 //
-//   * Codes become fp16 numbers by masking: a key's code c in bits 2 .. 5 or 6 .. 9 of a 16-bit half is the fp16 subnormal c * 2^-22 or c * 2^-18, two
+//   * Codes become fp16 numbers by masking alone: a code c in bits 2 .. 5 or 6 .. 9 of a 16-bit half is the fp16 subnormal c * 2^-22 or c * 2^-18, two
 //     codes per instruction, and tensor cores take subnormals at full speed.  They add products by the exponents as they stand, so
-//     that a number whose first bit is k places below the tenth loses k bits of the sum: at most 4 here, which is why the keys' words are kept
-//     turned by two bits (bits 0 .. 3 and 4 .. 7 lost 7 and 3).  fp32 queries, and values, have the mask's result put behind the exponent of 1024
-//     by the same instruction and the centre taken off by a second one.
+//     that a number whose first bit is k places below the tenth loses k bits of the sum: at most 4 here, which is why units of 4-bit codes are kept
+//     turned by two bits (bits 0 .. 3 and 4 .. 7 would lose 7 and 3).
 //   * Both products have the cache's rows as the operand of many rows: S[token, column] = K q (16 tokens by 8 columns per MMA, m16n8k16)
 //     and O[element, column] += V^T P.  A column is one (new token, query head) pair of the key / value head.  The cache's
 //     layout gives a lane the codes that it needs as one piece, the query is permuted to match, and P goes from the accumulator's
 //     layout to the operand's by an 8 x 8 transpose within the warp.  The rows go through tcgen05 only if they were first widened into
 //     shared memory at 16 bits per element, which is four times the traffic of reading them; as register operands they are widened in place.
-//   * Key codes stay uncentred (c + 8, c + 128); a group's sum is multiplied by its key scale in fp32, and what the centre comes to is one more small
-//     product, of the key scales and the query's sums over the groups, which the scores start from.  Value codes are centred, because over thousands of tokens the sum of uncentred ones grows far beyond
-//     what is left when the centre is taken off.
-//   * A probability times a value scale is rounded to fp16 (11 bits; the output has 8).  To keep it in range whatever the scales
-//     are, it is taken relative to the largest scale's exponent so far, and the accumulators are rescaled when that grows: below 2^15
-//     always, and full precision down to scales 2^20 below the largest.
-//   * fp32 queries and probabilities are sums of two fp16 numbers (22 bits), in columns of their own, and only 16 tokens' products are
-//     added up in the tensor core, whose sums are cut off and not rounded.
-//   * Softmax: scores in the log2 domain, reference maxima that move only when a score has outgrown its reference by more than 2^8 (one vote
-//     per stage), sums per lane until the end, all in fp32.
+//   * Codes stay uncentred (c + 8, c + 128).  What the keys' centre comes to is a small product of the key scales and the query's sums over the
+//     groups, which the scores start from; the values' is a row of ones in their product.  A group's sum is multiplied by its key scale in fp32.
+//   * A probability is rounded to fp16, multiplied by its value scale there and rounded again (11 bits; the output has 8).  To keep that in range
+//     whatever the scales are, they are taken relative to the largest exponent so far, and the accumulators are rescaled when that
+//     grows: products stay below 2^15, and scales down to 2^-17 of the largest keep all their bits.
+//   * fp32 queries and weights are sums of two fp16 numbers (22 bits), in columns of their own; codes are put behind the exponent of 1024 by the
+//     mask's instruction and the centre is taken off by a second one; and only 16 tokens' products are added up in the tensor core, whose
+//     sums are cut off and not rounded.
+//   * Softmax: scores in the log2 domain, references that move only when a score has outgrown its own by more than 2^8 (one vote per stage), sums per
+//     lane until the end, all in fp32.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -52,6 +51,7 @@ struct AttendParams {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLowest = -3.0e38f;  // a reference where nothing was seen yet: any score has outgrown it, and differences stay finite
 constexpr int kScaleExpMin = 17;  // (biased) smaller exponents of value scales are taken for this one: 2^-110
 
 __device__ __forceinline__ float ex2(float x) {
@@ -61,18 +61,24 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// d = the product alone
+__device__ __forceinline__ void mma_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ uint32_t half_sub(uint32_t a, uint32_t b) {
@@ -83,6 +89,11 @@ __device__ __forceinline__ uint32_t half_sub(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {  // one instruction
     uint32_t y;
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+    return y;
+}
+__device__ __forceinline__ uint32_t half_mul(uint32_t a, uint32_t b) {
+    uint32_t y;
+    asm("mul.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
     return y;
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
@@ -185,6 +196,9 @@ struct Attend {
     static constexpr int kSG = scale_row(NG), kOffs = kF32 ? 1 : kSG == 8 ? 4 : 2;
     static constexpr int kKOff = KB == 4 ? 8 : 128;  // what is added to a key's code
     static constexpr float kKeyUnit = (KB == 4 ? 4.0f : 1.0f) * (kF32 ? 1.0f : 0x1p-24f);
+    // Weights are probabilities times 2^kShift, up to 2^(8 + kShift); times a value scale, 2^(6 - exponent) times that at most: below 2^15.
+    static constexpr int kShift = kF32 ? 0 : 3;
+    static constexpr float kValueUnit = (VB == 4 ? 4.0f : 1.0f) * (kF32 ? 1.0f : 0x1p-24f);  // of a code of one; every other row of 4 bits has 16 times that
 
     // Where 16-byte piece ch of row r lies in a stage: moved about so that the lanes that read together meet different banks.
     __device__ static __forceinline__ int k_place(int r, int ch) {
@@ -200,16 +214,48 @@ struct Attend {
         return r * kVRow + ch * 16;
     }
 
+    // Where a lane reads and copies within a stage, from one row or piece to the next.  The rows 8 further on lie 8 rows further on, whatever
+    // the moving about.
+    struct Lane {
+        uint32_t k;         // its piece of row gid of the keys
+        uint32_t v[2];      // its pieces of rows 2 tig and 2 tig + 1 of the values
+        uint32_t put_k, put_v;  // its first 16-byte piece of a copy
+        __device__ __forceinline__ void set() {
+            const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+            k = NG == 3 ? gid * kKRow + tig * NG * KB : k_place(gid, tig * NG * KB / 16) + tig * NG * KB % 16;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = 2 * tig + i, at = gid * (NG * VB / 2);
+                v[i] = kKBytes + (NG == 3 ? r * kVRow + at : v_place(r, at / 16) + at % 16);
+            }
+            put_k = k_place(lane / (kKRow / 16), lane % (kKRow / 16));
+            put_v = kKBytes + v_place(lane / (kVRow / 16), lane % (kVRow / 16));
+        }
+    };
+    // Piece i * 32 + lane lies at (the lane's first) ^ this + i * 512.
+    __device__ static __forceinline__ uint32_t moved_v(int i) {
+        return kVRow == 128 ? (i & 1) * 64 : kVRow == 256 ? (i & 1) * 16 + ((i >> 1) & 1) * 64 : 0;
+    }
+
+    // What is seldom asked for, in shared memory: of a column of the CTA's present pair.
+    struct Column {
+        int lo, lim;  // it sees tokens lo <= t < lim
+        float slope;  // log2 e times its slope
+        float f;      // a score is the product's sum times this (before a cap and a bias)
+    };
+
     struct Warp {
         uint32_t q[NT][NG][2][2];  // the query as the second operand of S = K q
         uint32_t off[NT][kOffs];   // what the key's centre comes to, as the second operand of a product with the key scales (not for fp32)
-        float f[NT][2];            // score = sum * f
-        float slope[NT][2];        // log2 e times the column's slope
-        int lo[NT][2], lim[NT][2]; // the column sees tokens lo <= t < lim
+        float f[NT][2];            // the same where there is neither cap nor bias, else 1
         int all_lo, all_lim;       // tokens that every used column sees
         float o[NT][NG * 2][4];    // elements 32 (j / 2) + 4 gid + 2 (j & 1) (+1 in the last two), columns 2 tig, 2 tig + 1
-        float top[NT][2], sum[NT][2];
+        float ref[NT][2];          // scores are taken relative to this: what was the largest so far, less kShift
+        float sum[NT][2];          // of 2^(score - ref), this lane's tokens
+        float ones[NT][4];         // sums of a column's weights per group, row = group (not for fp32)
+        uint32_t poison;           // groups whose value scale was NaN, of column gid (not for fp32)
         int scale_exp;
+        bool fresh;                // some column may not have seen anything yet
     };
 
     // fp32: both tiles are the same columns.
@@ -222,7 +268,7 @@ struct Attend {
     __device__ static void load8(const __nv_bfloat16* p, float (&x)[8]) { Elt<__nv_bfloat16>::widen(*reinterpret_cast<const uint4*>(p), x); }
 
     // Queries of sequence b, head g, column tile ct, and what goes with them.  n: tokens of the sequence.
-    __device__ static __forceinline__ void begin(const AttendParams& p, Warp& w, int b, int g, int ct, int n) {
+    __device__ static __forceinline__ void begin(const AttendParams& p, Warp& w, Column* columns, int b, int g, int ct, int n) {
         const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
         const int used = p.m * p.R;
         w.all_lo = 0, w.all_lim = 0x7fffffff;
@@ -274,7 +320,6 @@ struct Attend {
                     }
                 }
             }
-            const int from0 = 8 * tig, from1 = 8 * tig + 4;  // lanes that loaded columns 2 tig and 2 tig + 1
             if constexpr (!kF32) {
                 float sum[NG];
 #pragma unroll
@@ -301,24 +346,23 @@ struct Attend {
                     w.off[nt][i] = *reinterpret_cast<const uint32_t*>(&both);
                 }
             }
-            w.f[nt][0] = __shfl_sync(~0u, f, from0);
-            w.f[nt][1] = __shfl_sync(~0u, f, from1);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int mine = ct * kCols + col_of(nt, 2 * tig + e);
-                const int i = mine / p.R, place = n - p.m + i;
-                const bool is = mine < used;
-                w.lim[nt][e] = is ? place + 1 : 0;
-                w.lo[nt][e] = is && p.window > 0 ? max(place + 1 - p.window, 0) : 0;
-                w.slope[nt][e] = is && p.slopes != nullptr ? p.slopes[g * p.R + mine - i * p.R] * kLog2e : 0.0f;
-                if (is) w.all_lim = min(w.all_lim, w.lim[nt][e]), w.all_lo = max(w.all_lo, w.lo[nt][e]);
-            }
+            const float shown = p.softcap == 0.0f && p.slopes == nullptr ? f : 1.0f;
+            w.f[nt][0] = __shfl_sync(~0u, shown, 8 * tig);  // from the lanes that loaded columns 2 tig and 2 tig + 1
+            w.f[nt][1] = __shfl_sync(~0u, shown, 8 * tig + 4);
+            // (every warp of the CTA writes the same)
+            const bool is = col < used;
+            const int i = col / p.R, place = n - p.m + i;
+            const Column mine{is && p.window > 0 ? max(place + 1 - p.window, 0) : 0, is ? place + 1 : 0,
+                              is && p.slopes != nullptr ? p.slopes[g * p.R + col - i * p.R] * kLog2e : 0.0f, f};
+            if (tig == 0) columns[col_of(nt, gid)] = mine;
+            if (is) w.all_lim = min(w.all_lim, mine.lim), w.all_lo = max(w.all_lo, mine.lo);
         }
 #pragma unroll
-        for (int d = 1; d <= 2; d <<= 1) {  // (used columns differ from lane to lane)
+        for (int d = 4; d <= 16; d <<= 1) {
             w.all_lim = min(w.all_lim, __shfl_xor_sync(~0u, w.all_lim, d));
             w.all_lo = max(w.all_lo, __shfl_xor_sync(~0u, w.all_lo, d));
         }
+        __syncwarp();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -326,8 +370,12 @@ struct Attend {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w.o[nt][j][e] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) w.top[nt][e] = kNegInf, w.sum[nt][e] = 0.0f;
+            for (int e = 0; e < 4; ++e) w.ones[nt][e] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) w.ref[nt][e] = kLowest, w.sum[nt][e] = 0.0f;
         }
+        w.poison = 0;
+        w.fresh = true;
         w.scale_exp = kScaleExpMin;
     }
 
@@ -338,7 +386,7 @@ struct Attend {
     }
 
     // Starts the copies of a tile whose rows `find` gave (zeros where there is none); a bit for each token that is there.
-    __device__ static __forceinline__ uint32_t copy_paged(const AttendParams& p, uint32_t stage, int64_t row) {
+    __device__ static __forceinline__ uint32_t copy_paged(const AttendParams& p, const Lane& l, uint32_t stage, int64_t row) {
         const int lane = threadIdx.x & 31;
         const uint32_t there = __ballot_sync(~0u, row >= 0);
         const int64_t at = row >= 0 ? row : 0;
@@ -347,24 +395,24 @@ struct Attend {
             copy_small<kSRow>(ks + lane * kSRow, static_cast<const uint8_t*>(p.c.k_scales) + at * kSRow, row >= 0);
             copy_small<kSRow>(ks + kSBytes + lane * kSRow, static_cast<const uint8_t*>(p.c.v_scales) + at * kSRow, row >= 0);
         }
-        pieces_paged<kKRow>(stage, static_cast<const uint8_t*>(p.c.k_codes), at, there, [](int r, int ch) { return k_place(r, ch); });
-        pieces_paged<kVRow>(stage + kKBytes, static_cast<const uint8_t*>(p.c.v_codes), at, there, [](int r, int ch) { return v_place(r, ch); });
+        pieces_paged<kKRow>(stage + l.put_k, static_cast<const uint8_t*>(p.c.k_codes), at, there, [](int) { return 0u; });
+        pieces_paged<kVRow>(stage + l.put_v, static_cast<const uint8_t*>(p.c.v_codes), at, there, moved_v);
         return there;
     }
     template <int ROW, typename F>
-    __device__ static __forceinline__ void pieces_paged(uint32_t dst, const uint8_t* src, int64_t mine, uint32_t there, F&& place) {
+    __device__ static __forceinline__ void pieces_paged(uint32_t dst, const uint8_t* src, int64_t mine, uint32_t there, F&& moved) {
         constexpr int kCh = ROW / 16, kPieces = kCh * kTok, kPer = (kPieces + 31) / 32;
         const int lane = threadIdx.x & 31;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int idx = i * 32 + lane, r = idx / kCh, ch = idx - r * kCh;
             const int64_t row = __shfl_sync(~0u, mine, r & 31);
-            if (kPieces % 32 == 0 || idx < kPieces) copy16(dst + place(r, ch), src + row * ROW + ch * 16, (there >> r) & 1u);
+            if (kPieces % 32 == 0 || idx < kPieces) copy16((dst ^ moved(i)) + i * 512, src + row * ROW + ch * 16, (there >> r) & 1u);
         }
     }
 
     // The same for rows that follow one another, the sequence's first one at row `row`: tokens t0 .., those from `seen` to n - 1.
-    __device__ static __forceinline__ uint32_t copy_run(const AttendParams& p, uint32_t stage, int64_t row, int t0, int seen, int n) {
+    __device__ static __forceinline__ uint32_t copy_run(const AttendParams& p, const Lane& l, uint32_t stage, int64_t row, int t0, int seen, int n) {
         const int lane = threadIdx.x & 31;
         const int64_t at = row + t0;
         const uint32_t ks = stage + kKBytes + kVBytes + lane * kSRow;
@@ -378,8 +426,8 @@ struct Attend {
                 copy_small<kSRow>(ks, k_scale);
                 copy_small<kSRow>(ks + kSBytes, v_scale);
             }
-            pieces_run<kKRow, true>(stage, k, there, [](int r, int ch) { return k_place(r, ch); });
-            pieces_run<kVRow, true>(stage + kKBytes, v, there, [](int r, int ch) { return v_place(r, ch); });
+            pieces_run<kKRow, true>(stage + l.put_k, k, there, [](int) { return 0u; });
+            pieces_run<kVRow, true>(stage + l.put_v, v, there, moved_v);
         } else {
             const int t = t0 + (lane & (kTok - 1));
             const bool is = t >= seen && t < n;
@@ -388,68 +436,69 @@ struct Attend {
                 copy_small<kSRow>(ks, is ? k_scale : static_cast<const uint8_t*>(p.c.k_scales), is);
                 copy_small<kSRow>(ks + kSBytes, is ? v_scale : static_cast<const uint8_t*>(p.c.v_scales), is);
             }
-            pieces_run<kKRow, false>(stage, k, there, [](int r, int ch) { return k_place(r, ch); });
-            pieces_run<kVRow, false>(stage + kKBytes, v, there, [](int r, int ch) { return v_place(r, ch); });
+            pieces_run<kKRow, false>(stage + l.put_k, k, there, [](int) { return 0u; });
+            pieces_run<kVRow, false>(stage + l.put_v, v, there, moved_v);
         }
         return there;
     }
     template <int ROW, bool kAll, typename F>
-    __device__ static __forceinline__ void pieces_run(uint32_t dst, const uint8_t* src, uint32_t there, F&& place) {
+    __device__ static __forceinline__ void pieces_run(uint32_t dst, const uint8_t* src, uint32_t there, F&& moved) {
         constexpr int kCh = ROW / 16, kPieces = kCh * kTok, kPer = (kPieces + 31) / 32;
         const int lane = threadIdx.x & 31;
         const uint8_t* const from = src + lane * 16;
         const uint8_t* const some = src + (there != 0 ? __ffs(there) - 1 : 0) * ROW;  // a row that is there, for the address of those that are not
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int idx = i * 32 + lane, r = idx / kCh, ch = idx - r * kCh;
+            const int idx = i * 32 + lane, r = idx / kCh;
             if (kPieces % 32 == 0 || idx < kPieces) {
                 if constexpr (kAll) {
-                    copy16(dst + place(r, ch), from + i * 512);
+                    copy16((dst ^ moved(i)) + i * 512, from + i * 512);
                 } else {
                     const bool is = (there >> r) & 1u;
-                    copy16(dst + place(r, ch), is ? from + i * 512 : some, is);
+                    copy16((dst ^ moved(i)) + i * 512, is ? from + i * 512 : some, is);
                 }
             }
         }
     }
 
-    // Codes in bits 0 .. 3 or 4 .. 7 of 16-bit halves, or in bytes, as centred fp16 numbers (the higher ones times 16).
-    __device__ static __forceinline__ uint32_t centred4(uint32_t x, bool high) {
-        return high ? half_sub(and_or(x, 0x00f000f0u, 0x64006400u), 0x64806480u) : half_sub(and_or(x, 0x000f000fu, 0x64006400u), 0x64086408u);
+    // Codes as fp16 numbers: of bits 2 .. 5 and 6 .. 9 of 16-bit halves, or of two bytes.  As stored for bfloat16, centred for fp32.
+    __device__ static __forceinline__ void pieces4(uint32_t x, uint32_t& low, uint32_t& high) {
+        if constexpr (kF32) {
+            low = half_sub(and_or(x, 0x003c003cu, 0x64006400u), 0x64206420u);   // 1024 + 4 c less 1024 + 32
+            high = half_sub(and_or(x, 0x03c003c0u, 0x64006400u), 0x66006600u);  // 1024 + 64 c less 1024 + 512
+        } else {
+            low = x & 0x003c003cu;
+            high = x & 0x03c003c0u;
+        }
     }
-    __device__ static __forceinline__ uint32_t centred8(uint32_t x, int sel) { return half_sub(__byte_perm(x, 0x64646464u, sel), 0x64806480u); }
+    __device__ static __forceinline__ uint32_t piece8(uint32_t x, int sel) {
+        return kF32 ? half_sub(__byte_perm(x, 0x64646464u, sel), 0x64806480u) : __byte_perm(x, 0, sel);
+    }
 
     // A row's codes of half a group as operand pieces (a0 and a2, or a1 and a3).
     template <int STEP>
     __device__ static __forceinline__ void k_piece(const uint32_t* w, uint32_t& first, uint32_t& second) {
         if constexpr (KB == 4) {
-            const uint32_t x = STEP == 0 ? w[0] : __funnelshift_r(w[0], w[0], 8);
-            if constexpr (kF32) {
-                first = half_sub(and_or(x, 0x003c003cu, 0x64006400u), 0x64206420u);   // 1024 + 4 c less 1024 + 32
-                second = half_sub(and_or(x, 0x03c003c0u, 0x64006400u), 0x66006600u);  // 1024 + 64 c less 1024 + 512
-            } else {
-                first = x & 0x003c003cu;
-                second = x & 0x03c003c0u;
-            }
+            pieces4(STEP == 0 ? w[0] : __funnelshift_r(w[0], w[0], 8), first, second);
         } else {
-            first = kF32 ? centred8(w[STEP], 0x4140) : __byte_perm(w[STEP], 0, 0x4140);
-            second = kF32 ? centred8(w[STEP], 0x4342) : __byte_perm(w[STEP], 0, 0x4342);
+            first = piece8(w[STEP], 0x4140);
+            second = piece8(w[STEP], 0x4342);
         }
     }
 
     // The tokens of a stage, t0 the first.
-    __device__ static __forceinline__ void fold(const AttendParams& p, Warp& w, uint32_t stage, int t0, uint32_t there) {
+    __device__ static __forceinline__ void fold(const AttendParams& p, const Lane& l, Warp& w, const Column* columns, uint32_t stage, int t0, uint32_t there) {
         const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-        const uint32_t ks = stage + kKBytes + kVBytes, vs = ks + kSBytes, vc = stage + kKBytes;
-        constexpr int kKPiece = NG * KB, kVPiece = NG * VB / 2;  // bytes of a row that a lane reads
-        constexpr int NS = kF32 ? 1 : NT;                        // tiles of scores
+        const uint32_t ks = stage + kKBytes + kVBytes, vs = ks + kSBytes;
+        constexpr int kKPiece = NG * KB;   // bytes of a row that a lane reads
+        constexpr int NS = kF32 ? 1 : NT;  // tiles of scores
         float s[MT][NS][4];
 #pragma unroll
         for (int h = 0; h < MT; ++h) {
             const int r = h * 16 + gid;
             Words<kKPiece> k0, k1;
-            load_k(k0, stage, r, tig);
-            load_k(k1, stage, r + 8, tig);
+            load_k(k0, stage + l.k, h * 16);
+            load_k(k1, stage + l.k, h * 16 + 8);
             Words<kSRow> s0, s1;
             s0.load(ks + r * kSRow);
             s1.load(ks + (r + 8) * kSRow);
@@ -480,8 +529,8 @@ struct Attend {
                 const float f1 = __uint_as_float(u & 1 ? s1.w[u >> 1] & 0xffff0000u : s1.w[u >> 1] << 16);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma(d, a[0][0], a[0][1], a[0][2], a[0][3], w.q[nt][u][0][0], w.q[nt][u][0][1]);
+                    float d[4];
+                    mma_new(d, a[0][0], a[0][1], a[0][2], a[0][3], w.q[nt][u][0][0], w.q[nt][u][0][1]);
                     mma(d, a[1][0], a[1][1], a[1][2], a[1][3], w.q[nt][u][1][0], w.q[nt][u][1][1]);
                     acc[nt][0] = fmaf(f0, d[0], acc[nt][0]);
                     acc[nt][1] = fmaf(f0, d[1], acc[nt][1]);
@@ -492,52 +541,80 @@ struct Attend {
 #pragma unroll
             for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[h][nt][e] = (kF32 ? acc[0][e] + acc[NT - 1][e] : acc[nt][e]) * w.f[nt][e & 1];
+                for (int e = 0; e < 4; ++e) s[h][nt][e] = kF32 ? acc[0][e] + acc[NT - 1][e] : acc[nt][e];
         }
-        if (p.softcap > 0.0f) {
-            const float down = 1.0f / (p.softcap * kLog2e), up = p.softcap * kLog2e;
+        if (p.softcap > 0.0f || p.slopes != nullptr) {
 #pragma unroll
-            for (int h = 0; h < MT; ++h)
+            for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NS; ++nt)
+                for (int e = 0; e < 4; ++e) {
+                    const float f = columns[col_of(nt, 2 * tig + (e & 1))].f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[h][nt][e] = tanhf(s[h][nt][e] * down) * up;
-        }
-        if (p.slopes != nullptr) {
+                    for (int h = 0; h < MT; ++h) s[h][nt][e] *= f;
+                }
+            if (p.softcap > 0.0f) {
+                const float down = 1.0f / (p.softcap * kLog2e), up = p.softcap * kLog2e;
 #pragma unroll
-            for (int h = 0; h < MT; ++h)
+                for (int h = 0; h < MT; ++h)
 #pragma unroll
-                for (int nt = 0; nt < NS; ++nt)
+                    for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[h][nt][e] -= w.slope[nt][e & 1] * static_cast<float>(w.lim[nt][e & 1] - 1 - (t0 + h * 16 + (e >> 1) * 8 + gid));
-        }
-        // Masks, where the stage has a token that some column does not see.
-        const bool masked = there != ~0u || t0 < w.all_lo || t0 + kTok > w.all_lim;
-        uint32_t hidden = 0;  // a bit per score of this lane
-        if (masked) {
-#pragma unroll
-            for (int h = 0; h < MT; ++h)
+                        for (int e = 0; e < 4; ++e) s[h][nt][e] = tanhf(s[h][nt][e] * down) * up;
+            }
+            if (p.slopes != nullptr) {
 #pragma unroll
                 for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
+                        const Column c = columns[col_of(nt, 2 * tig + (e & 1))];
+#pragma unroll
+                        for (int h = 0; h < MT; ++h) s[h][nt][e] -= c.slope * static_cast<float>(c.lim - 1 - (t0 + h * 16 + (e >> 1) * 8 + gid));
+                    }
+            }
+        }
+        // Relative to the references, which move where a score has outgrown its own by more than 2^8 (or may be the first one seen).
+        const bool masked = there != ~0u || t0 < w.all_lo || t0 + kTok > w.all_lim;  // the stage has a token that some column does not see
+        uint32_t hidden = 0;                                                         // then: a bit per score of this lane
+        bool move = masked || w.fresh;
+        if (!move) {
+            float most = kNegInf;
+#pragma unroll
+            for (int nt = 0; nt < NS; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int h = 0; h < MT; ++h) {
+                        s[h][nt][e] = fmaf(s[h][nt][e], w.f[nt][e & 1], -w.ref[nt][e & 1]);
+                        most = fmaxf(most, s[h][nt][e]);
+                    }
+            move = __any_sync(~0u, most > 8.0f + kShift);
+            if (move) {
+#pragma unroll
+                for (int h = 0; h < MT; ++h)
+#pragma unroll
+                    for (int nt = 0; nt < NS; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[h][nt][e] += w.ref[nt][e & 1];
+            }
+        } else {
+#pragma unroll
+            for (int nt = 0; nt < NS; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const Column c = columns[col_of(nt, 2 * tig + (e & 1))];
+#pragma unroll
+                    for (int h = 0; h < MT; ++h) {
                         const int r = h * 16 + (e >> 1) * 8 + gid, t = t0 + r;
-                        if (!((there >> r) & 1u) || t < w.lo[nt][e & 1] || t >= w.lim[nt][e & 1]) {
+                        s[h][nt][e] *= w.f[nt][e & 1];
+                        if (!((there >> r) & 1u) || t < c.lo || t >= c.lim) {
                             s[h][nt][e] = kNegInf;
                             hidden |= 1u << ((h * NS + nt) * 4 + e);
                         }
                     }
+                }
+            w.fresh = w.fresh && masked;
         }
-        // The references, where a score has outgrown its own by more than 2^8.
-        bool grown = false;
-#pragma unroll
-        for (int h = 0; h < MT; ++h)
-#pragma unroll
-            for (int nt = 0; nt < NS; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) grown = grown || s[h][nt][e] > w.top[nt][e & 1] + 8.0f;
-        if (__any_sync(~0u, grown)) {
+        if (move) {
 #pragma unroll
             for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
@@ -547,104 +624,192 @@ struct Attend {
                     for (int h = 0; h < MT; ++h) top = fmaxf(top, fmaxf(s[h][nt][e], s[h][nt][e + 2]));
 #pragma unroll
                     for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-                    top = fmaxf(top, w.top[nt][e]);
-                    const float by = top == w.top[nt][e] ? 1.0f : ex2(w.top[nt][e] - top);
-                    w.top[nt][e] = top;
+                    top = fmaxf(top - kShift, w.ref[nt][e]);
+                    const float by = top == w.ref[nt][e] ? 1.0f : ex2(w.ref[nt][e] - top);
+                    w.ref[nt][e] = top;
                     w.sum[nt][e] *= by;
 #pragma unroll
-                    for (int l = 0; l < (kF32 ? 2 : 1); ++l)
+                    for (int k = 0; k < (kF32 ? 2 : 1); ++k) {
 #pragma unroll
-                        for (int j = 0; j < NG * 2; ++j) w.o[nt + l][j][e] *= by, w.o[nt + l][j][e + 2] *= by;
+                        for (int j = 0; j < NG * 2; ++j) w.o[nt + k][j][e] *= by, w.o[nt + k][j][e + 2] *= by;
+                        if constexpr (!kF32) w.ones[nt + k][e] *= by;
+                    }
+#pragma unroll
+                    for (int h = 0; h < MT; ++h) s[h][nt][e] -= top, s[h][nt][e + 2] -= top;
                 }
         }
 #pragma unroll
         for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float top = w.top[nt][e] == kNegInf ? 0.0f : w.top[nt][e];
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int h = 0; h < MT; ++h) {
-                    s[h][nt][e] = ex2(s[h][nt][e] - top);
-                    s[h][nt][e + 2] = ex2(s[h][nt][e + 2] - top);
+                    s[h][nt][e] = ex2(s[h][nt][e]);
+                    s[h][nt][e + 2] = ex2(s[h][nt][e + 2]);
                     w.sum[nt][e] += s[h][nt][e] + s[h][nt][e + 2];
                 }
-            }
-        // The largest exponent of a value scale (NaN groups have none).
-        {
-            Words<kSRow> mine;
-            mine.load(vs + (lane & (kTok - 1)) * kSRow);
-            uint32_t most = 0;
+        // The largest exponent of a value scale so far (NaN groups have none).
+        Words<kSRow> mine;
+        mine.load(vs + (lane & (kTok - 1)) * kSRow);
+        uint32_t most = mine.w[0];
+#pragma unroll
+        for (int i = 1; i < kSG / 2; ++i) most = __vmaxu2(most, mine.w[i]);
+        most = __reduce_max_sync(~0u, max(most >> 16, most & 0xffffu));
+        const bool nan = most >= 0x7f80u;
+        if (nan) {
+            most = 0;
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
-                const uint32_t x = i & 1 ? mine.w[i >> 1] >> 16 : mine.w[i >> 1] & 0xffffu;
-                most = max(most, x >= 0x7f80u ? 0u : x);
+                const uint32_t y = i & 1 ? mine.w[i >> 1] >> 16 : mine.w[i >> 1] & 0xffffu;
+                most = max(most, y >= 0x7f80u ? 0u : y);
             }
-            const int now = static_cast<int>(__reduce_max_sync(~0u, most) >> 7);
-            if (now > w.scale_exp) {
-                const float by = w.scale_exp - now < -126 ? 0.0f : __int_as_float((127 + w.scale_exp - now) << 23);
-                w.scale_exp = now;
+            most = __reduce_max_sync(~0u, most);
+        }
+        const int now = static_cast<int>(most >> 7);
+        if (now > w.scale_exp) {
+            const float by = w.scale_exp - now < -126 ? 0.0f : __int_as_float((127 + w.scale_exp - now) << 23);
+            w.scale_exp = now;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int j = 0; j < NG * 2; ++j)
+                for (int j = 0; j < NG * 2; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) w.o[nt][j][e] *= by;
+                    for (int e = 0; e < 4; ++e) w.o[nt][j][e] *= by;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w.ones[nt][e] *= by;
             }
         }
-        {
-            const float vf = __int_as_float((260 - w.scale_exp) << 23);  // 2^(6 - exponent)
-#pragma unroll
-            for (int h = 0; h < MT; ++h)
-#pragma unroll
-                for (int nt = 0; nt < NS; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[h][nt][e] *= vf;
-        }
+        if constexpr (kF32)
+            values_f32(l, w, stage, s, masked, hidden);
+        else
+            values_bf16(l, w, stage, s, mine, nan, hidden);
+    }
+
+    // O += V^T P for fp32: weights times value scales in 32 bits, then as two fp16 numbers.
+    template <int NS>
+    __device__ static __forceinline__ void values_f32(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NS][4], bool masked, uint32_t hidden) {
+        const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+        const float vf = __int_as_float((260 - w.scale_exp) << 23);  // 2^(6 - exponent)
+        const uint32_t vs = stage + kKBytes + kVBytes + kSBytes;
 #pragma unroll
         for (int h = 0; h < MT; ++h) {
             const int r = h * 16 + gid;
             Words<kSRow> s0, s1;
             s0.load(vs + r * kSRow);
             s1.load(vs + (r + 8) * kSRow);
-            Words<kVPiece> v[4];  // tokens 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9
+            Words<NG * VB / 2> v[4];  // tokens 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_v(v[i], vc, h * 16 + 2 * tig + (i & 1) + (i >> 1) * 8, gid);
+            for (int i = 0; i < 4; ++i) load_v(v[i], stage + l.v[i & 1], h * 16 + (i >> 1) * 8);
 #pragma unroll
             for (int u = 0; u < NG; ++u) {
-                const float f0 = __uint_as_float(u & 1 ? s0.w[u >> 1] & 0xffff0000u : s0.w[u >> 1] << 16);
-                const float f1 = __uint_as_float(u & 1 ? s1.w[u >> 1] & 0xffff0000u : s1.w[u >> 1] << 16);
-                uint32_t b[NT][2];
+                const float f0 = vf * __uint_as_float(u & 1 ? s0.w[u >> 1] & 0xffff0000u : s0.w[u >> 1] << 16);
+                const float f1 = vf * __uint_as_float(u & 1 ? s1.w[u >> 1] & 0xffff0000u : s1.w[u >> 1] << 16);
+                float x[4] = {weight[h][0][0] * f0, weight[h][0][1] * f0, weight[h][0][2] * f1, weight[h][0][3] * f1};
+                if (masked) {  // (0 times a NaN scale)
 #pragma unroll
-                for (int nt = 0; nt < NS; ++nt) {
-                    float x[4] = {s[h][nt][0] * f0, s[h][nt][1] * f0, s[h][nt][2] * f1, s[h][nt][3] * f1};
-                    if (masked) {  // (0 times a NaN scale)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = (hidden >> ((h * NS + nt) * 4 + e)) & 1u ? 0.0f : x[e];
-                    }
-                    const uint32_t p0 = pack_half(x[0], x[1]), p1 = pack_half(x[2], x[3]);
-                    b[nt][0] = transpose8x8(p0);
-                    b[nt][1] = transpose8x8(p1);
-                    if constexpr (kF32) {
-                        const float2 g0 = unpack_half(p0), g1 = unpack_half(p1);
-                        b[1][0] = transpose8x8(pack_half(x[0] - g0.x, x[1] - g0.y));
-                        b[1][1] = transpose8x8(pack_half(x[2] - g1.x, x[3] - g1.y));
-                    }
+                    for (int e = 0; e < 4; ++e) x[e] = (hidden >> (h * 4 + e)) & 1u ? 0.0f : x[e];
                 }
+                const uint32_t p0 = pack_half(x[0], x[1]), p1 = pack_half(x[2], x[3]);
+                const float2 g0 = unpack_half(p0), g1 = unpack_half(p1);
+                const uint32_t b[2][2] = {{transpose8x8(p0), transpose8x8(p1)},
+                                          {transpose8x8(pack_half(x[0] - g0.x, x[1] - g0.y)), transpose8x8(pack_half(x[2] - g1.x, x[3] - g1.y))}};
                 uint32_t a[2][4];
                 v_pieces(v, u, a);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        if constexpr (kF32) {
-                            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma(d, a[j][0], a[j][1], a[j][2], a[j][3], b[nt][0], b[nt][1]);
+                        float d[4];
+                        mma_new(d, a[j][0], a[j][1], a[j][2], a[j][3], b[nt][0], b[nt][1]);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) w.o[nt][2 * u + j][e] += d[e];
-                        } else {
-                            mma(w.o[nt][2 * u + j], a[j][0], a[j][1], a[j][2], a[j][3], b[nt][0], b[nt][1]);
-                        }
+                        for (int e = 0; e < 4; ++e) w.o[nt][2 * u + j][e] += d[e];
                     }
+            }
+        }
+    }
+
+    // O += V^T P for bfloat16: weights go to the operand's layout as fp16 numbers and meet the value scales there, two per instruction.  The scales
+    // are made fp16 (relative to the largest exponent) and brought into that order by the lane that has the token, in place.
+    template <int NS>
+    __device__ static __forceinline__ void values_bf16(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NS][4], const Words<kSRow>& mine, bool nan,
+                                                       uint32_t hidden) {
+        const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+        constexpr int kWords = kSG / 2;
+        const uint32_t vs = stage + kKBytes + kVBytes + kSBytes;
+        {
+            const float vf = __int_as_float((257 - w.scale_exp) << 23);  // 2^(6 - kShift - exponent)
+            uint32_t c[kWords];
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) c[i] = pack_half(__uint_as_float(mine.w[i] << 16) * vf, __uint_as_float(mine.w[i] & 0xffff0000u) * vf);
+            const bool odd = lane & 1;
+            const int r = lane & (kTok - 1);
+            const uint32_t to = vs + (((r >> 4) * 4 + ((r & 7) >> 1)) * 2 + ((r >> 3) & 1)) * (kSG * 4);
+            __syncwarp();  // every lane has its row
+            if constexpr (kWords == 1) {
+                const uint32_t other = __shfl_xor_sync(~0u, c[0], 1);
+                const uint32_t y = odd ? __byte_perm(other, c[0], 0x7632) : __byte_perm(c[0], other, 0x5410);
+                if (kTok == 32 || lane < kTok) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + odd * 4), "r"(y) : "memory");
+            } else {
+                uint32_t y[kWords];
+#pragma unroll
+                for (int i = 0; i < kWords / 2; ++i) {
+                    const uint32_t other = __shfl_xor_sync(~0u, odd ? c[i] : c[i + kWords / 2], 1);
+                    const uint32_t own = odd ? c[i + kWords / 2] : c[i];
+                    const uint32_t first = odd ? other : own, second = odd ? own : other;
+                    y[2 * i] = __byte_perm(first, second, 0x5410);
+                    y[2 * i + 1] = __byte_perm(first, second, 0x7632);
+                }
+                if (kTok == 32 || lane < kTok) {
+#pragma unroll
+                    for (int i = 0; i < kWords; i += 2)
+                        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(to + odd * kWords * 4 + i * 4), "r"(y[i]), "r"(y[i + 1]) : "memory");
+                }
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int h = 0; h < MT; ++h) {
+            Words<2 * kSG * 4> sv;  // groups of tokens 2 tig and 2 tig + 1, then of 2 tig + 8 and 2 tig + 9
+            sv.load(vs + (h * 4 + tig) * (2 * kSG * 4));
+            Words<NG * VB / 2> v[4];  // tokens 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load_v(v[i], stage + l.v[i & 1], h * 16 + (i >> 1) * 8);
+            uint32_t weights[NS][2];
+#pragma unroll
+            for (int nt = 0; nt < NS; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) weights[nt][i] = transpose8x8(pack_half(weight[h][nt][2 * i], weight[h][nt][2 * i + 1]));
+#pragma unroll
+            for (int u = 0; u < NG; ++u) {
+                uint32_t b[NS][2];
+#pragma unroll
+                for (int nt = 0; nt < NS; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) b[nt][i] = half_mul(weights[nt][i], sv.w[i * kSG + u]);
+                if (nan) {
+                    // A NaN scale counts where its token is seen, and for its own group alone: it stays out of the products, which know
+                    // neither, and is put into the result at the end.
+#pragma unroll
+                    for (int nt = 0; nt < NS; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t bits = hidden >> ((h * NS + nt) * 4 + 2 * i);
+                            const uint32_t seen = transpose8x8((bits & 1u ? 0u : 0xffffu) | (bits & 2u ? 0u : 0xffff0000u));
+                            const uint32_t x = sv.w[i * kSG + u];
+                            const uint32_t bad = ((x & 0x7fffu) > 0x7c00u ? 0xffffu : 0u) | ((x & 0x7fff0000u) > 0x7c000000u ? 0xffff0000u : 0u);
+                            if ((bad & seen) != 0) w.poison |= 1u << (nt * NG + u);
+                            b[nt][i] &= ~bad;
+                        }
+                }
+                uint32_t a[2][4];
+                v_pieces(v, u, a);
+                const uint32_t one = gid == u ? 0x3c003c00u : 0u;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma(w.o[nt][2 * u], a[0][0], a[0][1], a[0][2], a[0][3], b[nt][0], b[nt][1]);
+                    mma(w.o[nt][2 * u + 1], a[1][0], a[1][1], a[1][2], a[1][3], b[nt][0], b[nt][1]);
+                    mma(w.ones[nt], one, 0, one, 0, b[nt][0], b[nt][1]);
+                }
             }
         }
     }
@@ -656,47 +821,39 @@ struct Attend {
             const int sel = u & 1 ? 0x7632 : 0x5410;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const uint32_t x = __byte_perm(v[2 * i].w[u >> 1], v[2 * i + 1].w[u >> 1], sel);
-                a[0][2 * i] = centred4(x, false);
-                a[0][2 * i + 1] = centred4(x, true);
-                a[1][2 * i] = centred4(x >> 8, false);
-                a[1][2 * i + 1] = centred4(x >> 8, true);
+                const uint32_t x = __byte_perm(v[2 * i].w[u >> 1], v[2 * i + 1].w[u >> 1], sel), y = __byte_perm(x, 0, 0x2301);
+                pieces4(x, a[0][2 * i], a[0][2 * i + 1]);
+                pieces4(y, a[1][2 * i], a[1][2 * i + 1]);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t x = __byte_perm(v[2 * i].w[u], v[2 * i + 1].w[u], 0x5410), y = __byte_perm(v[2 * i].w[u], v[2 * i + 1].w[u], 0x7632);
-                a[0][2 * i] = centred8(x, 0x4240);
-                a[0][2 * i + 1] = centred8(x, 0x4341);
-                a[1][2 * i] = centred8(y, 0x4240);
-                a[1][2 * i + 1] = centred8(y, 0x4341);
+                a[0][2 * i] = piece8(x, 0x4240);
+                a[0][2 * i + 1] = piece8(x, 0x4341);
+                a[1][2 * i] = piece8(y, 0x4240);
+                a[1][2 * i + 1] = piece8(y, 0x4341);
             }
         }
     }
 
-    // A lane's pieces of a row, which lie in one 16-byte piece or are whole ones.
+    // A lane's piece of a row `rows` (a multiple of 8) behind the one at `at`: whole 16-byte pieces, which were moved about, or a part of one.
     template <typename W>
-    __device__ static __forceinline__ void load_k(W& k, uint32_t stage, int r, int tig) {
-        constexpr int kBytes = NG * KB;
-        if constexpr (kBytes > 16 && kBytes % 16 == 0) {
+    __device__ static __forceinline__ void load_k(W& k, uint32_t at, int rows) {
+        if constexpr (NG * KB > 16 && NG != 3) {
 #pragma unroll
-            for (int i = 0; i < kBytes / 16; ++i) k.load16(stage + k_place(r, tig * (kBytes / 16) + i), 4 * i);
-        } else if constexpr (NG == 3) {
-            k.load(stage + r * kKRow + tig * kBytes);
+            for (int i = 0; i < NG * KB / 16; ++i) k.load16((at ^ (i * 16)) + rows * kKRow, 4 * i);
         } else {
-            k.load(stage + k_place(r, tig * kBytes / 16) + tig * kBytes % 16);
+            k.load(at + rows * kKRow);
         }
     }
     template <typename W>
-    __device__ static __forceinline__ void load_v(W& v, uint32_t codes, int r, int gid) {
-        constexpr int kBytes = NG * VB / 2;
-        if constexpr (kBytes > 16 && kBytes % 16 == 0) {
+    __device__ static __forceinline__ void load_v(W& v, uint32_t at, int rows) {
+        if constexpr (NG * VB / 2 > 16) {
 #pragma unroll
-            for (int i = 0; i < kBytes / 16; ++i) v.load16(codes + v_place(r, gid * (kBytes / 16) + i), 4 * i);
-        } else if constexpr (NG == 3) {
-            v.load(codes + r * kVRow + gid * kBytes);
+            for (int i = 0; i < NG * VB / 32; ++i) v.load16((at ^ (i * 16)) + rows * kVRow, 4 * i);
         } else {
-            v.load(codes + v_place(r, gid * kBytes / 16) + gid * kBytes % 16);
+            v.load(at + rows * kVRow);
         }
     }
 
@@ -711,34 +868,44 @@ struct Attend {
                 for (int d = 4; d <= 16; d <<= 1) w.sum[nt][e] += __shfl_xor_sync(~0u, w.sum[nt][e], d);
                 if (gid == 0) {
                     float* const to = ml + col_of(nt, 2 * tig + e) * 2;
-                    to[0] = w.top[nt][e], to[1] = w.sum[nt][e];
+                    to[0] = w.ref[nt][e], to[1] = w.sum[nt][e];
                 }
             }
     }
     // Its normalised result for columns c0 .. c0 + kRoundCols - 1 into o [kRoundCols][D].
     __device__ static __forceinline__ void leave(const Warp& w, uint32_t o, int c0) {
         const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-        // the accumulators are in units of 2^(exponent - 6)
+        // the accumulators are in units of 2^(exponent - 6) kValueUnit, the sums in units of 2^-kShift
         const float up = __int_as_float(w.scale_exp << 23);
+        uint32_t poison = w.poison;
+        if constexpr (!kF32) {
+            poison |= __shfl_xor_sync(~0u, poison, 1);
+            poison |= __shfl_xor_sync(~0u, poison, 2);
+        }
 #pragma unroll
         for (int nt = 0; nt < (kF32 ? 1 : NT); ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int col = col_of(nt, 2 * tig + e) - c0;
-                if (col < 0 || col >= kRoundCols) continue;
-                const float sum = w.sum[nt][e], by = sum == 0.0f ? 0.0f : 0x1p-6f / sum;
+                const float sum = w.sum[nt][e], by = sum == 0.0f ? 0.0f : (kF32 ? 0x1p-6f : 0x1p-3f) / kValueUnit / sum;
+                const uint32_t bad = __shfl_sync(~0u, poison, (2 * tig + e) * 4);
 #pragma unroll
                 for (int u = 0; u < NG; ++u) {
+                    // what the values' centre comes to
+                    const float centre = kF32 ? 0.0f : (VB == 4 ? 8.0f : 128.0f) * kValueUnit * __shfl_sync(~0u, w.ones[nt][e], u * 4 + tig);
                     float x[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int j = 2 * u + (i >> 1), at = (i & 1) * 2 + e;
-                        const float y = kF32 ? w.o[0][j][at] + w.o[NT - 1][j][at] : w.o[nt][j][at];
-                        x[i] = y * by * (VB == 4 && (i & 1) ? 0.0625f : 1.0f) * up;
+                        const float times = VB == 4 && (i & 1) ? 16.0f : 1.0f;
+                        const float y = kF32 ? w.o[0][j][at] + w.o[NT - 1][j][at] : w.o[nt][j][at] - times * centre;
+                        x[i] = y * (by / times) * up;
+                        if (!kF32 && ((bad >> (nt * NG + u)) & 1u)) x[i] = __int_as_float(0x7fc00000);
                     }
-                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(o + (col * D + u * kGroup + gid * 4) * 4), "f"(x[0]), "f"(x[1]), "f"(x[2]),
-                                 "f"(x[3])
-                                 : "memory");
+                    if (col >= 0 && col < kRoundCols)
+                        asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(o + (col * D + u * kGroup + gid * 4) * 4), "f"(x[0]), "f"(x[1]),
+                                     "f"(x[2]), "f"(x[3])
+                                     : "memory");
                 }
             }
     }
@@ -831,26 +998,38 @@ struct Cut {
     }
 };
 
-// A place in a CTA's run of tiles: tiles tile .. end - 1 of the pair (b, g, ct) are its next ones.
+// A place in a CTA's run of tiles: tiles tile .. end - 1 of the pair (b, g, ct), whose first is token `first` of the sequence's n, are its next ones.
+// What is only needed from pair to pair lies in shared memory, one for each warp (all lanes write the same).
+struct Pair {
+    int b, g, ct, tiles;
+    int left;  // tiles of the run, from the pair's first of them on
+};
 template <int TOK>
 struct Walk {
-    int b, g, ct, n, first, tiles, tile, end;
-    int64_t left;  // tiles of the run, from `tile` on
+    int n, first, tile, end;
 
-    __device__ __forceinline__ void at_sequence(const AttendParams& p) {
-        n = attended<TOK>(p, b, first);
-        tiles = max(1, (n - first + TOK - 1) / TOK);
+    __device__ __forceinline__ void enter(const AttendParams& p, Pair& at) {  // a sequence; `tile` and at.left are set
+        n = attended<TOK>(p, at.b, first);
+        at.tiles = max(1, (n - first + TOK - 1) / TOK);
+        end = min(at.tiles, tile + at.left);
     }
-    __device__ __forceinline__ void limit() { end = static_cast<int>(min(static_cast<int64_t>(tiles), tile + left)); }
-    __device__ __forceinline__ bool next(const AttendParams& p) {
-        left -= end - tile;
-        if (left <= 0) return false;
+    __device__ __forceinline__ bool next(const AttendParams& p, Pair* in) {
+        Pair at = *in;
+        at.left -= end - tile;
+        if (at.left <= 0) return false;
         tile = 0;
-        if (++ct == p.col_tiles) {
-            ct = 0;
-            if (++g == p.c.G) g = 0, ++b, at_sequence(p);
+        if (++at.ct == p.col_tiles) {
+            at.ct = 0;
+            if (++at.g == p.c.G) {
+                at.g = 0, ++at.b;
+                n = attended<TOK>(p, at.b, first);
+                at.tiles = max(1, (n - first + TOK - 1) / TOK);
+            }
         }
-        limit();
+        end = min(at.tiles, at.left);
+        __syncwarp();
+        *in = at;
+        __syncwarp();
         return true;
     }
 };
@@ -862,61 +1041,73 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
     extern __shared__ __align__(128) uint8_t smem[];
     float* const ml = reinterpret_cast<float*>(smem + A::kRing);
     uint32_t* const left_at = reinterpret_cast<uint32_t*>(smem + A::kRing + A::kMl);
+    __shared__ typename A::Column columns[A::kCols];
+    __shared__ Pair now[W], ahead_at[W];
     const int warp = threadIdx.x >> 5;
     const uint32_t ring = smem_u32(smem) + warp * S * A::kStage;
     grid_dependency_wait();
 
     // This CTA's run of tiles, and which of a pair's tiles are this warp's.
     Walk<kTok> w;
+    Pair at;
     int step = W, skip = warp;
     if (p.cluster > 0) {
-        const int at = blockIdx.x / p.cluster, each = p.c.G * p.col_tiles;
-        w.b = at / each, w.tile = 0;
-        w.g = (at - w.b * each) / p.col_tiles, w.ct = at - w.b * each - w.g * p.col_tiles;
-        w.at_sequence(p);
-        w.left = w.tiles;
+        const int in_all = blockIdx.x / p.cluster, each = p.c.G * p.col_tiles;
+        at.b = in_all / each;
+        const int pair = in_all - at.b * each;
+        at.g = pair / p.col_tiles, at.ct = pair - at.g * p.col_tiles;
+        at.left = 0x7fffffff;
+        w.tile = 0;
+        w.enter(p, at);
+        at.left = at.tiles;
+        w.end = at.tiles;
         step *= p.cluster;
-        skip += W * (blockIdx.x - at * p.cluster);
+        skip += W * (blockIdx.x - in_all * p.cluster);
     } else {
         const auto cut = Cut<kTok, kThreads>::make(p, reinterpret_cast<int64_t*>(smem));
         const int64_t from = cut.start(blockIdx.x, gridDim.x);
-        w.left = cut.start(blockIdx.x + 1, gridDim.x) - from;
-        int64_t first;
-        w.b = cut.sequence_of(p, from, first);
-        w.at_sequence(p);
-        const int pair = static_cast<int>((from - first) / w.tiles);
-        w.tile = static_cast<int>((from - first) - static_cast<int64_t>(pair) * w.tiles);
-        w.g = pair / p.col_tiles, w.ct = pair - w.g * p.col_tiles;
+        at.left = static_cast<int>(cut.start(blockIdx.x + 1, gridDim.x) - from);
+        int64_t start;
+        at.b = cut.sequence_of(p, from, start);
+        w.tile = 0;
+        w.enter(p, at);
+        const int pair = static_cast<int>((from - start) / at.tiles);
+        w.tile = static_cast<int>((from - start) - static_cast<int64_t>(pair) * at.tiles);
+        w.end = min(at.tiles, w.tile + at.left);
+        at.g = pair / p.col_tiles, at.ct = pair - at.g * p.col_tiles;
         __syncthreads();  // (the scan lies where the ring does)
     }
-    if (w.left <= 0) return;
-    w.limit();
+    if (at.left <= 0) return;
+    now[warp] = ahead_at[warp] = at;
+    __syncwarp();
 
     // Copies run ahead of the arithmetic, across pairs too: `ahead` is the place of the next tile to be copied, `row` where this lane's token of it lies
     // (contiguous: only the pair's first row is kept).
     Walk<kTok> ahead = w;
     int tile = ahead.tile + skip, seen = first_seen(p, ahead.n);
     const bool paged = p.c.block_table != nullptr;
-    int64_t row = paged ? 0 : row_of(p.c, ahead.b, ahead.g, 0, nullptr);
+    int64_t row = paged ? 0 : row_of(p.c, at.b, at.g, 0, nullptr);
     bool more = true;
     const auto look = [&] {
         while (tile >= ahead.end) {
-            if (!ahead.next(p)) {
+            if (!ahead.next(p, ahead_at + warp)) {
                 more = false;
                 return;
             }
             tile = ahead.tile + skip;
             seen = first_seen(p, ahead.n);
-            if (!paged) row = row_of(p.c, ahead.b, ahead.g, 0, nullptr);
+            if (!paged) row = row_of(p.c, ahead_at[warp].b, ahead_at[warp].g, 0, nullptr);
         }
-        if (paged) row = A::find(p, ahead.b, ahead.g, ahead.first + tile * kTok, seen, ahead.n);
+        if (paged) row = A::find(p, ahead_at[warp].b, ahead_at[warp].g, ahead.first + tile * kTok, seen, ahead.n);
     };
+    typename A::Lane l;
+    l.set();
     uint32_t there[S];  // [0]: of the stage that is next in the arithmetic
     const auto copy = [&](int slot) {
         uint32_t is = 0;
         if (more) {
             const uint32_t to = ring + slot * A::kStage;
-            is = paged ? A::copy_paged(p, to, row) : A::copy_run(p, to, row, ahead.first + tile * kTok, seen, ahead.n);
+            is = paged ? A::copy_paged(p, l, to, row) : A::copy_run(p, l, to, row, ahead.first + tile * kTok, seen, ahead.n);
             tile += step;
             look();
         }
@@ -931,13 +1122,12 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
     int slot = 0;
     bool first_of_run = true;
     for (;;) {
-        const int g = w.g, ct = w.ct;
-        A::begin(p, q, w.b, g, ct, w.n);
+        A::begin(p, q, columns, now[warp].b, now[warp].g, now[warp].ct, w.n);
         for (int t = w.tile + skip; t < w.end; t += step) {
             copy_wait<S - 2>();
             __syncwarp();
             there[S - 1] = copy(slot == 0 ? S - 1 : slot - 1);
-            A::fold(p, q, ring + slot * A::kStage, w.first + t * kTok, there[0]);
+            A::fold(p, l, q, columns, ring + slot * A::kStage, w.first + t * kTok, there[0]);
 #pragma unroll
             for (int i = 0; i < S - 1; ++i) there[i] = there[i + 1];
             slot = slot == S - 1 ? 0 : slot + 1;
@@ -947,7 +1137,8 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
         __syncwarp();
         A::leave_sums(q, ml + warp * A::kCols * 2);
         if ((threadIdx.x & 31) == 0) left_at[warp] = mine;
-        const bool whole = p.cluster == 1 || (p.cluster == 0 && w.tile == 0 && w.end == w.tiles);
+        const int b = now[warp].b, g = now[warp].g, ct = now[warp].ct;
+        const bool whole = p.cluster == 1 || (p.cluster == 0 && w.tile == 0 && w.end == now[warp].tiles);
         const int used = min(p.m * p.R - ct * A::kCols, A::kCols);
         constexpr int kQuads = A::kRoundCols * D / 4, kPer = (kQuads + kThreads - 1) / kThreads;
         float kept[A::kRounds * kPer][4];
@@ -980,7 +1171,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
                     for (int e = 0; e < 4; ++e) x[e] *= by;
                     kept_lse[r * kPer + k] = total == 0.0f ? kNegInf : ref + log2f(total);
                     if (whole) {
-                        A::store(A::out_row(p, w.b, g, ct * A::kCols + col) + d, x);
+                        A::store(A::out_row(p, b, g, ct * A::kCols + col) + d, x);
                     } else if (p.cluster == 0) {
                         const int64_t at = 2ll * blockIdx.x + (first_of_run ? 0 : 1);
                         *reinterpret_cast<float4*>(p.ws_o + (at * A::kCols + col) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
@@ -1019,13 +1210,13 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
                     x0 += l * y.x, x1 += l * y.y;
                 }
                 const float by = total == 0.0f ? 0.0f : 1.0f / total;
-                T* const out = A::out_row(p, w.b, g, ct * A::kCols + col) + d;
+                T* const out = A::out_row(p, b, g, ct * A::kCols + col) + d;
                 out[0] = Elt<T>::from_float(x0 * by), out[1] = Elt<T>::from_float(x1 * by);
             }
             cluster_sync();  // nobody leaves while its results are read
         }
         first_of_run = false;
-        if (p.cluster > 0 || !w.next(p)) break;
+        if (p.cluster > 0 || !w.next(p, now + warp)) break;
     }
     copy_wait<0>();
 }

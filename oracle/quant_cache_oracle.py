@@ -65,15 +65,20 @@ def attention(q, k, v, scale, softcap=0.0, window=0, slopes=None):
 def tolerance(out, mean, size, n, dtype: str, extra: float = 0.0, largest: float = 0.0):
     """How far an output element may be off, from the formulas' roundings:
     - the output's own rounding: half a step, 2^-8 (bfloat16) or 2^-24 of the value;
-    - a probability times a value scale is held in 11 (fp32: 22) bits: 2^-11 (2^-21) of the mean magnitude;
-    - a score is a sum in fp32 of products of whole codes up to twice (4 bits: 15 / 7) what they stand for: 2^-20 of the sum of magnitudes
-      `size` twice over, which scales probabilities above and below the line;
-    - the sums over n tokens in fp32, 16 tokens at a time: 2^-23 of the mean magnitude each, and as much for their reunion.
+    - a probability is rounded to 11 bits, and so is its product with a value scale: 2^-10 of the mean magnitude (fp32: 22 bits once, 2^-21);
+    - a score is sums over groups of products with codes.  The tensor core adds 16 products and what it had, each cut off 24 bits below the
+      largest, twice per group: 34 * 2^-24 of it.  bfloat16: codes as stored, up to 15 where the value's is 7, with 4 bits less: 34 * 2^-20 * 15 / 7.
+      The largest product is at most `size`.  It scales probabilities above and below the line;
+    - sums over n tokens, 16 at a time: 2^-23 of the sum each, and as much for their reunion.  bfloat16: of codes as stored and of their centre, together
+      up to (15 + 8) / 7 of the largest value (17 addends of 2^-20 each are within that where probabilities are even, and below the roundings above
+      where they are not).
     `extra` is an absolute error of scores beyond that (bias, cap).
     - fp16 numbers below 2^-14 lie 2^-24 apart.  A probability (relative to a score that was seen, so their sum is at least 1) times a
       value scale s is held as a multiple p s / 2^(E - 6), 2^E <= the largest scale: off by up to half of 2^-24 * 2^(E - 6) = 2^-31 2^E beyond the
       relative error, times a code up to L, over a sum of at least 1.  L 2^E <= `largest`, the largest magnitude held: 2^-31 * largest per token.
       (It shows where one token has nearly all the weight and a code of zero, and what is left is below 2^-31 of the values.)"""
-    half, held_in = (2.0 ** -8, 2.0 ** -11) if dtype == "bf16" else (2.0 ** -24, 2.0 ** -21)
-    score = 2.0 ** -20 * 2.2 * size + extra
-    return half * np.abs(out) + (held_in + 2 * score + 2.0 ** -23 * (n / 16 + 32)) * mean + n * 2.0 ** -31 * largest
+    bf16 = dtype == "bf16"
+    half, held_in = (2.0 ** -8, 2.0 ** -10) if bf16 else (2.0 ** -24, 2.0 ** -21)
+    score = 34 * (2.0 ** -20 * 15 / 7 if bf16 else 2.0 ** -24) * size + extra
+    summed = 2.0 ** -23 * (n / 16 + 32) * (largest * 23 / 7 if bf16 else mean)
+    return half * np.abs(out) + (held_in + 2 * score) * mean + summed + n * 2.0 ** -31 * largest
