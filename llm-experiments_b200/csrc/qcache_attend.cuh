@@ -4,23 +4,24 @@
 // arithmetic has to be hidden behind 23 bytes per clock and SM, and with 4 bits 46 elements per clock have to be widened.  Plain
 // fp32 arithmetic cannot (128 FMAs per clock and SM, one per element and query head); the tensor cores can, if widening is cheap:
 //
-//   * Codes become fp16 numbers by masking alone: a code c in bits 2 .. 5 or 6 .. 9 of a 16-bit half is the fp16 subnormal c * 2^-22 or c * 2^-18, two
+//   * Keys' codes become fp16 numbers by masking alone: a code c in bits 2 .. 5 or 6 .. 9 of a 16-bit half is the fp16 subnormal c * 2^-22 or c * 2^-18, two
 //     codes per instruction, and tensor cores take subnormals at full speed.  They add products by the exponents as they stand, so
 //     that a number whose first bit is k places below the tenth loses k bits of the sum: at most 4 here, which is why units of 4-bit codes are kept
-//     turned by two bits (bits 0 .. 3 and 4 .. 7 would lose 7 and 3).
+//     turned by two bits (bits 0 .. 3 and 4 .. 7 would lose 7 and 3).  Codes stay uncentred (c + 8, c + 128): what the centre comes to is a small product of
+//     the key scales and the query's sums over the groups, which the scores start from.  A group's sum is multiplied by its key scale in fp32.
+//   * Values' codes are put behind the exponent of 1024 by the mask's instruction, and the centre is taken off by a second one (a row of ones in the
+//     product does that too, but moving its operand into place costs as much, and over thousands of tokens the sums of uncentred codes grow far
+//     beyond what is left in the end).
 //   * Both products have the cache's rows as the operand of many rows: S[token, column] = K q (16 tokens by 8 columns per MMA, m16n8k16)
 //     and O[element, column] += V^T P.  A column is one (new token, query head) pair of the key / value head.  The cache's
 //     layout gives a lane the codes that it needs as one piece, the query is permuted to match, and P goes from the accumulator's
 //     layout to the operand's by an 8 x 8 transpose within the warp.  The rows go through tcgen05 only if they were first widened into
 //     shared memory at 16 bits per element, which is four times the traffic of reading them; as register operands they are widened in place.
-//   * Codes stay uncentred (c + 8, c + 128).  What the keys' centre comes to is a small product of the key scales and the query's sums over the
-//     groups, which the scores start from; the values' is a row of ones in their product.  A group's sum is multiplied by its key scale in fp32.
 //   * A probability is rounded to fp16, multiplied by its value scale there and rounded again (11 bits; the output has 8).  To keep that in range
 //     whatever the scales are, they are taken relative to the largest exponent so far, and the accumulators are rescaled when that
 //     grows: products stay below 2^15, and scales down to 2^-17 of the largest keep all their bits.
-//   * fp32 queries and weights are sums of two fp16 numbers (22 bits), in columns of their own; codes are put behind the exponent of 1024 by the
-//     mask's instruction and the centre is taken off by a second one; and only 16 tokens' products are added up in the tensor core, whose
-//     sums are cut off and not rounded.
+//   * fp32 queries and weights are sums of two fp16 numbers (22 bits), in columns of their own; keys are centred like values; and only 16 tokens'
+//     products are added up in the tensor core, whose sums are cut off and not rounded.
 //   * Softmax: scores in the log2 domain, references that move only when a score has outgrown its own by more than 2^8 (one vote per stage), sums per
 //     lane until the end, all in fp32.
 #pragma once
@@ -54,6 +55,11 @@ constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLowest = -3.0e38f;  // a reference where nothing was seen yet: any score has outgrown it, and differences stay finite
 constexpr int kScaleExpMin = 17;  // (biased) smaller exponents of value scales are taken for this one: 2^-110
 
+__device__ __forceinline__ int lane_id() {
+    int lane;
+    asm("mov.u32 %0, %%laneid;" : "=r"(lane));
+    return lane;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -165,7 +171,7 @@ struct Ring {
     static constexpr int kWarps = 8;
     static constexpr int kCtas = NT == 1 && NG <= 4 ? 2 : 1;
     static constexpr int kToken = NG * 4 * (KB + VB) + 4 * scale_row(NG);
-    static constexpr int kRoom = (kCtas == 2 ? 113 : 225) * 1024 / kWarps;
+    static constexpr int kRoom = ((kCtas == 2 ? 112 : 224) * 1024 - NG * NT * 512 - NT * 512) / kWarps;  // (beside the queries, and a few hundred bytes more)
     static constexpr int kTokens = 3 * 32 * kToken <= kRoom ? 32 : 16;
     static constexpr int kFit = kRoom / (kTokens * kToken);
     static constexpr int kStages = kFit > 6 ? 6 : kFit;
@@ -190,7 +196,7 @@ struct Attend {
     static constexpr int kRounds = kCols / kRoundCols;
     static_assert(kRoundCols * D * 4 <= kStage && kRoundCols % 2 == 0, "");
     static constexpr int kMl = WARPS * kCols * 2 * 4;
-    static constexpr int kSmem = kRing + kMl + WARPS * 4;
+    static constexpr int kSmem = kRing + kMl + 16 * ((WARPS * 4 + 15) / 16) + NG * NT * 512;
     // The centre of the keys costs -kKOff * sum over groups of (key scale) * (sum of the group's query): a product over the groups, the sums
     // in three bfloat16 parts (16 places: part k / kSG of group k % kSG; with 8 groups in two products).
     static constexpr int kSG = scale_row(NG), kOffs = kF32 ? 1 : kSG == 8 ? 4 : 2;
@@ -198,7 +204,7 @@ struct Attend {
     static constexpr float kKeyUnit = (KB == 4 ? 4.0f : 1.0f) * (kF32 ? 1.0f : 0x1p-24f);
     // Weights are probabilities times 2^kShift, up to 2^(8 + kShift); times a value scale, 2^(6 - exponent) times that at most: below 2^15.
     static constexpr int kShift = kF32 ? 0 : 3;
-    static constexpr float kValueUnit = (VB == 4 ? 4.0f : 1.0f) * (kF32 ? 1.0f : 0x1p-24f);  // of a code of one; every other row of 4 bits has 16 times that
+    static constexpr float kValueUnit = VB == 4 ? 4.0f : 1.0f;  // of a code of one; every other row of 4 bits has 16 times that
 
     // Where 16-byte piece ch of row r lies in a stage: moved about so that the lanes that read together meet different banks.
     __device__ static __forceinline__ int k_place(int r, int ch) {
@@ -218,16 +224,15 @@ struct Attend {
     // the moving about.
     struct Lane {
         uint32_t k;         // its piece of row gid of the keys
-        uint32_t v[2];      // its pieces of rows 2 tig and 2 tig + 1 of the values
+        uint32_t v;         // its piece of row 2 tig of the values
         uint32_t put_k, put_v;  // its first 16-byte piece of a copy
+        // Its piece of row 2 tig + 1: the rows in between were moved about alike.
+        __device__ __forceinline__ uint32_t v_next() const { return NG == 3 ? v + kVRow : v ^ kVRow; }
         __device__ __forceinline__ void set() {
-            const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+            const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
             k = NG == 3 ? gid * kKRow + tig * NG * KB : k_place(gid, tig * NG * KB / 16) + tig * NG * KB % 16;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = 2 * tig + i, at = gid * (NG * VB / 2);
-                v[i] = kKBytes + (NG == 3 ? r * kVRow + at : v_place(r, at / 16) + at % 16);
-            }
+            const int at = gid * (NG * VB / 2);
+            v = NG == 3 ? 2 * tig * kVRow + at : v_place(2 * tig, at / 16) + at % 16;
             put_k = k_place(lane / (kKRow / 16), lane % (kKRow / 16));
             put_v = kKBytes + v_place(lane / (kVRow / 16), lane % (kVRow / 16));
         }
@@ -245,15 +250,12 @@ struct Attend {
     };
 
     struct Warp {
-        uint32_t q[NT][NG][2][2];  // the query as the second operand of S = K q
         uint32_t off[NT][kOffs];   // what the key's centre comes to, as the second operand of a product with the key scales (not for fp32)
         float f[NT][2];            // the same where there is neither cap nor bias, else 1
         int all_lo, all_lim;       // tokens that every used column sees
         float o[NT][NG * 2][4];    // elements 32 (j / 2) + 4 gid + 2 (j & 1) (+1 in the last two), columns 2 tig, 2 tig + 1
         float ref[NT][2];          // scores are taken relative to this: what was the largest so far, less kShift
         float sum[NT][2];          // of 2^(score - ref), this lane's tokens
-        float ones[NT][4];         // sums of a column's weights per group, row = group (not for fp32)
-        uint32_t poison;           // groups whose value scale was NaN, of column gid (not for fp32)
         int scale_exp;
         bool fresh;                // some column may not have seen anything yet
     };
@@ -268,8 +270,8 @@ struct Attend {
     __device__ static void load8(const __nv_bfloat16* p, float (&x)[8]) { Elt<__nv_bfloat16>::widen(*reinterpret_cast<const uint4*>(p), x); }
 
     // Queries of sequence b, head g, column tile ct, and what goes with them.  n: tokens of the sequence.
-    __device__ static __forceinline__ void begin(const AttendParams& p, Warp& w, Column* columns, int b, int g, int ct, int n) {
-        const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+    __device__ static __forceinline__ void begin(const AttendParams& p, Warp& w, uint4* queries, Column* columns, int b, int g, int ct, int n) {
+        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         const int used = p.m * p.R;
         w.all_lo = 0, w.all_lim = 0x7fffffff;
 #pragma unroll
@@ -303,6 +305,7 @@ struct Attend {
 #pragma unroll
             for (int u = 0; u < NG; ++u) {
                 part[u] = 0.0f;
+                uint32_t high[4], low[4];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[u][e] *= down;
                 // elements in the order of the codes in a word's halves: 4 bits (0,4) (1,5) (2,6) (3,7), the odd ones 16 times too
@@ -313,12 +316,15 @@ struct Attend {
                     const float a = x[u][KB == 4 ? j : 2 * j] * by, c = x[u][KB == 4 ? j + 4 : 2 * j + 1] * by;
                     const uint32_t h = pack_half(a, c);
                     const float2 got = unpack_half(h);
-                    w.q[nt][u][j >> 1][j & 1] = h;
+                    high[j] = h;
                     part[u] += (got.x + got.y) / by;
                     if constexpr (kF32) {
-                        w.q[1][u][j >> 1][j & 1] = pack_half(a - got.x, c - got.y);
+                        low[j] = pack_half(a - got.x, c - got.y);
                     }
                 }
+                // the query as the second operand of S = K q, both steps of a group (every warp of the CTA writes the same)
+                queries[(nt * NG + u) * 32 + lane] = make_uint4(high[0], high[1], high[2], high[3]);
+                if constexpr (kF32) queries[(NG + u) * 32 + lane] = make_uint4(low[0], low[1], low[2], low[3]);
             }
             if constexpr (!kF32) {
                 float sum[NG];
@@ -370,24 +376,21 @@ struct Attend {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w.o[nt][j][e] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w.ones[nt][e] = 0.0f;
-#pragma unroll
             for (int e = 0; e < 2; ++e) w.ref[nt][e] = kLowest, w.sum[nt][e] = 0.0f;
         }
-        w.poison = 0;
         w.fresh = true;
         w.scale_exp = kScaleExpMin;
     }
 
     // Where a lane's token of a tile lies: its row, -1 where there is none or no query sees it.
     __device__ static __forceinline__ int64_t find(const AttendParams& p, int b, int g, int t0, int seen, int n) {
-        const int lane = threadIdx.x & 31, t = t0 + (lane & (kTok - 1));
+        const int lane = lane_id(), t = t0 + (lane & (kTok - 1));
         return t < n && t >= seen ? row_of(p.c, b, g, t, p.dev_status) : -1;
     }
 
     // Starts the copies of a tile whose rows `find` gave (zeros where there is none); a bit for each token that is there.
     __device__ static __forceinline__ uint32_t copy_paged(const AttendParams& p, const Lane& l, uint32_t stage, int64_t row) {
-        const int lane = threadIdx.x & 31;
+        const int lane = lane_id();
         const uint32_t there = __ballot_sync(~0u, row >= 0);
         const int64_t at = row >= 0 ? row : 0;
         const uint32_t ks = stage + kKBytes + kVBytes;
@@ -402,7 +405,7 @@ struct Attend {
     template <int ROW, typename F>
     __device__ static __forceinline__ void pieces_paged(uint32_t dst, const uint8_t* src, int64_t mine, uint32_t there, F&& moved) {
         constexpr int kCh = ROW / 16, kPieces = kCh * kTok, kPer = (kPieces + 31) / 32;
-        const int lane = threadIdx.x & 31;
+        const int lane = lane_id();
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int idx = i * 32 + lane, r = idx / kCh, ch = idx - r * kCh;
@@ -413,7 +416,7 @@ struct Attend {
 
     // The same for rows that follow one another, the sequence's first one at row `row`: tokens t0 .., those from `seen` to n - 1.
     __device__ static __forceinline__ uint32_t copy_run(const AttendParams& p, const Lane& l, uint32_t stage, int64_t row, int t0, int seen, int n) {
-        const int lane = threadIdx.x & 31;
+        const int lane = lane_id();
         const int64_t at = row + t0;
         const uint32_t ks = stage + kKBytes + kVBytes + lane * kSRow;
         const uint8_t* const k = static_cast<const uint8_t*>(p.c.k_codes) + at * kKRow;
@@ -444,7 +447,7 @@ struct Attend {
     template <int ROW, bool kAll, typename F>
     __device__ static __forceinline__ void pieces_run(uint32_t dst, const uint8_t* src, uint32_t there, F&& moved) {
         constexpr int kCh = ROW / 16, kPieces = kCh * kTok, kPer = (kPieces + 31) / 32;
-        const int lane = threadIdx.x & 31;
+        const int lane = lane_id();
         const uint8_t* const from = src + lane * 16;
         const uint8_t* const some = src + (there != 0 ? __ffs(there) - 1 : 0) * ROW;  // a row that is there, for the address of those that are not
 #pragma unroll
@@ -461,9 +464,10 @@ struct Attend {
         }
     }
 
-    // Codes as fp16 numbers: of bits 2 .. 5 and 6 .. 9 of 16-bit halves, or of two bytes.  As stored for bfloat16, centred for fp32.
+    // Codes as fp16 numbers, as stored or centred: of bits 2 .. 5 and 6 .. 9 of 16-bit halves, or of two bytes.
+    template <bool kCentred>
     __device__ static __forceinline__ void pieces4(uint32_t x, uint32_t& low, uint32_t& high) {
-        if constexpr (kF32) {
+        if constexpr (kCentred) {
             low = half_sub(and_or(x, 0x003c003cu, 0x64006400u), 0x64206420u);   // 1024 + 4 c less 1024 + 32
             high = half_sub(and_or(x, 0x03c003c0u, 0x64006400u), 0x66006600u);  // 1024 + 64 c less 1024 + 512
         } else {
@@ -471,77 +475,89 @@ struct Attend {
             high = x & 0x03c003c0u;
         }
     }
+    template <bool kCentred>
     __device__ static __forceinline__ uint32_t piece8(uint32_t x, int sel) {
-        return kF32 ? half_sub(__byte_perm(x, 0x64646464u, sel), 0x64806480u) : __byte_perm(x, 0, sel);
+        return kCentred ? half_sub(__byte_perm(x, 0x64646464u, sel), 0x64806480u) : __byte_perm(x, 0, sel);
     }
 
     // A row's codes of half a group as operand pieces (a0 and a2, or a1 and a3).
     template <int STEP>
     __device__ static __forceinline__ void k_piece(const uint32_t* w, uint32_t& first, uint32_t& second) {
         if constexpr (KB == 4) {
-            pieces4(STEP == 0 ? w[0] : __funnelshift_r(w[0], w[0], 8), first, second);
+            pieces4<kF32>(STEP == 0 ? w[0] : __funnelshift_r(w[0], w[0], 8), first, second);
         } else {
-            first = piece8(w[STEP], 0x4140);
-            second = piece8(w[STEP], 0x4342);
+            first = piece8<kF32>(w[STEP], 0x4140);
+            second = piece8<kF32>(w[STEP], 0x4342);
         }
     }
 
     // The tokens of a stage, t0 the first.
-    __device__ static __forceinline__ void fold(const AttendParams& p, const Lane& l, Warp& w, const Column* columns, uint32_t stage, int t0, uint32_t there) {
-        const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+    __device__ static __forceinline__ void fold(const AttendParams& p, const Lane& l, Warp& w, const uint4* queries, const Column* columns, uint32_t stage, int t0, uint32_t there) {
+        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         const uint32_t ks = stage + kKBytes + kVBytes, vs = ks + kSBytes;
         constexpr int kKPiece = NG * KB;   // bytes of a row that a lane reads
         constexpr int NS = kF32 ? 1 : NT;  // tiles of scores
         float s[MT][NS][4];
+        {
+            Words<kKPiece> k[MT][2];
+            Words<kSRow> scales[MT][2];
+            float acc[MT][NT][4];
 #pragma unroll
-        for (int h = 0; h < MT; ++h) {
-            const int r = h * 16 + gid;
-            Words<kKPiece> k0, k1;
-            load_k(k0, stage + l.k, h * 16);
-            load_k(k1, stage + l.k, h * 16 + 8);
-            Words<kSRow> s0, s1;
-            s0.load(ks + r * kSRow);
-            s1.load(ks + (r + 8) * kSRow);
-            float acc[NT][4];
+            for (int h = 0; h < MT; ++h) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
-            if constexpr (!kF32) {
-                uint32_t a0, a1;  // key scales of the two rows, groups 2 tig and 2 tig + 1 of as many as there are
-                const uint32_t at = ks + r * kSRow + tig % (kSG / 2) * 4;
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(a0) : "r"(at) : "memory");
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(a1) : "r"(at + 8 * kSRow) : "memory");
+                for (int i = 0; i < 2; ++i) {
+                    load_k(k[h][i], stage + l.k, h * 16 + i * 8);
+                    scales[h][i].load(ks + (h * 16 + i * 8 + gid) * kSRow);
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int i = 0; i < kOffs; i += 2) mma_bf16(acc[nt], a0, a1, a0, a1, w.off[nt][i], w.off[nt][i + 1]);
-            }
+                    for (int e = 0; e < 4; ++e) acc[h][nt][e] = 0.0f;
+                if constexpr (!kF32) {
+                    uint32_t a0, a1;  // key scales of the two rows, groups 2 tig and 2 tig + 1 of as many as there are
+                    const uint32_t at = ks + (h * 16 + gid) * kSRow + tig % (kSG / 2) * 4;
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(a0) : "r"(at) : "memory");
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(a1) : "r"(at + 8 * kSRow) : "memory");
 #pragma unroll
-            for (int u = 0; u < NG; ++u) {
-                uint32_t a[2][4];
-                constexpr int kW = KB / 4;  // words of a lane's piece of a group
-                k_piece<0>(k0.w + u * kW, a[0][0], a[0][2]);
-                k_piece<0>(k1.w + u * kW, a[0][1], a[0][3]);
-                k_piece<1>(k0.w + u * kW, a[1][0], a[1][2]);
-                k_piece<1>(k1.w + u * kW, a[1][1], a[1][3]);
-                const float f0 = __uint_as_float(u & 1 ? s0.w[u >> 1] & 0xffff0000u : s0.w[u >> 1] << 16);
-                const float f1 = __uint_as_float(u & 1 ? s1.w[u >> 1] & 0xffff0000u : s1.w[u >> 1] << 16);
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float d[4];
-                    mma_new(d, a[0][0], a[0][1], a[0][2], a[0][3], w.q[nt][u][0][0], w.q[nt][u][0][1]);
-                    mma(d, a[1][0], a[1][1], a[1][2], a[1][3], w.q[nt][u][1][0], w.q[nt][u][1][1]);
-                    acc[nt][0] = fmaf(f0, d[0], acc[nt][0]);
-                    acc[nt][1] = fmaf(f0, d[1], acc[nt][1]);
-                    acc[nt][2] = fmaf(f1, d[2], acc[nt][2]);
-                    acc[nt][3] = fmaf(f1, d[3], acc[nt][3]);
+                        for (int i = 0; i < kOffs; i += 2) mma_bf16(acc[h][nt], a0, a1, a0, a1, w.off[nt][i], w.off[nt][i + 1]);
                 }
             }
 #pragma unroll
-            for (int nt = 0; nt < NS; ++nt)
+            for (int u = 0; u < NG; ++u) {
+                uint4 q[NT];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[h][nt][e] = kF32 ? acc[0][e] + acc[NT - 1][e] : acc[nt][e];
+                for (int nt = 0; nt < NT; ++nt) q[nt] = queries[(nt * NG + u) * 32 + lane];
+#pragma unroll
+                for (int h = 0; h < MT; ++h) {
+                    uint32_t a[2][4];
+                    constexpr int kW = KB / 4;  // words of a lane's piece of a group
+                    k_piece<0>(k[h][0].w + u * kW, a[0][0], a[0][2]);
+                    k_piece<0>(k[h][1].w + u * kW, a[0][1], a[0][3]);
+                    k_piece<1>(k[h][0].w + u * kW, a[1][0], a[1][2]);
+                    k_piece<1>(k[h][1].w + u * kW, a[1][1], a[1][3]);
+                    const uint32_t s0 = scales[h][0].w[u >> 1], s1 = scales[h][1].w[u >> 1];
+                    const float f0 = __uint_as_float(u & 1 ? s0 & 0xffff0000u : s0 << 16);
+                    const float f1 = __uint_as_float(u & 1 ? s1 & 0xffff0000u : s1 << 16);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float d[4];
+                        mma_new(d, a[0][0], a[0][1], a[0][2], a[0][3], q[nt].x, q[nt].y);
+                        mma(d, a[1][0], a[1][1], a[1][2], a[1][3], q[nt].z, q[nt].w);
+                        acc[h][nt][0] = fmaf(f0, d[0], acc[h][nt][0]);
+                        acc[h][nt][1] = fmaf(f0, d[1], acc[h][nt][1]);
+                        acc[h][nt][2] = fmaf(f1, d[2], acc[h][nt][2]);
+                        acc[h][nt][3] = fmaf(f1, d[3], acc[h][nt][3]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < MT; ++h)
+#pragma unroll
+                for (int nt = 0; nt < NS; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[h][nt][e] = kF32 ? acc[h][0][e] + acc[h][NT - 1][e] : acc[h][nt][e];
         }
         if (p.softcap > 0.0f || p.slopes != nullptr) {
 #pragma unroll
@@ -632,7 +648,6 @@ struct Attend {
                     for (int k = 0; k < (kF32 ? 2 : 1); ++k) {
 #pragma unroll
                         for (int j = 0; j < NG * 2; ++j) w.o[nt + k][j][e] *= by, w.o[nt + k][j][e + 2] *= by;
-                        if constexpr (!kF32) w.ones[nt + k][e] *= by;
                     }
 #pragma unroll
                     for (int h = 0; h < MT; ++h) s[h][nt][e] -= top, s[h][nt][e + 2] -= top;
@@ -670,27 +685,25 @@ struct Attend {
             const float by = w.scale_exp - now < -126 ? 0.0f : __int_as_float((127 + w.scale_exp - now) << 23);
             w.scale_exp = now;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < NG * 2; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) w.o[nt][j][e] *= by;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w.ones[nt][e] *= by;
-            }
         }
         if constexpr (kF32)
             values_f32(l, w, stage, s, masked, hidden);
         else
-            values_bf16(l, w, stage, s, mine, nan, hidden);
+            values_bf16(l, w, stage, s, mine, nan, masked, hidden);
     }
 
     // O += V^T P for fp32: weights times value scales in 32 bits, then as two fp16 numbers.
     template <int NS>
     __device__ static __forceinline__ void values_f32(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NS][4], bool masked, uint32_t hidden) {
-        const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         const float vf = __int_as_float((260 - w.scale_exp) << 23);  // 2^(6 - exponent)
         const uint32_t vs = stage + kKBytes + kVBytes + kSBytes;
+        const uint32_t values_at[2] = {stage + kKBytes + l.v, stage + kKBytes + l.v_next()};
 #pragma unroll
         for (int h = 0; h < MT; ++h) {
             const int r = h * 16 + gid;
@@ -699,7 +712,7 @@ struct Attend {
             s1.load(vs + (r + 8) * kSRow);
             Words<NG * VB / 2> v[4];  // tokens 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_v(v[i], stage + l.v[i & 1], h * 16 + (i >> 1) * 8);
+            for (int i = 0; i < 4; ++i) load_v(v[i], values_at[i & 1], h * 16 + (i >> 1) * 8);
 #pragma unroll
             for (int u = 0; u < NG; ++u) {
                 const float f0 = vf * __uint_as_float(u & 1 ? s0.w[u >> 1] & 0xffff0000u : s0.w[u >> 1] << 16);
@@ -732,10 +745,11 @@ struct Attend {
     // are made fp16 (relative to the largest exponent) and brought into that order by the lane that has the token, in place.
     template <int NS>
     __device__ static __forceinline__ void values_bf16(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NS][4], const Words<kSRow>& mine, bool nan,
-                                                       uint32_t hidden) {
-        const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+                                                       bool hidden_any, uint32_t hidden) {
+        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         constexpr int kWords = kSG / 2;
         const uint32_t vs = stage + kKBytes + kVBytes + kSBytes;
+        const uint32_t values_at[2] = {stage + kKBytes + l.v, stage + kKBytes + l.v_next()};
         {
             const float vf = __int_as_float((257 - w.scale_exp) << 23);  // 2^(6 - kShift - exponent)
             uint32_t c[kWords];
@@ -773,7 +787,7 @@ struct Attend {
             sv.load(vs + (h * 4 + tig) * (2 * kSG * 4));
             Words<NG * VB / 2> v[4];  // tokens 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_v(v[i], stage + l.v[i & 1], h * 16 + (i >> 1) * 8);
+            for (int i = 0; i < 4; ++i) load_v(v[i], values_at[i & 1], h * 16 + (i >> 1) * 8);
             uint32_t weights[NS][2];
 #pragma unroll
             for (int nt = 0; nt < NS; ++nt)
@@ -786,29 +800,21 @@ struct Attend {
                 for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) b[nt][i] = half_mul(weights[nt][i], sv.w[i * kSG + u]);
-                if (nan) {
-                    // A NaN scale counts where its token is seen, and for its own group alone: it stays out of the products, which know
-                    // neither, and is put into the result at the end.
+                if (nan && hidden_any) {  // (0 times a NaN scale)
 #pragma unroll
                     for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const uint32_t bits = hidden >> ((h * NS + nt) * 4 + 2 * i);
-                            const uint32_t seen = transpose8x8((bits & 1u ? 0u : 0xffffu) | (bits & 2u ? 0u : 0xffff0000u));
-                            const uint32_t x = sv.w[i * kSG + u];
-                            const uint32_t bad = ((x & 0x7fffu) > 0x7c00u ? 0xffffu : 0u) | ((x & 0x7fff0000u) > 0x7c000000u ? 0xffff0000u : 0u);
-                            if ((bad & seen) != 0) w.poison |= 1u << (nt * NG + u);
-                            b[nt][i] &= ~bad;
+                            b[nt][i] &= transpose8x8((bits & 1u ? 0u : 0xffffu) | (bits & 2u ? 0u : 0xffff0000u));
                         }
                 }
                 uint32_t a[2][4];
                 v_pieces(v, u, a);
-                const uint32_t one = gid == u ? 0x3c003c00u : 0u;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     mma(w.o[nt][2 * u], a[0][0], a[0][1], a[0][2], a[0][3], b[nt][0], b[nt][1]);
                     mma(w.o[nt][2 * u + 1], a[1][0], a[1][1], a[1][2], a[1][3], b[nt][0], b[nt][1]);
-                    mma(w.ones[nt], one, 0, one, 0, b[nt][0], b[nt][1]);
                 }
             }
         }
@@ -822,17 +828,17 @@ struct Attend {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t x = __byte_perm(v[2 * i].w[u >> 1], v[2 * i + 1].w[u >> 1], sel), y = __byte_perm(x, 0, 0x2301);
-                pieces4(x, a[0][2 * i], a[0][2 * i + 1]);
-                pieces4(y, a[1][2 * i], a[1][2 * i + 1]);
+                pieces4<true>(x, a[0][2 * i], a[0][2 * i + 1]);
+                pieces4<true>(y, a[1][2 * i], a[1][2 * i + 1]);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t x = __byte_perm(v[2 * i].w[u], v[2 * i + 1].w[u], 0x5410), y = __byte_perm(v[2 * i].w[u], v[2 * i + 1].w[u], 0x7632);
-                a[0][2 * i] = piece8(x, 0x4240);
-                a[0][2 * i + 1] = piece8(x, 0x4341);
-                a[1][2 * i] = piece8(y, 0x4240);
-                a[1][2 * i + 1] = piece8(y, 0x4341);
+                a[0][2 * i] = piece8<true>(x, 0x4240);
+                a[0][2 * i + 1] = piece8<true>(x, 0x4341);
+                a[1][2 * i] = piece8<true>(y, 0x4240);
+                a[1][2 * i + 1] = piece8<true>(y, 0x4341);
             }
         }
     }
@@ -859,7 +865,7 @@ struct Attend {
 
     // This warp's reference and sum of each column into ml [kCols][2]; sums of all lanes are left in w.sum.
     __device__ static __forceinline__ void leave_sums(Warp& w, float* ml) {
-        const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
 #pragma unroll
         for (int nt = 0; nt < (kF32 ? 1 : NT); ++nt)
 #pragma unroll
@@ -874,33 +880,24 @@ struct Attend {
     }
     // Its normalised result for columns c0 .. c0 + kRoundCols - 1 into o [kRoundCols][D].
     __device__ static __forceinline__ void leave(const Warp& w, uint32_t o, int c0) {
-        const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         // the accumulators are in units of 2^(exponent - 6) kValueUnit, the sums in units of 2^-kShift
         const float up = __int_as_float(w.scale_exp << 23);
-        uint32_t poison = w.poison;
-        if constexpr (!kF32) {
-            poison |= __shfl_xor_sync(~0u, poison, 1);
-            poison |= __shfl_xor_sync(~0u, poison, 2);
-        }
 #pragma unroll
         for (int nt = 0; nt < (kF32 ? 1 : NT); ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int col = col_of(nt, 2 * tig + e) - c0;
                 const float sum = w.sum[nt][e], by = sum == 0.0f ? 0.0f : (kF32 ? 0x1p-6f : 0x1p-3f) / kValueUnit / sum;
-                const uint32_t bad = __shfl_sync(~0u, poison, (2 * tig + e) * 4);
 #pragma unroll
                 for (int u = 0; u < NG; ++u) {
-                    // what the values' centre comes to
-                    const float centre = kF32 ? 0.0f : (VB == 4 ? 8.0f : 128.0f) * kValueUnit * __shfl_sync(~0u, w.ones[nt][e], u * 4 + tig);
                     float x[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int j = 2 * u + (i >> 1), at = (i & 1) * 2 + e;
                         const float times = VB == 4 && (i & 1) ? 16.0f : 1.0f;
-                        const float y = kF32 ? w.o[0][j][at] + w.o[NT - 1][j][at] : w.o[nt][j][at] - times * centre;
+                        const float y = kF32 ? w.o[0][j][at] + w.o[NT - 1][j][at] : w.o[nt][j][at];
                         x[i] = y * (by / times) * up;
-                        if (!kF32 && ((bad >> (nt * NG + u)) & 1u)) x[i] = __int_as_float(0x7fc00000);
                     }
                     if (col >= 0 && col < kRoundCols)
                         asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(o + (col * D + u * kGroup + gid * 4) * 4), "f"(x[0]), "f"(x[1]),
@@ -998,37 +995,32 @@ struct Cut {
     }
 };
 
-// A place in a CTA's run of tiles: tiles tile .. end - 1 of the pair (b, g, ct), whose first is token `first` of the sequence's n, are its next ones.
-// What is only needed from pair to pair lies in shared memory, one for each warp (all lanes write the same).
-struct Pair {
-    int b, g, ct, tiles;
-    int left;  // tiles of the run, from the pair's first of them on
-};
+// A place in a CTA's run of tiles: tiles tile .. end - 1 of the pair (b, g, ct), whose first is token `first` of the sequence's n, are its next ones, and `left`
+// more tiles follow in other pairs.  In shared memory, one for each warp (all lanes write the same): it is needed from pair to pair only.
 template <int TOK>
-struct Walk {
-    int n, first, tile, end;
+struct Place {
+    int b, g, ct, n, first, tiles, tile, end, left;
 
-    __device__ __forceinline__ void enter(const AttendParams& p, Pair& at) {  // a sequence; `tile` and at.left are set
-        n = attended<TOK>(p, at.b, first);
-        at.tiles = max(1, (n - first + TOK - 1) / TOK);
-        end = min(at.tiles, tile + at.left);
+    __device__ __forceinline__ void sequence(const AttendParams& p) {
+        n = attended<TOK>(p, b, first);
+        tiles = max(1, (n - first + TOK - 1) / TOK);
     }
-    __device__ __forceinline__ bool next(const AttendParams& p, Pair* in) {
-        Pair at = *in;
-        at.left -= end - tile;
+    __device__ __forceinline__ void take(int from, int run) {  // the pair's tiles from `from` on, of a run of `run`
+        tile = from;
+        end = min(tiles, from + run);
+        left = run - (end - from);
+    }
+    // The same of the run's next pair; false where there is none.
+    __device__ __forceinline__ bool next(const AttendParams& p) {
+        Place at = *this;
         if (at.left <= 0) return false;
-        tile = 0;
         if (++at.ct == p.col_tiles) {
             at.ct = 0;
-            if (++at.g == p.c.G) {
-                at.g = 0, ++at.b;
-                n = attended<TOK>(p, at.b, first);
-                at.tiles = max(1, (n - first + TOK - 1) / TOK);
-            }
+            if (++at.g == p.c.G) at.g = 0, ++at.b, at.sequence(p);
         }
-        end = min(at.tiles, at.left);
+        at.take(0, at.left);
         __syncwarp();
-        *in = at;
+        *this = at;
         __syncwarp();
         return true;
     }
@@ -1042,94 +1034,96 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
     float* const ml = reinterpret_cast<float*>(smem + A::kRing);
     uint32_t* const left_at = reinterpret_cast<uint32_t*>(smem + A::kRing + A::kMl);
     __shared__ typename A::Column columns[A::kCols];
-    __shared__ Pair now[W], ahead_at[W];
+    uint4* const queries = reinterpret_cast<uint4*>(smem + A::kRing + A::kMl + 16 * ((W * 4 + 15) / 16));
+    __shared__ Place<kTok> now[W], ahead[W];
+    __shared__ uint32_t there[W][S];  // which tokens of a stage are there
     const int warp = threadIdx.x >> 5;
     const uint32_t ring = smem_u32(smem) + warp * S * A::kStage;
     grid_dependency_wait();
 
-    // This CTA's run of tiles, and which of a pair's tiles are this warp's.
-    Walk<kTok> w;
-    Pair at;
-    int step = W, skip = warp;
-    if (p.cluster > 0) {
-        const int in_all = blockIdx.x / p.cluster, each = p.c.G * p.col_tiles;
-        at.b = in_all / each;
-        const int pair = in_all - at.b * each;
-        at.g = pair / p.col_tiles, at.ct = pair - at.g * p.col_tiles;
-        at.left = 0x7fffffff;
-        w.tile = 0;
-        w.enter(p, at);
-        at.left = at.tiles;
-        w.end = at.tiles;
-        step *= p.cluster;
-        skip += W * (blockIdx.x - in_all * p.cluster);
-    } else {
-        const auto cut = Cut<kTok, kThreads>::make(p, reinterpret_cast<int64_t*>(smem));
-        const int64_t from = cut.start(blockIdx.x, gridDim.x);
-        at.left = static_cast<int>(cut.start(blockIdx.x + 1, gridDim.x) - from);
-        int64_t start;
-        at.b = cut.sequence_of(p, from, start);
-        w.tile = 0;
-        w.enter(p, at);
-        const int pair = static_cast<int>((from - start) / at.tiles);
-        w.tile = static_cast<int>((from - start) - static_cast<int64_t>(pair) * at.tiles);
-        w.end = min(at.tiles, w.tile + at.left);
-        at.g = pair / p.col_tiles, at.ct = pair - at.g * p.col_tiles;
-        __syncthreads();  // (the scan lies where the ring does)
-    }
-    if (at.left <= 0) return;
-    now[warp] = ahead_at[warp] = at;
-    __syncwarp();
-
-    // Copies run ahead of the arithmetic, across pairs too: `ahead` is the place of the next tile to be copied, `row` where this lane's token of it lies
-    // (contiguous: only the pair's first row is kept).
-    Walk<kTok> ahead = w;
-    int tile = ahead.tile + skip, seen = first_seen(p, ahead.n);
-    const bool paged = p.c.block_table != nullptr;
-    int64_t row = paged ? 0 : row_of(p.c, at.b, at.g, 0, nullptr);
-    bool more = true;
-    const auto look = [&] {
-        while (tile >= ahead.end) {
-            if (!ahead.next(p, ahead_at + warp)) {
-                more = false;
-                return;
-            }
-            tile = ahead.tile + skip;
-            seen = first_seen(p, ahead.n);
-            if (!paged) row = row_of(p.c, ahead_at[warp].b, ahead_at[warp].g, 0, nullptr);
+    // This CTA's run of tiles, and which of a pair's tokens are this warp's: kTok from `skip` on, `step` further on the next ones.
+    int step = W * kTok, skip = warp * kTok;
+    {
+        Place<kTok> at;
+        if (p.cluster > 0) {
+            const int in_all = blockIdx.x / p.cluster, each = p.c.G * p.col_tiles;
+            at.b = in_all / each;
+            const int pair = in_all - at.b * each;
+            at.g = pair / p.col_tiles, at.ct = pair - at.g * p.col_tiles;
+            at.sequence(p);
+            at.take(0, at.tiles);
+            skip += step * (blockIdx.x - in_all * p.cluster);
+            step *= p.cluster;
+        } else {
+            const auto cut = Cut<kTok, kThreads>::make(p, reinterpret_cast<int64_t*>(smem));
+            const int64_t from = cut.start(blockIdx.x, gridDim.x);
+            const int run = static_cast<int>(cut.start(blockIdx.x + 1, gridDim.x) - from);
+            int64_t start;
+            at.b = cut.sequence_of(p, from, start);
+            at.sequence(p);
+            const int pair = static_cast<int>((from - start) / at.tiles);
+            at.take(static_cast<int>((from - start) - static_cast<int64_t>(pair) * at.tiles), run);
+            at.g = pair / p.col_tiles, at.ct = pair - at.g * p.col_tiles;
+            __syncthreads();  // (the scan lies where the ring does)
+            if (run <= 0) return;
         }
-        if (paged) row = A::find(p, ahead_at[warp].b, ahead_at[warp].g, ahead.first + tile * kTok, seen, ahead.n);
+        now[warp] = ahead[warp] = at;
+        __syncwarp();
+    }
+
+    // Copies run ahead of the arithmetic, across pairs too: the next one is of tokens copy_t .. of the pair at ahead[warp], whose copies end at copy_end, and
+    // of whose tokens those from `seen` to held - 1 are seen; `row`: where this lane's token of it lies (contiguous: the pair's first row).
+    const bool paged = p.c.block_table != nullptr;
+    int copy_t, copy_end, seen, held;
+    int64_t row = 0;
+    const auto enter = [&] {
+        const Place<kTok>& at = ahead[warp];
+        copy_t = at.first + at.tile * kTok + skip;
+        copy_end = at.first + at.end * kTok;
+        held = at.n;
+        seen = first_seen(p, held);
+        if (!paged) row = row_of(p.c, at.b, at.g, 0, nullptr);
+    };
+    const auto look = [&] {
+        while (copy_t >= copy_end) {
+            if (!ahead[warp].next(p)) return;
+            enter();
+        }
+        if (paged) row = A::find(p, ahead[warp].b, ahead[warp].g, copy_t, seen, held);
     };
     typename A::Lane l;
     l.set();
-    uint32_t there[S];  // [0]: of the stage that is next in the arithmetic
     const auto copy = [&](int slot) {
-        uint32_t is = 0;
-        if (more) {
+        if (copy_t < copy_end) {
             const uint32_t to = ring + slot * A::kStage;
-            is = paged ? A::copy_paged(p, l, to, row) : A::copy_run(p, l, to, row, ahead.first + tile * kTok, seen, ahead.n);
-            tile += step;
+            const uint32_t is = paged ? A::copy_paged(p, l, to, row) : A::copy_run(p, l, to, row, copy_t, seen, held);
+            there[warp][slot] = is;
+            copy_t += step;
             look();
         }
         copy_commit();
-        return is;
     };
+    enter();
     look();
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) there[i] = copy(i);
+    for (int i = 0; i < S - 1; ++i) copy(i);
 
     typename A::Warp q;
     int slot = 0;
     bool first_of_run = true;
     for (;;) {
-        A::begin(p, q, columns, now[warp].b, now[warp].g, now[warp].ct, w.n);
-        for (int t = w.tile + skip; t < w.end; t += step) {
+        int t, end;
+        {
+            const Place<kTok>& at = now[warp];
+            A::begin(p, q, queries, columns, at.b, at.g, at.ct, at.n);
+            t = at.first + at.tile * kTok + skip;
+            end = at.first + at.end * kTok;
+        }
+        for (; t < end; t += step) {
             copy_wait<S - 2>();
             __syncwarp();
-            there[S - 1] = copy(slot == 0 ? S - 1 : slot - 1);
-            A::fold(p, l, q, columns, ring + slot * A::kStage, w.first + t * kTok, there[0]);
-#pragma unroll
-            for (int i = 0; i < S - 1; ++i) there[i] = there[i + 1];
+            copy(slot == 0 ? S - 1 : slot - 1);
+            A::fold(p, l, q, queries, columns, ring + slot * A::kStage, t, there[warp][slot]);
             slot = slot == S - 1 ? 0 : slot + 1;
         }
         // The warps' results, in the stage of each ring that the next copy goes to.
@@ -1138,7 +1132,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
         A::leave_sums(q, ml + warp * A::kCols * 2);
         if ((threadIdx.x & 31) == 0) left_at[warp] = mine;
         const int b = now[warp].b, g = now[warp].g, ct = now[warp].ct;
-        const bool whole = p.cluster == 1 || (p.cluster == 0 && w.tile == 0 && w.end == now[warp].tiles);
+        const bool whole = p.cluster == 1 || (p.cluster == 0 && now[warp].tile == 0 && now[warp].end == now[warp].tiles);
         const int used = min(p.m * p.R - ct * A::kCols, A::kCols);
         constexpr int kQuads = A::kRoundCols * D / 4, kPer = (kQuads + kThreads - 1) / kThreads;
         float kept[A::kRounds * kPer][4];
@@ -1216,7 +1210,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
             cluster_sync();  // nobody leaves while its results are read
         }
         first_of_run = false;
-        if (p.cluster > 0 || !w.next(p, now + warp)) break;
+        if (p.cluster > 0 || !now[warp].next(p)) break;
     }
     copy_wait<0>();
 }

@@ -69,9 +69,7 @@ def tolerance(out, mean, size, n, dtype: str, extra: float = 0.0, largest: float
     - a score is sums over groups of products with codes.  The tensor core adds 16 products and what it had, each cut off 24 bits below the
       largest, twice per group: 34 * 2^-24 of it.  bfloat16: codes as stored, up to 15 where the value's is 7, with 4 bits less: 34 * 2^-20 * 15 / 7.
       The largest product is at most `size`.  It scales probabilities above and below the line;
-    - sums over n tokens, 16 at a time: 2^-23 of the sum each, and as much for their reunion.  bfloat16: of codes as stored and of their centre, together
-      up to (15 + 8) / 7 of the largest value (17 addends of 2^-20 each are within that where probabilities are even, and below the roundings above
-      where they are not).
+    - sums over n tokens, 16 at a time: 2^-23 of the mean magnitude each, and as much for their reunion;
     `extra` is an absolute error of scores beyond that (bias, cap).
     - fp16 numbers below 2^-14 lie 2^-24 apart.  A probability (relative to a score that was seen, so their sum is at least 1) times a
       value scale s is held as a multiple p s / 2^(E - 6), 2^E <= the largest scale: off by up to half of 2^-24 * 2^(E - 6) = 2^-31 2^E beyond the
@@ -80,5 +78,5 @@ def tolerance(out, mean, size, n, dtype: str, extra: float = 0.0, largest: float
     bf16 = dtype == "bf16"
     half, held_in = (2.0 ** -8, 2.0 ** -10) if bf16 else (2.0 ** -24, 2.0 ** -21)
     score = 34 * (2.0 ** -20 * 15 / 7 if bf16 else 2.0 ** -24) * size + extra
-    summed = 2.0 ** -23 * (n / 16 + 32) * (largest * 23 / 7 if bf16 else mean)
+    summed = 2.0 ** -23 * (n / 16 + 32) * mean
     return half * np.abs(out) + (held_in + 2 * score) * mean + summed + n * 2.0 ** -31 * largest
