@@ -154,6 +154,10 @@ struct Words {
             }
         }
     }
+    __device__ __forceinline__ void store(uint32_t at) const {
+#pragma unroll
+        for (int i = 0; i < BYTES / 4; ++i) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + 4 * i), "r"(w[i]) : "memory");
+    }
     __device__ __forceinline__ void load16(uint32_t at, int i) {
         asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "r"(at) : "memory");
     }
@@ -670,15 +674,34 @@ struct Attend {
 #pragma unroll
         for (int i = 1; i < kSG / 2; ++i) most = __vmaxu2(most, mine.w[i]);
         most = __reduce_max_sync(~0u, max(most >> 16, most & 0xffffu));
-        const bool nan = most >= 0x7f80u;
-        if (nan) {
-            most = 0;
+        if (most >= 0x7f80u) {
+            // Groups of NaN spoil their elements of the columns that see their token, and take no part in the products, which know neither.
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const uint32_t y = i & 1 ? mine.w[i >> 1] >> 16 : mine.w[i >> 1] & 0xffffu;
-                most = max(most, y >= 0x7f80u ? 0u : y);
+            for (int u = 0; u < NG; ++u) {
+                const uint32_t y = u & 1 ? mine.w[u >> 1] >> 16 : mine.w[u >> 1] & 0xffffu;
+                const uint32_t bad = __ballot_sync(~0u, y >= 0x7f80u);  // a bit per token
+                if (y >= 0x7f80u) mine.w[u >> 1] &= u & 1 ? 0x0000ffffu : 0xffff0000u;
+#pragma unroll
+                for (int nt = 0; nt < NS; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        bool spoilt = false;
+#pragma unroll
+                        for (int h = 0; h < MT; ++h)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                spoilt = spoilt || (((bad >> (h * 16 + i * 8 + gid)) & 1u) && !((hidden >> ((h * NS + nt) * 4 + i * 2 + e)) & 1u));
+                        const uint32_t lanes = __ballot_sync(~0u, spoilt);
+                        if ((lanes >> tig) & 0x11111111u) {
+#pragma unroll
+                            for (int j = 2 * u; j < 2 * u + 2; ++j) w.o[nt][j][e] = w.o[nt][j][e + 2] = __int_as_float(0x7fc00000);
+                        }
+                    }
             }
-            most = __reduce_max_sync(~0u, most);
+            most = mine.w[0];
+#pragma unroll
+            for (int i = 1; i < kSG / 2; ++i) most = __vmaxu2(most, mine.w[i]);
+            most = __reduce_max_sync(~0u, max(most >> 16, most & 0xffffu));
         }
         const int now = static_cast<int>(most >> 7);
         if (now > w.scale_exp) {
@@ -692,16 +715,19 @@ struct Attend {
                     for (int e = 0; e < 4; ++e) w.o[nt][j][e] *= by;
         }
         if constexpr (kF32)
-            values_f32(l, w, stage, s, masked, hidden);
+            values_f32(l, w, stage, s, mine);
         else
-            values_bf16(l, w, stage, s, mine, nan, masked, hidden);
+            values_bf16(l, w, stage, s, mine);
     }
 
     // O += V^T P for fp32: weights times value scales in 32 bits, then as two fp16 numbers.
     template <int NS>
-    __device__ static __forceinline__ void values_f32(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NS][4], bool masked, uint32_t hidden) {
+    __device__ static __forceinline__ void values_f32(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NS][4], const Words<kSRow>& mine) {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         const float vf = __int_as_float((260 - w.scale_exp) << 23);  // 2^(6 - exponent)
+        __syncwarp();
+        mine.store(stage + kKBytes + kVBytes + kSBytes + (lane & (kTok - 1)) * kSRow);  // (without the groups of NaN)
+        __syncwarp();
         const uint32_t vs = stage + kKBytes + kVBytes + kSBytes;
         const uint32_t values_at[2] = {stage + kKBytes + l.v, stage + kKBytes + l.v_next()};
 #pragma unroll
@@ -718,10 +744,6 @@ struct Attend {
                 const float f0 = vf * __uint_as_float(u & 1 ? s0.w[u >> 1] & 0xffff0000u : s0.w[u >> 1] << 16);
                 const float f1 = vf * __uint_as_float(u & 1 ? s1.w[u >> 1] & 0xffff0000u : s1.w[u >> 1] << 16);
                 float x[4] = {weight[h][0][0] * f0, weight[h][0][1] * f0, weight[h][0][2] * f1, weight[h][0][3] * f1};
-                if (masked) {  // (0 times a NaN scale)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = (hidden >> (h * 4 + e)) & 1u ? 0.0f : x[e];
-                }
                 const uint32_t p0 = pack_half(x[0], x[1]), p1 = pack_half(x[2], x[3]);
                 const float2 g0 = unpack_half(p0), g1 = unpack_half(p1);
                 const uint32_t b[2][2] = {{transpose8x8(p0), transpose8x8(p1)},
@@ -744,8 +766,7 @@ struct Attend {
     // O += V^T P for bfloat16: weights go to the operand's layout as fp16 numbers and meet the value scales there, two per instruction.  The scales
     // are made fp16 (relative to the largest exponent) and brought into that order by the lane that has the token, in place.
     template <int NS>
-    __device__ static __forceinline__ void values_bf16(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NS][4], const Words<kSRow>& mine, bool nan,
-                                                       bool hidden_any, uint32_t hidden) {
+    __device__ static __forceinline__ void values_bf16(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NS][4], const Words<kSRow>& mine) {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         constexpr int kWords = kSG / 2;
         const uint32_t vs = stage + kKBytes + kVBytes + kSBytes;
@@ -800,15 +821,6 @@ struct Attend {
                 for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) b[nt][i] = half_mul(weights[nt][i], sv.w[i * kSG + u]);
-                if (nan && hidden_any) {  // (0 times a NaN scale)
-#pragma unroll
-                    for (int nt = 0; nt < NS; ++nt)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint32_t bits = hidden >> ((h * NS + nt) * 4 + 2 * i);
-                            b[nt][i] &= transpose8x8((bits & 1u ? 0u : 0xffffu) | (bits & 2u ? 0u : 0xffff0000u));
-                        }
-                }
                 uint32_t a[2][4];
                 v_pieces(v, u, a);
 #pragma unroll
