@@ -1,16 +1,20 @@
 // Quantised key / value cache: rows into it and out of it.
 //
-// Both are streams: a row of D elements comes in at D * (2 or 4) bytes and leaves at D * bits / 8 + D / 16, or the other way round.
-// One thread has 8 neighbouring elements (16 bytes of bfloat16), four threads next to one another a group: its largest
-// magnitude is two shuffles away.
+// Both are streams: a row of D elements comes in at D * (2 or 4) bytes and leaves at D * bits / 8 + D / 16, or the other way round.  A thread has
+// octet o (8 neighbouring elements) of every group of a row, as the cache keeps them one behind the other: its codes are one piece of memory
+// (16 bytes for 4 bits and heads of 128), what it reads or writes of the row in full width are D / 32 pieces of 16 bytes, 64 bytes apart, which the
+// four threads of the row fill between them; and a group's largest magnitude is two shuffles away.  That keeps 64 bytes per thread on their way and
+// finds a row's place once for all of it (one octet per thread with its own divisions: 2.2 TB/s into the cache, 2.8 out of it).
 //
-// A code is the quotient rounded to the nearest whole number, ties to even, as if it had been computed exactly.  The fp32 division
-// gives that: x / scale lies exactly on a border n + 1/2 only if it is one.  (A border times the scale has at most 8 + 8
+// A code is the quotient rounded to the nearest whole number, ties to even, as if it had been computed exactly.  The correctly rounded fp32
+// quotient gives that: x / scale lies exactly on a border n + 1/2 only if it is one.  (A border times the scale has at most 8 + 8
 // bits, so it is a float; the next float away from it, a step u, moves the quotient by u / scale, which is more than half a step of
-// the quotient, because the scale's mantissa is below 2.  So no other quotient rounds onto the border.)  The same holds for max / L.
+// the quotient, because the scale's mantissa is below 2.  So no other quotient rounds onto the border.)  The same holds for max / L.  Scales
+// of ordinary size take the quotient from their reciprocal and one correction by the remainder, which an FMA gives exactly: a border comes out as
+// itself, and anything else is right to a small part of a step.
 #include "qcache.cuh"
 
-#include <algorithm>
+#include <type_traits>
 
 namespace b2kv {
 namespace qcache {
@@ -34,186 +38,276 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+// Quotients by a divisor that the host knows, of numbers below 2^31: m / 2^(31 + l) is above 1 / d by less than 2^-31 / d.
+struct Divisor {
+    uint32_t d, m;
+    int shift;
+    explicit Divisor(uint32_t by) : d(by) {
+        int l = 0;
+        while ((1ull << l) < by) ++l;
+        shift = 31 + l;
+        m = static_cast<uint32_t>(((1ull << shift) + by - 1) / by);
+    }
+    __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> shift); }
+};
+
+// Eight elements as they lie in memory.
+template <typename T>
+struct Octet {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+    __device__ __forceinline__ void widen(float (&f)[8]) const;
+};
+template <>
+__device__ __forceinline__ void Octet<float>::widen(float (&f)[8]) const {
+    Elt<float>::widen(w[0], f);
+    Elt<float>::widen(w[1], f + 4);
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) {
-    Elt<__nv_bfloat16>::widen(*reinterpret_cast<const uint4*>(p), f);
+template <>
+__device__ __forceinline__ void Octet<__nv_bfloat16>::widen(float (&f)[8]) const {
+    Elt<__nv_bfloat16>::widen(w[0], f);
 }
-__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+__device__ __forceinline__ void store4(float* p, const float* f) { *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]); }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float* f) {
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(f[0], f[1]), __floats2bfloat162_rn(f[2], f[3])};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(h);
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
+__device__ __forceinline__ void store8(float* p, const float* f) { store4(p, f), store4(p + 4, f + 4); }
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float* f) {
     __nv_bfloat162 h[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
 }
 
-// Eight stored codes of a group from its elements; every lane of the four that hold the group gets the scale.
+// Eight codes as numbers code + 8 or code + 128, lowest first, of a group's elements; all four lanes of the group get its scale.
 template <int BITS>
-__device__ __forceinline__ uint2 quantise(const float (&f)[8], __nv_bfloat16& scale) {
+__device__ __forceinline__ uint2 quantise(const float (&f)[8], uint32_t& scale) {
     constexpr int kTop = BITS == 4 ? 7 : 127;
-    float most = 0.0f;
-    bool finite = true;
+    constexpr uint32_t kTimes = BITS == 4 ? 16 : 256;
+    uint32_t most = 0;  // magnitudes as whole numbers: in the same order, NaN above infinity above all others
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        most = fmaxf(most, fabsf(f[e]));
-        finite = finite && fabsf(f[e]) <= 3.402823466e38f;
-    }
-    most = finite ? most : __int_as_float(0x7f800000);
-    most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
-    most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
-    finite = most <= 3.402823466e38f;
-    scale = __float2bfloat16_rn(finite ? most / static_cast<float>(kTop) : __int_as_float(0x7fc00000));
-    const float s = __bfloat162float(scale);
-    uint2 w = make_uint2(0, 0);
+    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(f[e]) & 0x7fffffffu);
+    most = max(most, __shfl_xor_sync(~0u, most, 1));
+    most = max(most, __shfl_xor_sync(~0u, most, 2));
+    const __nv_bfloat16 rounded = __float2bfloat16_rn(most < 0x7f800000u ? __uint_as_float(most) / kTop : __int_as_float(0x7fc00000));
+    scale = __bfloat16_as_ushort(rounded);
+    const float s = __bfloat162float(rounded);
+    uint32_t n[8];
+    if (s >= 0x1p-100f) {
+        const float inverse = 1.0f / s;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float q = s > 0.0f ? fminf(fmaxf(rintf(f[e] / s), -kTop), kTop) : 0.0f;
-        const uint32_t c = static_cast<uint32_t>(static_cast<int>(q) + kTop + 1);
-        if (BITS == 4)
-            w.x |= c << (4 * e);
-        else
-            (e < 4 ? w.x : w.y) |= c << (8 * (e & 3));
+        for (int e = 0; e < 8; ++e) {
+            const float q = f[e] * inverse;
+            const float right = fmaf(fmaf(-q, s, f[e]), inverse, q);
+            n[e] = __float_as_uint(right + (12582912.0f + (kTop + 1)));  // 1.5 * 2^23: the sum's last bits are the rounded number's
+        }
+    } else {  // (no scale, or a NaN, or one so small that remainders would be cut off)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float q = s > 0.0f ? fminf(fmaxf(f[e] / s, -kTop), kTop) : 0.0f;
+            n[e] = __float_as_uint(q + (12582912.0f + (kTop + 1)));
+        }
     }
-    return w;
+    constexpr int kPer = 32 / BITS;
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 8 / kPer; ++i) {
+        // all but the last code leave nothing above them but the same bits each time, which come off at the end
+        uint32_t x = n[i * kPer + kPer - 1], off = 0x4b400000u;
+#pragma unroll
+        for (int e = kPer - 2; e >= 0; --e) x = x * kTimes + n[i * kPer + e], off = off * kTimes + 0x4b400000u;
+        w[i] = x - off;
+    }
+    return make_uint2(w[0], w[8 / kPer - 1]);
 }
 
-// Octet o of group u of a row of `groups` groups; values are units of half an octet.
-template <int BITS, bool kValues>
-__device__ __forceinline__ void store_codes(uint8_t* row, int groups, int u, int o, uint2 w) {
-    if (!kValues && BITS == 4) {
-        reinterpret_cast<uint32_t*>(row)[o * groups + u] = __funnelshift_l(w.x, w.x, 2);
-    } else if (!kValues) {
-        reinterpret_cast<uint2*>(row)[o * groups + u] = w;
-    } else if (BITS == 4) {
-        w.x = ((w.x << 2) & 0xfffcfffcu) | ((w.x >> 14) & 0x00030003u);
-        reinterpret_cast<uint16_t*>(row)[2 * o * groups + u] = static_cast<uint16_t>(w.x);
-        reinterpret_cast<uint16_t*>(row)[(2 * o + 1) * groups + u] = static_cast<uint16_t>(w.x >> 16);
-    } else {
-        reinterpret_cast<uint32_t*>(row)[2 * o * groups + u] = w.x;
-        reinterpret_cast<uint32_t*>(row)[(2 * o + 1) * groups + u] = w.y;
+// What a row's thread keeps of it: octet o of all NG groups.
+template <int NG, int BITS>
+struct Codes {
+    static constexpr int kBytes = NG * BITS;
+    uint32_t w[(kBytes + 3) / 4];
+    __device__ __forceinline__ void load(const uint8_t* p) { each([&](auto* to, auto* from) { *to = *from; }, reinterpret_cast<uint8_t*>(w), p); }
+    __device__ __forceinline__ void store(uint8_t* p) const { each([&](auto* to, auto* from) { *to = *from; }, p, reinterpret_cast<const uint8_t*>(w)); }
+    // in pieces of the largest power of two that divides the whole, which is what the place is a multiple of
+    template <typename F>
+    __device__ static __forceinline__ void each(F&& copy, uint8_t* to, const uint8_t* from) {
+        using Piece = typename std::conditional<kBytes % 16 == 0, uint4, typename std::conditional<kBytes % 8 == 0, uint2, uint32_t>::type>::type;
+#pragma unroll
+        for (int i = 0; i < kBytes / static_cast<int>(sizeof(Piece)); ++i) copy(reinterpret_cast<Piece*>(to) + i, reinterpret_cast<const Piece*>(from) + i);
     }
-}
-template <int BITS, bool kValues>
-__device__ __forceinline__ uint2 load_codes(const uint8_t* row, int groups, int u, int o) {
-    if (!kValues && BITS == 4) {
-        const uint32_t w = reinterpret_cast<const uint32_t*>(row)[o * groups + u];
-        return make_uint2(__funnelshift_r(w, w, 2), 0);
+
+    // Octets to and from units of 8 codes (keys) or of 4, those of the octet's first half for all groups before those of its second (values).
+    template <bool kValues>
+    __device__ __forceinline__ void put(int u, uint2 c) {
+        if constexpr (BITS == 8) {
+            w[kValues ? u : 2 * u] = c.x, w[kValues ? NG + u : 2 * u + 1] = c.y;
+        } else if constexpr (!kValues) {
+            w[u] = __funnelshift_l(c.x, c.x, 2);
+        } else {
+            const uint32_t x = ((c.x << 2) & 0xfffcfffcu) | ((c.x >> 14) & 0x00030003u);
+            put16(u, x & 0xffffu);
+            put16(NG + u, x >> 16);
+        }
     }
-    if (!kValues) return reinterpret_cast<const uint2*>(row)[o * groups + u];
-    if (BITS == 4) {
-        const uint32_t w = reinterpret_cast<const uint16_t*>(row)[2 * o * groups + u] |
-                           static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[(2 * o + 1) * groups + u]) << 16;
-        return make_uint2(((w >> 2) & 0x3fff3fffu) | ((w << 14) & 0xc000c000u), 0);
+    template <bool kValues>
+    __device__ __forceinline__ uint2 get(int u) const {
+        if constexpr (BITS == 8) {
+            return make_uint2(w[kValues ? u : 2 * u], w[kValues ? NG + u : 2 * u + 1]);
+        } else if constexpr (!kValues) {
+            return make_uint2(__funnelshift_r(w[u], w[u], 2), 0);
+        } else {
+            const uint32_t x = get16(u) | get16(NG + u) << 16;
+            return make_uint2(((x >> 2) & 0x3fff3fffu) | ((x << 14) & 0xc000c000u), 0);
+        }
     }
-    return make_uint2(reinterpret_cast<const uint32_t*>(row)[2 * o * groups + u], reinterpret_cast<const uint32_t*>(row)[(2 * o + 1) * groups + u]);
+    __device__ __forceinline__ void put16(int i, uint32_t x) { w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | x << 16 : (w[i / 2] & 0xffff0000u) | x; }
+    __device__ __forceinline__ uint32_t get16(int i) const { return i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu; }
+};
+
+template <typename T, int NG, int BITS, bool kValues>
+__device__ __forceinline__ void write_row(const b2kv_qcache& c, const T* src, int o, int64_t row) {
+    Octet<T> in[NG];
+#pragma unroll
+    for (int u = 0; u < NG; ++u) in[u].load(src + u * kGroup + o * 8);
+    Codes<NG, BITS> codes = {};
+    uint32_t scales[scale_row(NG) / 2] = {};
+#pragma unroll
+    for (int u = 0; u < NG; ++u) {
+        float f[8];
+        in[u].widen(f);
+        uint32_t scale;
+        codes.template put<kValues>(u, quantise<BITS>(f, scale));
+        scales[u / 2] |= u & 1 ? scale << 16 : scale;
+    }
+    if (row < 0) return;
+    codes.store(static_cast<uint8_t*>(kValues ? c.v_codes : c.k_codes) + row * (NG * 4 * BITS) + o * (NG * BITS));
+    if (o == 0) {  // the row of scales; what lies behind the last takes part in products, with zeros
+        uint32_t* const to = static_cast<uint32_t*>(kValues ? c.v_scales : c.k_scales) + row * (scale_row(NG) / 2);
+        if constexpr (scale_row(NG) == 2) *to = scales[0];
+        if constexpr (scale_row(NG) == 4) *reinterpret_cast<uint2*>(to) = make_uint2(scales[0], scales[1]);
+        if constexpr (scale_row(NG) == 8) *reinterpret_cast<uint4*>(to) = make_uint4(scales[0], scales[1], scales[2], scales[3]);
+    }
 }
 
-// Thread = octet; grid.y 0 keys, 1 values.  `octets` is B * n * G * D / 8, a multiple of four: the lanes of a group are all inside or all outside.
-template <typename T, int KB, int VB>
-__global__ void __launch_bounds__(kThreads) write_kernel(b2kv_qcache c, const T* k, int64_t ld_k, const T* v, int64_t ld_v, int n, int64_t octets,
-                                                         int32_t* dev_status) {
+// Thread = (row of a head, octet); grid.y 0 keys, 1 values.
+template <typename T, int NG, int KB, int VB>
+__global__ void __launch_bounds__(kThreads) write_kernel(const b2kv_qcache c, const T* k, int64_t ld_k, const T* v, int64_t ld_v, int n, Divisor by_heads,
+                                                         Divisor by_rows, uint32_t rows, int32_t* dev_status) {
     grid_launch_dependents();
     grid_dependency_wait();
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    const bool inside = at < octets;
-    const int groups = c.D / kGroup, per_row = c.D / 8;
-    const int64_t i = inside ? at : 0;  // (lanes behind the end go along with the shuffles)
-    const int64_t head_row = i / per_row;
-    const int j = static_cast<int>(i - head_row * per_row), u = j >> 2, o = j & 3;
-    const int64_t src = head_row / c.G;
-    const int g = static_cast<int>(head_row - src * c.G), b = static_cast<int>(src / n);
-    const int64_t place = static_cast<int64_t>(tokens_held(c, b)) + (src - static_cast<int64_t>(b) * n);
+    const uint32_t at = blockIdx.x * (kThreads / 4) + threadIdx.x / 4, o = threadIdx.x & 3;
+    const uint32_t i = min(at, rows - 1);  // (lanes behind the end go along with the shuffles)
+    const uint32_t src = by_heads.quotient(i), g = i - src * by_heads.d, b = by_rows.quotient(src);
+    const int64_t place = static_cast<int64_t>(tokens_held(c, b)) + (src - b * by_rows.d);
     int64_t row = -1;
     if (place < 0 || place >= c.T_max)
         report_status(dev_status, B2KV_DEV_BAD_POSITION);
     else
         row = row_of(c, b, g, static_cast<int>(place), dev_status);
-    float f[8];
-    __nv_bfloat16 scale;
-    const bool values = blockIdx.y != 0;
-    load8((values ? v + src * ld_v : k + src * ld_k) + static_cast<int64_t>(g) * c.D + j * 8, f);
-    const uint2 w = (values ? VB : KB) == 4 ? quantise<4>(f, scale) : quantise<8>(f, scale);
-    if (!inside || row < 0) return;
-    if (values)
-        store_codes<VB, true>(static_cast<uint8_t*>(c.v_codes) + row * (c.D * VB / 8), groups, u, o, w);
+    if (at >= rows) row = -1;
+    if (blockIdx.y == 0)
+        write_row<T, NG, KB, false>(c, k + src * ld_k + static_cast<int64_t>(g) * (NG * kGroup), o, row);
     else
-        store_codes<KB, false>(static_cast<uint8_t*>(c.k_codes) + row * (c.D * KB / 8), groups, u, o, w);
-    if (o == 0) {
-        __nv_bfloat16* const to = static_cast<__nv_bfloat16*>(values ? c.v_scales : c.k_scales) + row * scale_row(groups);
-        to[u] = scale;
-        if (u == groups - 1)  // the rest takes part in products, with zeros
-            for (int r = groups; r < scale_row(groups); ++r) to[r] = __float2bfloat16_rn(0.0f);
-    }
+        write_row<T, NG, VB, true>(c, v + src * ld_v + static_cast<int64_t>(g) * (NG * kGroup), o, row);
 }
 
-// Thread = octet of the output.
-template <typename T, int BITS, bool kValues>
-__global__ void __launch_bounds__(kThreads) read_kernel(b2kv_qcache c, T* out, int n, int last, int len_bias, int64_t octets, int32_t* dev_status) {
+// Thread = (row of a head of the output, octet).
+template <typename T, int NG, int BITS, bool kValues>
+__global__ void __launch_bounds__(kThreads) read_kernel(const b2kv_qcache c, T* out, int n, int last, int len_bias, Divisor by_heads, Divisor by_rows,
+                                                        uint32_t rows, int32_t* dev_status) {
     grid_launch_dependents();
     grid_dependency_wait();
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    if (i >= octets) return;
-    const int groups = c.D / kGroup, per_row = c.D / 8;
-    const int64_t head_row = i / per_row;
-    const int j = static_cast<int>(i - head_row * per_row), u = j >> 2, o = j & 3;
-    const int64_t dst = head_row / c.G;
-    const int g = static_cast<int>(head_row - dst * c.G), b = static_cast<int>(dst / n);
+    const uint32_t i = blockIdx.x * (kThreads / 4) + threadIdx.x / 4, o = threadIdx.x & 3;
+    if (i >= rows) return;
+    const uint32_t dst = by_heads.quotient(i), g = i - dst * by_heads.d, b = by_rows.quotient(dst);
     const int64_t held = min(static_cast<int64_t>(tokens_held(c, b)) + len_bias, static_cast<int64_t>(c.T_max));
-    const int64_t place = dst - static_cast<int64_t>(b) * n + (last ? held - n : 0);
-    float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const int64_t place = static_cast<int64_t>(dst - b * by_rows.d) + (last ? held - n : 0);
     const int64_t row = place >= 0 && place < held ? row_of(c, b, g, static_cast<int>(place), dev_status) : -1;
+    Codes<NG, BITS> codes;
+    uint32_t scales[scale_row(NG) / 2] = {};
     if (row >= 0) {
-        const float s = __bfloat162float(static_cast<const __nv_bfloat16*>(kValues ? c.v_scales : c.k_scales)[row * scale_row(groups) + u]);
-        const uint2 w = load_codes<BITS, kValues>(static_cast<const uint8_t*>(kValues ? c.v_codes : c.k_codes) + row * (c.D * BITS / 8), groups, u, o);
+        codes.load(static_cast<const uint8_t*>(kValues ? c.v_codes : c.k_codes) + row * (NG * 4 * BITS) + o * (NG * BITS));
+        const uint32_t* const from = static_cast<const uint32_t*>(kValues ? c.v_scales : c.k_scales) + row * (scale_row(NG) / 2);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t code = BITS == 4 ? (w.x >> (4 * e)) & 15u : ((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 255u;
-            f[e] = static_cast<float>(static_cast<int>(code) - (1 << (BITS - 1))) * s;  // exact: 8 bits by 8
-        }
+        for (int u = 0; u < (NG + 1) / 2; ++u) scales[u] = from[u];
     }
-    store8(out + i * 8, f);
+    T* const to = out + static_cast<int64_t>(i) * (NG * kGroup) + o * 8;
+#pragma unroll
+    for (int u = 0; u < NG; ++u) {
+        float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (row >= 0) {
+            const float s = __uint_as_float(u & 1 ? scales[u / 2] & 0xffff0000u : scales[u / 2] << 16);
+            const uint2 x = codes.template get<kValues>(u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t code = BITS == 4 ? (x.x >> (4 * e)) & 15u : ((e < 4 ? x.x : x.y) >> (8 * (e & 3))) & 255u;
+                f[e] = (__uint_as_float(0x4b000000u | code) - (8388608.0f + (1 << (BITS - 1)))) * s;  // exact: 2^23 + code less that, 8 bits by 8
+            }
+        }
+        store8(to + u * kGroup, f);
+    }
 }
 
-template <typename T, int KB, int VB>
+template <typename T, int NG, int KB, int VB>
 int launch_write(const b2kv_qcache& c, const void* k, int64_t ld_k, const void* v, int64_t ld_v, int n, int32_t* dev_status, void* stream) {
-    const int64_t octets = static_cast<int64_t>(c.B) * n * c.G * (c.D / 8);
-    const int64_t blocks = (octets + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffff) return B2KV_ERR_UNSUPPORTED;
-    OverlapLaunch launch(dim3(static_cast<unsigned>(blocks), 2), kThreads, 0, stream);
-    B2KV_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, write_kernel<T, KB, VB>, c, static_cast<const T*>(k), ld_k, static_cast<const T*>(v), ld_v, n, octets,
-                                     dev_status));
+    const int64_t rows = static_cast<int64_t>(c.B) * n * c.G;
+    if (rows > 0x7fffffff) return B2KV_ERR_UNSUPPORTED;
+    OverlapLaunch launch(dim3(static_cast<unsigned>((rows + kThreads / 4 - 1) / (kThreads / 4)), 2), kThreads, 0, stream);
+    B2KV_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, write_kernel<T, NG, KB, VB>, c, static_cast<const T*>(k), ld_k, static_cast<const T*>(v), ld_v, n,
+                                     Divisor(c.G), Divisor(n), static_cast<uint32_t>(rows), dev_status));
     return B2KV_OK;
 }
 
-template <typename T, int BITS, bool kValues>
+template <typename T, int NG, int BITS, bool kValues>
 int launch_read(const b2kv_qcache& c, void* out, int n, int last, int len_bias, int32_t* dev_status, void* stream) {
-    const int64_t octets = static_cast<int64_t>(c.B) * n * c.G * (c.D / 8);
-    const int64_t blocks = (octets + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffff) return B2KV_ERR_UNSUPPORTED;
-    OverlapLaunch launch(static_cast<unsigned>(blocks), kThreads, 0, stream);
-    B2KV_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, read_kernel<T, BITS, kValues>, c, static_cast<T*>(out), n, last, len_bias, octets, dev_status));
+    const int64_t rows = static_cast<int64_t>(c.B) * n * c.G;
+    if (rows > 0x7fffffff) return B2KV_ERR_UNSUPPORTED;
+    OverlapLaunch launch(static_cast<unsigned>((rows + kThreads / 4 - 1) / (kThreads / 4)), kThreads, 0, stream);
+    B2KV_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, read_kernel<T, NG, BITS, kValues>, c, static_cast<T*>(out), n, last, len_bias, Divisor(c.G), Divisor(n),
+                                     static_cast<uint32_t>(rows), dev_status));
     return B2KV_OK;
+}
+
+// fn(NG as a type) for the cache's head size.
+template <int N>
+struct Groups {
+    static constexpr int value = N;
+};
+template <typename F>
+int by_size(int D, F&& fn) {
+    switch (D) {
+        case 32: return fn(Groups<1>());
+        case 64: return fn(Groups<2>());
+        case 96: return fn(Groups<3>());
+        case 128: return fn(Groups<4>());
+        default: return fn(Groups<8>());
+    }
 }
 
 template <typename T>
 int write_typed(const b2kv_qcache& c, const void* k, int64_t ld_k, const void* v, int64_t ld_v, int n, int32_t* dev_status, void* stream) {
-    if (c.k_bits == 4) return launch_write<T, 4, 4>(c, k, ld_k, v, ld_v, n, dev_status, stream);
-    if (c.v_bits == 4) return launch_write<T, 8, 4>(c, k, ld_k, v, ld_v, n, dev_status, stream);
-    return launch_write<T, 8, 8>(c, k, ld_k, v, ld_v, n, dev_status, stream);
+    return by_size(c.D, [&](auto groups) {
+        constexpr int NG = decltype(groups)::value;
+        if (c.k_bits == 4) return launch_write<T, NG, 4, 4>(c, k, ld_k, v, ld_v, n, dev_status, stream);
+        if (c.v_bits == 4) return launch_write<T, NG, 8, 4>(c, k, ld_k, v, ld_v, n, dev_status, stream);
+        return launch_write<T, NG, 8, 8>(c, k, ld_k, v, ld_v, n, dev_status, stream);
+    });
 }
 
 template <typename T>
 int read_typed(const b2kv_qcache& c, int which, void* out, int n, int last, int len_bias, int32_t* dev_status, void* stream) {
-    if (which == 0)
-        return c.k_bits == 4 ? launch_read<T, 4, false>(c, out, n, last, len_bias, dev_status, stream)
-                             : launch_read<T, 8, false>(c, out, n, last, len_bias, dev_status, stream);
-    return c.v_bits == 4 ? launch_read<T, 4, true>(c, out, n, last, len_bias, dev_status, stream)
-                         : launch_read<T, 8, true>(c, out, n, last, len_bias, dev_status, stream);
+    return by_size(c.D, [&](auto groups) {
+        constexpr int NG = decltype(groups)::value;
+        if (which == 0)
+            return c.k_bits == 4 ? launch_read<T, NG, 4, false>(c, out, n, last, len_bias, dev_status, stream)
+                                 : launch_read<T, NG, 8, false>(c, out, n, last, len_bias, dev_status, stream);
+        return c.v_bits == 4 ? launch_read<T, NG, 4, true>(c, out, n, last, len_bias, dev_status, stream)
+                             : launch_read<T, NG, 8, true>(c, out, n, last, len_bias, dev_status, stream);
+    });
 }
 
 }  // namespace

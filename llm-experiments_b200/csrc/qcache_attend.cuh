@@ -172,7 +172,7 @@ __device__ __forceinline__ int first_seen(const AttendParams& p, int n) { return
 // What a warp's ring holds: stages of 16 or 32 tokens, as many as fit with two CTAs per SM (one, where the registers leave room for no more).
 template <int NG, int KB, int VB, int NT>
 struct Ring {
-    static constexpr int kWarps = 8;
+    static constexpr int kWarps = NT == 1 && NG <= 4 ? 6 : 8;
     static constexpr int kCtas = NT == 1 && NG <= 4 ? 2 : 1;
     static constexpr int kToken = NG * 4 * (KB + VB) + 4 * scale_row(NG);
     static constexpr int kRoom = ((kCtas == 2 ? 112 : 224) * 1024 - NG * NT * 512 - NT * 512) / kWarps;  // (beside the queries, and a few hundred bytes more)
