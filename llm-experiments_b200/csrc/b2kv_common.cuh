@@ -239,6 +239,9 @@ __device__ __forceinline__ uint32_t peer_address(const void* local, uint32_t ran
 __device__ __forceinline__ void peer_store_u32(uint32_t local, uint32_t rank, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_address(local, rank)), "r"(v) : "memory");
 }
+__device__ __forceinline__ void peer_store4(uint32_t addr, const float (&v)[4]) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
+}
 __device__ __forceinline__ float2 peer_load2(uint32_t addr) {
     float2 v;
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");

@@ -4,6 +4,8 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 
 namespace b2kv {
 namespace qcache {
@@ -23,6 +25,9 @@ int check_attend(const b2kv_qcache* c, const b2kv_qcache_attend_args* a) {
     return B2KV_OK;
 }
 
+// Results of two pairs per CTA, their sums, and a ticket per pair.
+size_t tickets_at(const Plan& plan, const b2kv_qcache& c) { return static_cast<size_t>(plan.ctas) * 2 * plan.cols * (c.D + 1) * sizeof(float); }
+
 bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& plan) {
     const int columns = a.m * (a.H / c.G);
     plan.cols = c.dtype == B2KV_DTYPE_F32 || columns <= 8 ? 8 : 16;
@@ -30,8 +35,7 @@ bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& pla
     plan.pairs = static_cast<int64_t>(c.B) * c.G * plan.col_tiles;
     if (plan.pairs > 0x7fffffff) return false;
     const int most = a.window > 0 ? std::min(a.T_upper, a.window + a.m - 1) : a.T_upper;
-    // CTAs that run at the same time: two per SM for one tile of columns and heads up to 128, else one (Ring).
-    const int at_once = device_sm_count() * (c.dtype != B2KV_DTYPE_F32 && plan.cols == 8 && c.D <= 128 ? 2 : 1);
+    const int at_once = device_sm_count() * 2;  // CTAs that run at the same time
     // A cluster of 1, 2, 4 or 8 CTAs for each pair, or one run of tiles per CTA that is there.  In tokens that a CTA gets through in the time: setting
     // up and finishing a CTA is about 430, putting a cluster's results together 150, and the run's cuts with the second launch 1300.
     const int64_t runs = 1300 + plan.pairs * most / at_once;
@@ -48,7 +52,7 @@ bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& pla
     plan.workspace = 0;
     if (plan.cluster == 0) {
         plan.ctas = at_once;
-        plan.workspace = static_cast<size_t>(at_once) * 2 * plan.cols * (c.D + 1) * sizeof(float);
+        plan.workspace = tickets_at(plan, c) + static_cast<size_t>(plan.pairs) * sizeof(unsigned long long);
     } else {
         if (plan.pairs * plan.cluster > 0x7fffffff) return false;
         plan.ctas = static_cast<int>(plan.pairs) * plan.cluster;
@@ -91,6 +95,10 @@ int b2kv_qcache_attend(const b2kv_qcache* cache, const b2kv_qcache_attend_args* 
     p.scale = a.scale, p.softcap = a.softcap;
     p.ws_o = static_cast<float*>(workspace);
     p.ws_lse = p.ws_o + static_cast<size_t>(plan.ctas) * 2 * plan.cols * c.D;
+    p.tickets = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + tickets_at(plan, c));
+    static std::atomic<unsigned long long> calls{static_cast<unsigned long long>(std::chrono::steady_clock::now().time_since_epoch().count())};
+    do p.call = calls.fetch_add(1, std::memory_order_relaxed) & 0xffffffffffull;
+    while (p.call == 0);
     switch (c.D) {
         case 32: return attend_32(p, plan, stream);
         case 64: return attend_64(p, plan, stream);

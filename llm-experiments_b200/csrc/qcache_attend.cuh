@@ -28,7 +28,7 @@
 
 #include <cuda_fp16.h>
 
-#include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "qcache.cuh"
@@ -43,6 +43,8 @@ struct AttendParams {
     const float* slopes;
     float* ws_o;    // [2 * CTAs, kCols, D]: what a CTA has of its first (sequence, head) and of its last, normalised
     float* ws_lse;  // [2 * CTAs, kCols]: log2 of the sum of exponentials
+    unsigned long long* tickets;  // [pairs]: (number of the call << 24) | pieces of the pair that are there
+    unsigned long long call;      // 40 bits, another for each call and never 0
     int32_t* dev_status;
     int64_t ld_q, ld_out;
     int R, m, col_tiles, T_upper, len_bias, window;
@@ -169,13 +171,13 @@ struct Words {
 // The first token that any query of a sequence of n tokens sees.
 __device__ __forceinline__ int first_seen(const AttendParams& p, int n) { return p.window > 0 ? max(n - p.m + 1 - p.window, 0) : 0; }
 
-// What a warp's ring holds: stages of 16 or 32 tokens, as many as fit with two CTAs per SM (one, where the registers leave room for no more).
+// What a warp's ring holds: stages of 16 or 32 tokens, as many as fit with two CTAs per SM.
 template <int NG, int KB, int VB, int NT>
 struct Ring {
-    static constexpr int kWarps = NT == 1 && NG <= 4 ? 6 : 8;
-    static constexpr int kCtas = NT == 1 && NG <= 4 ? 2 : 1;
+    static constexpr int kWarps = NT == 1 && NG <= 4 ? 6 : 4;  // of 168 or 255 registers per thread
+    static constexpr int kCtas = 2;
     static constexpr int kToken = NG * 4 * (KB + VB) + 4 * scale_row(NG);
-    static constexpr int kRoom = ((kCtas == 2 ? 112 : 224) * 1024 - NG * NT * 512 - NT * 512) / kWarps;  // (beside the queries, and a few hundred bytes more)
+    static constexpr int kRoom = (112 * 1024 - NG * NT * 512 - NT * 512) / kWarps;  // (beside the queries, and a few hundred bytes more)
     static constexpr int kTokens = 3 * 32 * kToken <= kRoom ? 32 : 16;
     static constexpr int kFit = kRoom / (kTokens * kToken);
     static constexpr int kStages = kFit > 6 ? 6 : kFit;
@@ -267,36 +269,40 @@ struct Attend {
     // fp32: both tiles are the same columns.
     __device__ static __forceinline__ int col_of(int nt, int c) { return kF32 ? c : nt * 8 + c; }
 
-    __device__ static void load8(const float* p, float (&x)[8]) {
-        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    // A lane's part of the queries of sequence b, head g, column tile ct as they lie in memory: octet tig of every group, of column gid of each tile.
+    struct Query {
+        uint4 w[kF32 ? 1 : NT][NG][sizeof(T) / 2];
+    };
+    __device__ static __forceinline__ void load_query(const AttendParams& p, Query& raw, int b, int g, int ct) {
+        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
+#pragma unroll
+        for (int nt = 0; nt < (kF32 ? 1 : NT); ++nt) {
+            const int col = ct * kCols + col_of(nt, gid), i = col / p.R, h = g * p.R + col - i * p.R;
+            const T* const src = static_cast<const T*>(p.q) + (static_cast<int64_t>(b) * p.m + i) * p.ld_q + static_cast<int64_t>(h) * D + tig * 8;
+#pragma unroll
+            for (int u = 0; u < NG; ++u)
+#pragma unroll
+                for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k)
+                    raw.w[nt][u][k] = col < p.m * p.R ? reinterpret_cast<const uint4*>(src + u * kGroup)[k] : make_uint4(0, 0, 0, 0);
+        }
     }
-    __device__ static void load8(const __nv_bfloat16* p, float (&x)[8]) { Elt<__nv_bfloat16>::widen(*reinterpret_cast<const uint4*>(p), x); }
 
-    // Queries of sequence b, head g, column tile ct, and what goes with them.  n: tokens of the sequence.
-    __device__ static __forceinline__ void begin(const AttendParams& p, Warp& w, uint4* queries, Column* columns, int b, int g, int ct, int n) {
+    // The queries and what goes with them.  n: tokens of the sequence.
+    __device__ static __forceinline__ void begin(const AttendParams& p, Warp& w, const Query& raw, uint4* queries, Column* columns, int g, int ct, int n) {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         const int used = p.m * p.R;
         w.all_lo = 0, w.all_lim = 0x7fffffff;
 #pragma unroll
         for (int nt = 0; nt < (kF32 ? 1 : NT); ++nt) {
-            const int col = ct * kCols + col_of(nt, gid);  // the column whose query this lane loads
+            const int col = ct * kCols + col_of(nt, gid);
             float x[NG][8];
             float most = 0.0f;
-            if (col < used) {
-                const int i = col / p.R, h = g * p.R + col - i * p.R;
-                const T* src = static_cast<const T*>(p.q) + (static_cast<int64_t>(b) * p.m + i) * p.ld_q + static_cast<int64_t>(h) * D;
 #pragma unroll
-                for (int u = 0; u < NG; ++u) {
-                    load8(src + u * kGroup + tig * 8, x[u]);
+            for (int u = 0; u < NG; ++u) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[u][e]));
-                }
-            } else {
+                for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k) Elt<T>::widen(raw.w[nt][u][k], x[u] + k * Elt<T>::kPerChunk);
 #pragma unroll
-                for (int u = 0; u < NG; ++u)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[u][e] = 0.0f;
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[u][e]));
             }
             most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
             most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
@@ -947,21 +953,25 @@ __device__ __forceinline__ int tiles_of(const AttendParams& p, int b) {  // at l
     return max(1, (n - first + TOK - 1) / TOK);
 }
 
-// How the tiles of all (sequence, head, column tile) pairs, laid end to end, are cut into pieces of the same size.  Every thread takes the same
-// stretch of sequences, whose sums are scanned; part[i] is what lies before stretch i.
+// The tiles of all (sequence, head, column tile) pairs, laid end to end, are cut into pieces of the same size (the first ones have one more).
+__device__ __forceinline__ int64_t piece_start(int i, int64_t total, int pieces) { return total / pieces * i + min(static_cast<int64_t>(i), total % pieces); }
+__device__ __forceinline__ int piece_of(int64_t u, int64_t total, int pieces) {
+    const int64_t each = total / pieces, more = total % pieces;
+    return static_cast<int>(u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each);
+}
+// Every thread adds up the same stretch of sequences; part[i] is what lies before stretch i.
 template <int TOK, int THREADS>
 struct Cut {
     const int64_t* part;
     int64_t total;
     int stretch;
 
-    __device__ static Cut make(const AttendParams& p, int64_t* part) {
+    __device__ __forceinline__ Cut(const AttendParams& p, int64_t* before) : part(before), total(0), stretch((p.c.B + THREADS - 1) / THREADS) {
         __shared__ int64_t sums[THREADS / 32];
-        Cut c{part, 0, (p.c.B + THREADS - 1) / THREADS};
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        const int from = threadIdx.x * c.stretch;
+        const int from = threadIdx.x * stretch;
         int64_t mine = 0;
-        for (int b = from; b < min(from + c.stretch, p.c.B); ++b) mine += tiles_of<TOK>(p, b);
+        for (int b = from; b < min(from + stretch, p.c.B); ++b) mine += tiles_of<TOK>(p, b);
         int64_t sum = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -970,40 +980,32 @@ struct Cut {
         }
         if (lane == 31) sums[warp] = sum;
         __syncthreads();
-        int64_t before = 0;
+        int64_t first = 0;
 #pragma unroll
         for (int i = 0; i < THREADS / 32; ++i) {
-            if (i < warp) before += sums[i];
-            c.total += sums[i];
+            if (i < warp) first += sums[i];
+            total += sums[i];
         }
-        part[threadIdx.x] = before + sum - mine;
+        before[threadIdx.x] = first + sum - mine;
         __syncthreads();
-        c.total *= pairs_each(p);
-        return c;
-    }
-    __device__ static __forceinline__ int pairs_each(const AttendParams& p) { return p.c.G * p.col_tiles; }
-    // First tile of piece i of `pieces`.
-    __device__ __forceinline__ int64_t start(int i, int pieces) const { return total / pieces * i + min(static_cast<int64_t>(i), total % pieces); }
-    // The piece that tile u lies in.
-    __device__ __forceinline__ int piece_of(int64_t u, int pieces) const {
-        const int64_t each = total / pieces, more = total % pieces;  // the first `more` have one more
-        return static_cast<int>(u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each);
+        total *= p.c.G * p.col_tiles;
     }
     // The sequence that tile u lies in, and its first tile.
     __device__ __forceinline__ int sequence_of(const AttendParams& p, int64_t u, int64_t& first) const {
-        const int each = pairs_each(p);
+        const int each = p.c.G * p.col_tiles;
         int lo = 0, hi = THREADS - 1;
         while (lo < hi) {  // the last stretch that begins at or before u
             const int mid = (lo + hi + 1) >> 1;
             if (part[mid] * each <= u) lo = mid; else hi = mid - 1;
         }
-        int b = lo * stretch;
+        int b = min(lo * stretch, p.c.B - 1);
         first = part[lo] * each;
-        for (;;) {
+        while (stretch > 1 && b + 1 < p.c.B) {
             const int64_t next = first + static_cast<int64_t>(tiles_of<TOK>(p, b)) * each;
-            if (u < next || b + 1 >= p.c.B) return b;
+            if (u < next) break;
             first = next, ++b;
         }
+        return b;
     }
 };
 
@@ -1049,12 +1051,15 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
     uint4* const queries = reinterpret_cast<uint4*>(smem + A::kRing + A::kMl + 16 * ((W * 4 + 15) / 16));
     __shared__ Place<kTok> now[W], ahead[W];
     __shared__ uint32_t there[W][S];  // which tokens of a stage are there
+    __shared__ int pieces[3];
     const int warp = threadIdx.x >> 5;
     const uint32_t ring = smem_u32(smem) + warp * S * A::kStage;
     grid_dependency_wait();
 
     // This CTA's run of tiles, and which of a pair's tokens are this warp's: kTok from `skip` on, `step` further on the next ones.
     int step = W * kTok, skip = warp * kTok;
+    typename A::Query raw;
+    int64_t at_tile = 0, total = 0;  // the run's place among all tiles
     {
         Place<kTok> at;
         if (p.cluster > 0) {
@@ -1066,17 +1071,20 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
             at.take(0, at.tiles);
             skip += step * (blockIdx.x - in_all * p.cluster);
             step *= p.cluster;
+            A::load_query(p, raw, at.b, at.g, at.ct);
         } else {
-            const auto cut = Cut<kTok, kThreads>::make(p, reinterpret_cast<int64_t*>(smem));
-            const int64_t from = cut.start(blockIdx.x, gridDim.x);
-            const int run = static_cast<int>(cut.start(blockIdx.x + 1, gridDim.x) - from);
+            const Cut<kTok, kThreads> cut(p, reinterpret_cast<int64_t*>(smem));
+            total = cut.total;
+            at_tile = piece_start(blockIdx.x, total, gridDim.x);
+            const int run = static_cast<int>(piece_start(blockIdx.x + 1, total, gridDim.x) - at_tile);
             int64_t start;
-            at.b = cut.sequence_of(p, from, start);
+            at.b = cut.sequence_of(p, at_tile, start);
             at.sequence(p);
-            const int pair = static_cast<int>((from - start) / at.tiles);
-            at.take(static_cast<int>((from - start) - static_cast<int64_t>(pair) * at.tiles), run);
+            const int pair = static_cast<int>((at_tile - start) / at.tiles);
+            at.take(static_cast<int>((at_tile - start) - static_cast<int64_t>(pair) * at.tiles), run);
             at.g = pair / p.col_tiles, at.ct = pair - at.g * p.col_tiles;
-            __syncthreads();  // (the scan lies where the ring does)
+            if (run > 0) A::load_query(p, raw, at.b, at.g, at.ct);  // (ahead of the copies, which would hold it up)
+            __syncthreads();                                       // (the scan lies where the ring does)
             if (run <= 0) return;
         }
         now[warp] = ahead[warp] = at;
@@ -1124,13 +1132,9 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
     int slot = 0;
     bool first_of_run = true;
     for (;;) {
-        int t, end;
-        {
-            const Place<kTok>& at = now[warp];
-            A::begin(p, q, queries, columns, at.b, at.g, at.ct, at.n);
-            t = at.first + at.tile * kTok + skip;
-            end = at.first + at.end * kTok;
-        }
+        int t = now[warp].first + now[warp].tile * kTok + skip;
+        const int end = now[warp].first + now[warp].end * kTok;
+        A::begin(p, q, raw, queries, columns, now[warp].g, now[warp].ct, now[warp].n);
         for (; t < end; t += step) {
             copy_wait<S - 2>();
             __syncwarp();
@@ -1138,13 +1142,22 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
             A::fold(p, l, q, queries, columns, ring + slot * A::kStage, t, there[warp][slot]);
             slot = slot == S - 1 ? 0 : slot + 1;
         }
-        // The warps' results, in the stage of each ring that the next copy goes to.
-        const uint32_t mine = static_cast<uint32_t>((warp * S + (slot == 0 ? S - 1 : slot - 1)) * A::kStage);
-        __syncwarp();
+        if (p.cluster > 1) {
+            copy_wait<0>();
+            cluster_arrive();  // this CTA's ring is free for the others' results
+        }
+        // The pair, and on to the next one, whose queries are on their way while the warps' results are put together.
+        const int b = now[warp].b, g = now[warp].g, ct = now[warp].ct, tile = now[warp].tile, tiles = now[warp].tiles;
+        const int64_t from = at_tile;
+        at_tile += now[warp].end - tile;
+        const bool whole = p.cluster == 1 || (p.cluster == 0 && tile == 0 && now[warp].end == tiles);
+        const bool on = p.cluster == 0 && now[warp].next(p);
+        if (on) A::load_query(p, raw, now[warp].b, now[warp].g, now[warp].ct);
+
+        // The warps' results, in the stage of each ring that the next copy goes to (clusters: in the first one, all are free).
+        const uint32_t mine = static_cast<uint32_t>((warp * S + (p.cluster > 1 ? 0 : slot == 0 ? S - 1 : slot - 1)) * A::kStage);
         A::leave_sums(q, ml + warp * A::kCols * 2);
         if ((threadIdx.x & 31) == 0) left_at[warp] = mine;
-        const int b = now[warp].b, g = now[warp].g, ct = now[warp].ct;
-        const bool whole = p.cluster == 1 || (p.cluster == 0 && now[warp].tile == 0 && now[warp].end == now[warp].tiles);
         const int used = min(p.m * p.R - ct * A::kCols, A::kCols);
         constexpr int kQuads = A::kRoundCols * D / 4, kPer = (kQuads + kThreads - 1) / kThreads;
         float kept[A::kRounds * kPer][4];
@@ -1164,10 +1177,9 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
                     float top = kNegInf, total = 0.0f;
 #pragma unroll
                     for (int j = 0; j < W; ++j) top = fmaxf(top, ml[(j * A::kCols + col) * 2]);
-                    const float ref = top == kNegInf ? 0.0f : top;
 #pragma unroll
                     for (int j = 0; j < W; ++j) {
-                        const float l = ml[(j * A::kCols + col) * 2 + 1] * ex2(ml[(j * A::kCols + col) * 2] - ref);
+                        const float l = ml[(j * A::kCols + col) * 2 + 1] * ex2(ml[(j * A::kCols + col) * 2] - top);
                         const float4 y = *reinterpret_cast<const float4*>(smem + left_at[j] + (in_round * D + d) * 4);
                         total += l;
                         x[0] += l * y.x, x[1] += l * y.y, x[2] += l * y.z, x[3] += l * y.w;
@@ -1175,7 +1187,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
                     const float by = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[e] *= by;
-                    kept_lse[r * kPer + k] = total == 0.0f ? kNegInf : ref + log2f(total);
+                    kept_lse[r * kPer + k] = total == 0.0f ? kNegInf : top + log2f(total);
                     if (whole) {
                         A::store(A::out_row(p, b, g, ct * A::kCols + col) + d, x);
                     } else if (p.cluster == 0) {
@@ -1185,96 +1197,109 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
                     }
                 }
             }
-            __syncthreads();
+            if (r + 1 < A::kRounds || p.cluster == 0) __syncthreads();
         }
         if (p.cluster > 1) {
-            // One pair per cluster: the CTAs' results, each left at the start of its ring, and each CTA puts its share of the columns together.
-            float* const o = reinterpret_cast<float*>(smem);
-            float* const lse = o + A::kCols * D;
-            static_assert(A::kCols * (D + 1) * 4 <= A::kRing, "");
+            // One pair per cluster.  Every CTA has a share of the columns' elements, quads rank, rank + cluster, ... of them, and gets all CTAs' results for
+            // it, each behind the other, into the rings (all but the first stages), and their sums to where the queries were.
+            constexpr int kRoom = (S - 1) * A::kStage / 16;  // quads in a warp's ring
+            static_assert(A::kCols * D / 4 <= W * kRoom && 8 * A::kCols * 4 <= NG * NT * 512, "");
+            const auto where = [](int quad) { return static_cast<uint32_t>(quad / kRoom * (S * A::kStage) + A::kStage + quad % kRoom * 16); };
+            const uint32_t their_lse = smem_u32(queries);
+            const int rank = static_cast<int>(cluster_rank()), each = (A::kCols * D / 4 + p.cluster - 1) / p.cluster;
+            cluster_wait();
 #pragma unroll
             for (int k = 0; k < A::kRounds * kPer; ++k) {
                 const int i = threadIdx.x + k % kPer * kThreads;
-                const int in_round = i / (D / 4), col = k / kPer * A::kRoundCols + in_round, d = (i - in_round * (D / 4)) * 4;
-                if (kQuads % kThreads == 0 || i < kQuads) {
-                    *reinterpret_cast<float4*>(o + col * D + d) = make_float4(kept[k][0], kept[k][1], kept[k][2], kept[k][3]);
-                    if (d == 0) lse[col] = kept_lse[k];
+                const int quad = k / kPer * kQuads + i, col = quad / (D / 4);
+                if ((kQuads % kThreads == 0 || i < kQuads) && col < used) {
+                    peer_store4(peer_address(smem_u32(smem) + where(rank * each + quad / p.cluster), quad % p.cluster), kept[k]);
+                    if (quad % (D / 4) == 0)
+                        for (int j = 0; j < p.cluster; ++j) peer_store_u32(their_lse + (rank * A::kCols + col) * 4, j, __float_as_uint(kept_lse[k]));
                 }
             }
             cluster_sync();
-            const uint32_t o_at = smem_u32(o), lse_at = smem_u32(lse);
-            const int rank = static_cast<int>(cluster_rank());
-            for (int i = threadIdx.x + rank * kThreads; i < used * (D / 2); i += kThreads * p.cluster) {
-                const int col = i / (D / 2), d = (i - col * (D / 2)) * 2;
-                float top = kNegInf, total = 0.0f, x0 = 0.0f, x1 = 0.0f;
-                for (int j = 0; j < p.cluster; ++j) top = fmaxf(top, __int_as_float(peer_load1(peer_address(lse_at + col * 4, j))));
+            const float* const lse = reinterpret_cast<const float*>(queries);
+            for (int i = threadIdx.x; i * p.cluster + rank < used * (D / 4); i += kThreads) {
+                const int quad = i * p.cluster + rank, col = quad / (D / 4), d = (quad - col * (D / 4)) * 4;
+                float top = kNegInf, total = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int j = 0; j < p.cluster; ++j) top = fmaxf(top, lse[j * A::kCols + col]);
                 const float ref = top == kNegInf ? 0.0f : top;
                 for (int j = 0; j < p.cluster; ++j) {
-                    const float l = ex2(__int_as_float(peer_load1(peer_address(lse_at + col * 4, j))) - ref);
-                    const float2 y = peer_load2(peer_address(o_at + (col * D + d) * 4, j));
+                    const float l = ex2(lse[j * A::kCols + col] - ref);
+                    const float4 y = *reinterpret_cast<const float4*>(smem + where(j * each + i));
                     total += l;
-                    x0 += l * y.x, x1 += l * y.y;
+                    x[0] += l * y.x, x[1] += l * y.y, x[2] += l * y.z, x[3] += l * y.w;
                 }
                 const float by = total == 0.0f ? 0.0f : 1.0f / total;
-                T* const out = A::out_row(p, b, g, ct * A::kCols + col) + d;
-                out[0] = Elt<T>::from_float(x0 * by), out[1] = Elt<T>::from_float(x1 * by);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] *= by;
+                A::store(A::out_row(p, b, g, ct * A::kCols + col) + d, x);
             }
-            cluster_sync();  // nobody leaves while its results are read
+        } else if (p.cluster == 0 && !whole) {
+            // A pair that was cut: the CTA that brings its last piece puts them together.  (The rounds' last barrier has ordered this CTA's stores.)
+            if (threadIdx.x == 0) {
+                const int64_t first = from - tile;
+                const int c0 = piece_of(first, total, gridDim.x), c1 = piece_of(first + tiles - 1, total, gridDim.x);
+                __threadfence();
+                unsigned long long* const word = p.tickets + (static_cast<int64_t>(b) * p.c.G + g) * p.col_tiles + ct;
+                // the word may hold anything: the first piece to come makes it this call's
+                const unsigned long long old = *reinterpret_cast<volatile unsigned long long*>(word), own = p.call << 24;
+                if (old >> 24 != p.call) atomicCAS(word, old, own);
+                const int before = static_cast<int>(atomicAdd(word, 1ull) & 0xffffffu);
+                const bool last = before == c1 - c0;
+                if (last) {
+                    atomicExch(word, 0ull);  // (a launch replayed from a graph has the same number)
+                    __threadfence();
+                }
+                // the first piece is its CTA's last pair, unless it is its first one too
+                pieces[0] = last ? c1 - c0 + 1 : 0;
+                pieces[1] = 2 * c0 + (piece_start(c0, total, gridDim.x) < first ? 1 : 0);
+                pieces[2] = 2 * (c0 + 1);
+            }
+            __syncthreads();
+            const int n = pieces[0], piece0 = pieces[1], piece1 = pieces[2];
+            const auto place = [&](int i, int col) { return static_cast<int64_t>(i == 0 ? piece0 : piece1 + 2 * (i - 1)) * A::kCols + col; };
+            if (n > 0) {
+                for (int i = threadIdx.x; i < used * (D / 4); i += kThreads) {
+                    const int col = i / (D / 4), d = (i - col * (D / 4)) * 4;
+                    // the pieces' results in the order of the tokens, each taken relative to the largest so far
+                    float top = kLowest, total_weight = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int j0 = 0; j0 < n; j0 += 4) {
+                        float lse[4];
+                        float4 y[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int64_t at = place(min(j0 + j, n - 1), col);
+                            lse[j] = j0 + j < n ? __ldcg(p.ws_lse + at) : kNegInf;
+                            y[j] = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * D + d));
+                        }
+                        float most = fmaxf(fmaxf(lse[0], lse[1]), fmaxf(lse[2], lse[3]));
+                        most = fmaxf(most, top);
+                        const float by = ex2(top - most);
+                        top = most;
+                        total_weight *= by;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] *= by;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float l = ex2(lse[j] - top);
+                            total_weight += l;
+                            if (j0 + j < n) x[0] += l * y[j].x, x[1] += l * y[j].y, x[2] += l * y[j].z, x[3] += l * y[j].w;
+                        }
+                    }
+                    const float by = total_weight == 0.0f ? 0.0f : 1.0f / total_weight;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] *= by;
+                    A::store(A::out_row(p, b, g, ct * A::kCols + col) + d, x);
+                }
+            }
+            __syncthreads();  // (pieces)
         }
         first_of_run = false;
-        if (p.cluster > 0 || !now[warp].next(p)) break;
+        if (!on) break;
     }
     copy_wait<0>();
-}
-
-// Pairs that were cut, put together: one CTA per cut and column; the first cut of a pair has it.
-template <typename T, int D, int COLS, int TOK>
-__global__ void __launch_bounds__(256) merge_kernel(const AttendParams p, int pieces) {
-    __shared__ int64_t part[256];
-    __shared__ float sums[256 / (D / 4)][D + 1];
-    grid_dependency_wait();
-    const auto cut = Cut<TOK, 256>::make(p, part);
-    const int c0 = blockIdx.x;  // the cut is between pieces c0 and c0 + 1
-    const int64_t at_cut = cut.start(c0 + 1, pieces);
-    if (at_cut >= cut.total) return;
-    int64_t first;
-    const int b = cut.sequence_of(p, at_cut, first), tiles = tiles_of<TOK>(p, b);
-    const int pair = static_cast<int>((at_cut - first) / tiles), g = pair / p.col_tiles, ct = pair - g * p.col_tiles;
-    first += static_cast<int64_t>(pair) * tiles;
-    const int64_t before = cut.start(c0, pieces);
-    const int mine = ct * COLS + blockIdx.y;
-    if (first == at_cut || before > first || mine >= p.m * p.R) return;
-    const int c1 = cut.piece_of(first + tiles - 1, pieces);
-    // the first CTA has it as its last pair, unless it is its first one too
-    const auto place = [&](int c) { return (2ll * c + (c == c0 && before < first ? 1 : 0)) * COLS + blockIdx.y; };
-    float top = kNegInf;
-    for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.ws_lse[place(c)]);
-    const float ref = top == kNegInf ? 0.0f : top;
-    constexpr int kLanes = D / 4, kRows = 256 / kLanes;
-    const int lane = threadIdx.x % kLanes, r = threadIdx.x / kLanes;
-    float total = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (r < kRows)
-        for (int c = c0 + r; c <= c1; c += kRows) {
-            const int64_t at = place(c);
-            const float l = ex2(p.ws_lse[at] - ref);
-            const float4 y = *reinterpret_cast<const float4*>(p.ws_o + at * D + lane * 4);
-            total += l;
-            x[0] += l * y.x, x[1] += l * y.y, x[2] += l * y.z, x[3] += l * y.w;
-        }
-    if (r < kRows) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sums[r][lane * 4 + e] = x[e];
-        if (lane == 0) sums[r][D] = total;
-    }
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= D) return;
-    float y = 0.0f, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) y += sums[i][d], l += sums[i][D];
-    y = l == 0.0f ? 0.0f : y / l;
-    const int i = mine / p.R, h = g * p.R + mine - i * p.R;
-    static_cast<T*>(p.out)[(static_cast<int64_t>(b) * p.m + i) * p.ld_out + static_cast<int64_t>(h) * D + d] = Elt<T>::from_float(y);
 }
 
 struct Plan {
@@ -1287,13 +1312,15 @@ template <typename T, int NG, int KB, int VB, int NT>
 int launch_attend(const AttendParams& p, const Plan& plan, void* stream) {
     using A = Attend<T, NG, KB, VB, NT>;
     auto kernel = attend_kernel<T, NG, KB, VB, NT>;
-    B2KV_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, A::kSmem));
+    static std::atomic<bool> ready[64];
+    int device = 0;
+    B2KV_CUDA_TRY(cudaGetDevice(&device));
+    if (device >= 64 || !ready[device].load(std::memory_order_relaxed)) {
+        B2KV_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, A::kSmem));
+        if (device < 64) ready[device].store(true, std::memory_order_relaxed);
+    }
     OverlapLaunch launch(dim3(static_cast<unsigned>(plan.ctas)), A::kThreads, A::kSmem, stream, plan.cluster > 1 ? plan.cluster : 1);
     B2KV_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, kernel, p));
-    if (plan.cluster == 0) {
-        OverlapLaunch second(dim3(plan.ctas - 1, std::min(A::kCols, p.m * p.R)), 256, 0, stream);
-        B2KV_CUDA_TRY(cudaLaunchKernelEx(&second.cfg, merge_kernel<T, A::D, A::kCols, A::kTok>, p, plan.ctas));
-    }
     return B2KV_OK;
 }
 
