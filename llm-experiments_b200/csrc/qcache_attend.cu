@@ -37,18 +37,20 @@ bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& pla
     const int most = a.window > 0 ? std::min(a.T_upper, a.window + a.m - 1) : a.T_upper;
     const int at_once = device_sm_count() * 2;  // CTAs that run at the same time
     // A cluster of 1, 2, 4 or 8 CTAs for each pair, or one run of tiles per CTA that is there.  In tokens that a CTA gets through in the time: setting
-    // up and finishing a CTA is about 430, putting a cluster's results together 150, and the run's cuts with the second launch 1300.
-    const int64_t runs = 1300 + plan.pairs * most / at_once;
+    // up and finishing a CTA is about 430, putting a cluster's results together 150, finding and cutting a run 1000.
+    const int64_t runs = 1000 + plan.pairs * most / at_once;
     int64_t best = 0;
     for (int size = 1; size <= 8; size *= 2) {
         const int64_t waves = (plan.pairs * size + at_once - 1) / at_once;
         const int64_t cost = waves * (430 + (size > 1 ? 150 : 0) + (most + size - 1) / size);
         if (size == 1 || cost < best) best = cost, plan.cluster = size;
     }
-    if (runs < best) plan.cluster = 0;
+    // (a run counts units in 32 bits)
+    const bool countable = plan.pairs * (most / 16 + 1 + kPairCost) < (1ll << 31);
+    if (runs < best && countable) plan.cluster = 0;
     const int forced = tune_get("qcache_cluster");
     if (forced == 1 || forced == 2 || forced == 4 || forced == 8) plan.cluster = forced;
-    if (forced < 0) plan.cluster = 0;
+    if (forced < 0 && countable) plan.cluster = 0;
     plan.workspace = 0;
     if (plan.cluster == 0) {
         plan.ctas = at_once;
