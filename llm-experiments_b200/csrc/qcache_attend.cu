@@ -30,12 +30,16 @@ size_t tickets_at(const Plan& plan, const b2kv_qcache& c) { return static_cast<s
 
 bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& plan) {
     const int columns = a.m * (a.H / c.G);
-    plan.cols = c.dtype == B2KV_DTYPE_F32 || columns <= 8 ? 8 : 16;
-    plan.col_tiles = (columns + plan.cols - 1) / plan.cols;
-    plan.pairs = static_cast<int64_t>(c.B) * c.G * plan.col_tiles;
-    if (plan.pairs > 0x7fffffff) return false;
     const int most = a.window > 0 ? std::min(a.T_upper, a.window + a.m - 1) : a.T_upper;
+    const int64_t heads = static_cast<int64_t>(c.B) * c.G;
     const int at_once = device_sm_count() * 2;  // CTAs that run at the same time
+    // Columns (new token, query head) of a key / value head that are taken together: 16 share the widening of the codes (4 sequences of 131072
+    // tokens, 16 heads to one: 198 against 242 us), 8 make more pairs where there are few tokens to a CTA (40 columns over 2048 tokens: 22.1 against 25.5 us).
+    const bool wide = c.dtype != B2KV_DTYPE_F32 && columns > 8 && heads * ((columns + 15) / 16) * most >= at_once * 1024ll;
+    plan.cols = wide ? 16 : 8;
+    plan.col_tiles = (columns + plan.cols - 1) / plan.cols;
+    plan.pairs = heads * plan.col_tiles;
+    if (plan.pairs > 0x7fffffff) return false;
     // A cluster of 1, 2, 4 or 8 CTAs for each pair, or one run of tiles per CTA that is there.  In tokens that a CTA gets through in the time: setting
     // up and finishing a CTA is about 430, putting a cluster's results together 150, finding and cutting a run 1000.
     const int64_t runs = 1000 + plan.pairs * most / at_once;

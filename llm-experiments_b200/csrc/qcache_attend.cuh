@@ -177,7 +177,8 @@ struct Ring {
     static constexpr int kWarps = NT == 1 && NG <= 4 ? 6 : 4;  // of 168 or 255 registers per thread
     static constexpr int kCtas = 2;
     static constexpr int kToken = NG * 4 * (KB + VB) + 4 * scale_row(NG);
-    static constexpr int kRoom = (112 * 1024 - NG * NT * 512 - NT * 512) / kWarps;  // (beside the queries, and a few hundred bytes more)
+    // Half of what an SM has for two CTAs, less the queries, what is kept per column, and 1 KB of small things.
+    static constexpr int kRoom = (113 * 1024 - 1024 - NG * NT * 512 - NT * (640 + kWarps * 64) - 64) / kWarps;
     static constexpr int kTokens = 3 * 32 * kToken <= kRoom ? 32 : 16;
     static constexpr int kFit = kRoom / (kTokens * kToken);
     static constexpr int kStages = kFit > 6 ? 6 : kFit;
@@ -202,8 +203,7 @@ struct Attend {
     static constexpr int kRounds = kCols / kRoundCols;
     static_assert(kRoundCols * D * 4 <= kStage && kRoundCols % 2 == 0, "");
     static constexpr int kMl = WARPS * kCols * 2 * 4;
-    static constexpr int kSmem = kRing + kMl + 16 * ((WARPS * 4 + 15) / 16) + NG * NT * 512;
-    // The centre of the keys costs -kKOff * sum over groups of (key scale) * (sum of the group's query): a product over the groups, the sums
+        // The centre of the keys costs -kKOff * sum over groups of (key scale) * (sum of the group's query): a product over the groups, the sums
     // in three bfloat16 parts (16 places: part k / kSG of group k % kSG; with 8 groups in two products).
     static constexpr int kSG = scale_row(NG), kOffs = kF32 ? 1 : kSG == 8 ? 4 : 2;
     static constexpr int kKOff = KB == 4 ? 8 : 128;  // what is added to a key's code
@@ -269,116 +269,122 @@ struct Attend {
     // fp32: both tiles are the same columns.
     __device__ static __forceinline__ int col_of(int nt, int c) { return kF32 ? c : nt * 8 + c; }
 
-    // A lane's part of the queries of sequence b, head g, column tile ct as they lie in memory: octet tig of every group, of column gid of each tile.
+    // The queries of a pair are prepared by the CTA's warps together: unit i, group i % NG of the columns of tile i / NG, is warp i % WARPS's.
+    static constexpr int kUnits = (kF32 ? 1 : NT) * NG, kUnitsEach = (kUnits + WARPS - 1) / WARPS;
+    struct Prepared {
+        uint32_t most[kUnits / NG][8][NG];  // largest magnitude of a column's group, as a whole number (NaN above infinity above all others)
+        float sum[kUnits / NG][8][kSG];     // what the centre of its keys comes to
+        Column columns[kCols];
+        uint4 queries[NG * NT * 32];        // the second operand of S = K q, both steps of a group in one
+    };
+    static constexpr int kSmem = kRing + kMl + 16 * ((WARPS * 4 + 15) / 16) + static_cast<int>(sizeof(Prepared));
+    // A lane's part of them as they lie in memory: octet tig of its warp's groups, of column gid.
     struct Query {
-        uint4 w[kF32 ? 1 : NT][NG][sizeof(T) / 2];
+        uint4 w[kUnitsEach][sizeof(T) / 2];
     };
     __device__ static __forceinline__ void load_query(const AttendParams& p, Query& raw, int b, int g, int ct) {
-        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
+        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3, warp = threadIdx.x >> 5;
 #pragma unroll
-        for (int nt = 0; nt < (kF32 ? 1 : NT); ++nt) {
-            const int col = ct * kCols + col_of(nt, gid), i = col / p.R, h = g * p.R + col - i * p.R;
-            const T* const src = static_cast<const T*>(p.q) + (static_cast<int64_t>(b) * p.m + i) * p.ld_q + static_cast<int64_t>(h) * D + tig * 8;
+        for (int i = 0; i < kUnitsEach; ++i) {
+            const int unit = warp + i * WARPS, nt = unit / NG, u = unit - nt * NG;
+            const int col = ct * kCols + col_of(nt, gid), row = col / p.R, h = g * p.R + col - row * p.R;
+            const bool is = (kUnits % WARPS == 0 || unit < kUnits) && col < p.m * p.R;
+            const T* const src = static_cast<const T*>(p.q) + (static_cast<int64_t>(b) * p.m + row) * p.ld_q + static_cast<int64_t>(h) * D + u * kGroup + tig * 8;
 #pragma unroll
-            for (int u = 0; u < NG; ++u)
-#pragma unroll
-                for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k)
-                    raw.w[nt][u][k] = col < p.m * p.R ? reinterpret_cast<const uint4*>(src + u * kGroup)[k] : make_uint4(0, 0, 0, 0);
+            for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k)
+                raw.w[i][k] = is ? reinterpret_cast<const uint4*>(src)[k] : make_uint4(0, 0, 0, 0);
         }
     }
 
-    // The queries and what goes with them.  n: tokens of the sequence.
-    __device__ static __forceinline__ void begin(const AttendParams& p, Warp& w, const Query& raw, uint4* queries, Column* columns, int g, int ct, int n) {
-        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
-        const int used = p.m * p.R;
-        w.all_lo = 0, w.all_lim = 0x7fffffff;
+    // The CTA's part in it (two barriers), then the warp's own.  n: tokens of the sequence.
+    __device__ static __forceinline__ void begin(const AttendParams& p, Warp& w, const Query& raw, Prepared& q, int g, int ct, int n) {
+        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3, warp = threadIdx.x >> 5;
+        float x[kUnitsEach][8];
+#pragma unroll
+        for (int i = 0; i < kUnitsEach; ++i) {
+            const int unit = warp + i * WARPS, nt = unit / NG, u = unit - nt * NG;
+#pragma unroll
+            for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k) Elt<T>::widen(raw.w[i][k], x[i] + k * Elt<T>::kPerChunk);
+            uint32_t most = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(x[i][e]) & 0x7fffffffu);
+            most = max(most, __shfl_xor_sync(~0u, most, 1));
+            most = max(most, __shfl_xor_sync(~0u, most, 2));
+            if (tig == 0 && (kUnits % WARPS == 0 || unit < kUnits)) q.most[nt][gid][u] = most;
+        }
+        __syncthreads();
+        // q = qn * 2^e with the largest |qn| of a column in [2^14, 2^15): exact, and no fp16 overflow.  The exponent, biased:
+        const auto exponent = [&](int nt, int c) {
+            uint32_t most = q.most[nt][c][0];
+#pragma unroll
+            for (int u = 1; u < NG; ++u) most = max(most, q.most[nt][c][u]);
+            return min(max(static_cast<int>(most >> 23), 27), 254);
+        };
+#pragma unroll
+        for (int i = 0; i < kUnitsEach; ++i) {
+            const int unit = warp + i * WARPS, nt = unit / NG, u = unit - nt * NG;
+            if (kUnits % WARPS != 0 && unit >= kUnits) break;  // (a warp's lanes all the same)
+            const float down = __int_as_float((254 + 14 - exponent(nt, gid)) << 23);
+            uint32_t high[4], low[4];
+            float sum = 0.0f;  // of what the products see
+            // elements in the order of the codes in a word's halves: 4 bits (0,4) (1,5) (2,6) (3,7), the odd ones 16 times too
+            // large there; 8 bits (0,1) (2,3) (4,5) (6,7)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float by = KB == 4 && (j & 1) ? 0.0625f : 1.0f;
+                const float a = x[i][KB == 4 ? j : 2 * j] * (down * by), c = x[i][KB == 4 ? j + 4 : 2 * j + 1] * (down * by);
+                high[j] = pack_half(a, c);
+                const float2 got = unpack_half(high[j]);
+                sum += (got.x + got.y) * (1.0f / by);
+                if constexpr (kF32) low[j] = pack_half(a - got.x, c - got.y);
+            }
+            q.queries[unit * 32 + lane] = make_uint4(high[0], high[1], high[2], high[3]);
+            if constexpr (kF32) q.queries[(NG + u) * 32 + lane] = make_uint4(low[0], low[1], low[2], low[3]);
+            sum += __shfl_xor_sync(~0u, sum, 1);
+            sum += __shfl_xor_sync(~0u, sum, 2);
+            if (tig == 0) {
+                q.sum[nt][gid][u] = sum * (-static_cast<float>(kKOff) * kKeyUnit);
+                if (u == NG - 1)
+                    for (int v = NG; v < kSG; ++v) q.sum[nt][gid][v] = 0.0f;
+            }
+        }
+        if (threadIdx.x < kCols) {
+            const int c = threadIdx.x, col = ct * kCols + c, i = col / p.R, place = n - p.m + i;
+            const bool is = col < p.m * p.R;
+            // a score is scale * 2^(e - 14) over what a code of one is in the product
+            const float f = p.scale * kLog2e * 0x1p-14f / kKeyUnit * __int_as_float(exponent(c / 8, c % 8) << 23);
+            q.columns[c] = Column{is && p.window > 0 ? max(place + 1 - p.window, 0) : 0, is ? place + 1 : 0,
+                                  is && p.slopes != nullptr ? p.slopes[g * p.R + col - i * p.R] * kLog2e : 0.0f, f};
+        }
+        __syncthreads();
+
+        const Column c = q.columns[lane & (kCols - 1)];
+        const bool is = ct * kCols + (lane & (kCols - 1)) < p.m * p.R;
+        w.all_lim = __reduce_min_sync(~0u, is ? c.lim : 0x7fffffff);
+        w.all_lo = __reduce_max_sync(~0u, is ? c.lo : 0);
+        const bool plain = p.softcap == 0.0f && p.slopes == nullptr;
 #pragma unroll
         for (int nt = 0; nt < (kF32 ? 1 : NT); ++nt) {
-            const int col = ct * kCols + col_of(nt, gid);
-            float x[NG][8];
-            float most = 0.0f;
 #pragma unroll
-            for (int u = 0; u < NG; ++u) {
-#pragma unroll
-                for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k) Elt<T>::widen(raw.w[nt][u][k], x[u] + k * Elt<T>::kPerChunk);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[u][e]));
-            }
-            most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
-            most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
-            // q = qn * 2^e with the largest |qn| in [2^14, 2^15): exact, and no fp16 overflow
-            const int biased = min(max(__float_as_int(most) >> 23, 27), 254);
-            const float down = __int_as_float((254 + 14 - biased) << 23);
-            // scale * 2^(e - 14) over what a code of one is in the product
-            const float f = p.scale * kLog2e * 0x1p-14f / kKeyUnit * __int_as_float(biased << 23);
-            float part[NG];  // the quad's shares of the groups' sums, of what the products see
-#pragma unroll
-            for (int u = 0; u < NG; ++u) {
-                part[u] = 0.0f;
-                uint32_t high[4], low[4];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[u][e] *= down;
-                // elements in the order of the codes in a word's halves: 4 bits (0,4) (1,5) (2,6) (3,7), the odd ones 16 times too
-                // large there; 8 bits (0,1) (2,3) (4,5) (6,7)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float by = KB == 4 && (j & 1) ? 0.0625f : 1.0f;
-                    const float a = x[u][KB == 4 ? j : 2 * j] * by, c = x[u][KB == 4 ? j + 4 : 2 * j + 1] * by;
-                    const uint32_t h = pack_half(a, c);
-                    const float2 got = unpack_half(h);
-                    high[j] = h;
-                    part[u] += (got.x + got.y) / by;
-                    if constexpr (kF32) {
-                        low[j] = pack_half(a - got.x, c - got.y);
-                    }
-                }
-                // the query as the second operand of S = K q, both steps of a group (every warp of the CTA writes the same)
-                queries[(nt * NG + u) * 32 + lane] = make_uint4(high[0], high[1], high[2], high[3]);
-                if constexpr (kF32) queries[(NG + u) * 32 + lane] = make_uint4(low[0], low[1], low[2], low[3]);
-            }
+            for (int e = 0; e < 2; ++e) w.f[nt][e] = plain ? q.columns[col_of(nt, 2 * tig + e)].f : 1.0f;
             if constexpr (!kF32) {
-                float sum[NG];
+                // places 2 tig and 2 tig + 1 of every eight: two neighbouring groups, one of their three parts
+                constexpr int kPairs = kSG / 2;
+                uint32_t parts[3];
+                float s[2] = {q.sum[nt][gid][tig % kPairs * 2], q.sum[nt][gid][tig % kPairs * 2 + 1]};
 #pragma unroll
-                for (int u = 0; u < NG; ++u) {
-                    sum[u] = part[u];
-                    sum[u] += __shfl_xor_sync(~0u, sum[u], 1);
-                    sum[u] += __shfl_xor_sync(~0u, sum[u], 2);
-                    sum[u] *= -static_cast<float>(kKOff) * kKeyUnit;
+                for (int i = 0; i < 3; ++i) {
+                    const __nv_bfloat162 both = __floats2bfloat162_rn(s[0], s[1]);
+                    parts[i] = *reinterpret_cast<const uint32_t*>(&both);
+                    s[0] -= __uint_as_float(parts[i] << 16), s[1] -= __uint_as_float(parts[i] & 0xffff0000u);
                 }
 #pragma unroll
                 for (int i = 0; i < kOffs; ++i) {
-                    float x[2] = {0.0f, 0.0f};
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int k = 2 * tig + e + 8 * i, which = k / kSG;
-#pragma unroll
-                        for (int u = 0; u < NG; ++u) {
-                            const float high = __bfloat162float(__float2bfloat16_rn(sum[u]));
-                            const float middle = __bfloat162float(__float2bfloat16_rn(sum[u] - high));
-                            if (k % kSG == u) x[e] = which == 0 ? high : which == 1 ? middle : which == 2 ? sum[u] - high - middle : 0.0f;
-                        }
-                    }
-                    const __nv_bfloat162 both = __floats2bfloat162_rn(x[0], x[1]);
-                    w.off[nt][i] = *reinterpret_cast<const uint32_t*>(&both);
+                    const int which = (tig + 4 * i) / kPairs;
+                    w.off[nt][i] = which == 0 ? parts[0] : which == 1 ? parts[1] : which == 2 ? parts[2] : 0u;
                 }
             }
-            const float shown = p.softcap == 0.0f && p.slopes == nullptr ? f : 1.0f;
-            w.f[nt][0] = __shfl_sync(~0u, shown, 8 * tig);  // from the lanes that loaded columns 2 tig and 2 tig + 1
-            w.f[nt][1] = __shfl_sync(~0u, shown, 8 * tig + 4);
-            // (every warp of the CTA writes the same)
-            const bool is = col < used;
-            const int i = col / p.R, place = n - p.m + i;
-            const Column mine{is && p.window > 0 ? max(place + 1 - p.window, 0) : 0, is ? place + 1 : 0,
-                              is && p.slopes != nullptr ? p.slopes[g * p.R + col - i * p.R] * kLog2e : 0.0f, f};
-            if (tig == 0) columns[col_of(nt, gid)] = mine;
-            if (is) w.all_lim = min(w.all_lim, mine.lim), w.all_lo = max(w.all_lo, mine.lo);
         }
-#pragma unroll
-        for (int d = 4; d <= 16; d <<= 1) {
-            w.all_lim = min(w.all_lim, __shfl_xor_sync(~0u, w.all_lim, d));
-            w.all_lo = max(w.all_lo, __shfl_xor_sync(~0u, w.all_lo, d));
-        }
-        __syncwarp();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -502,7 +508,7 @@ struct Attend {
     }
 
     // The tokens of a stage, t0 the first.
-    __device__ static __forceinline__ void fold(const AttendParams& p, const Lane& l, Warp& w, const uint4* queries, const Column* columns, uint32_t stage, int t0, uint32_t there) {
+    __device__ static __forceinline__ void fold(const AttendParams& p, const Lane& l, Warp& w, const Prepared& prepared, uint32_t stage, int t0, uint32_t there) {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         const uint32_t ks = stage + kKBytes + kVBytes, vs = ks + kSBytes;
         constexpr int kKPiece = NG * KB;   // bytes of a row that a lane reads
@@ -538,7 +544,7 @@ struct Attend {
             for (int u = 0; u < NG; ++u) {
                 uint4 q[NT];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) q[nt] = queries[(nt * NG + u) * 32 + lane];
+                for (int nt = 0; nt < NT; ++nt) q[nt] = prepared.queries[(nt * NG + u) * 32 + lane];
 #pragma unroll
                 for (int h = 0; h < MT; ++h) {
                     uint32_t a[2][4];
@@ -574,7 +580,7 @@ struct Attend {
             for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float f = columns[col_of(nt, 2 * tig + (e & 1))].f;
+                    const float f = prepared.columns[col_of(nt, 2 * tig + (e & 1))].f;
 #pragma unroll
                     for (int h = 0; h < MT; ++h) s[h][nt][e] *= f;
                 }
@@ -592,7 +598,7 @@ struct Attend {
                 for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const Column c = columns[col_of(nt, 2 * tig + (e & 1))];
+                        const Column c = prepared.columns[col_of(nt, 2 * tig + (e & 1))];
 #pragma unroll
                         for (int h = 0; h < MT; ++h) s[h][nt][e] -= c.slope * static_cast<float>(c.lim - 1 - (t0 + h * 16 + (e >> 1) * 8 + gid));
                     }
@@ -627,7 +633,7 @@ struct Attend {
             for (int nt = 0; nt < NS; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const Column c = columns[col_of(nt, 2 * tig + (e & 1))];
+                    const Column c = prepared.columns[col_of(nt, 2 * tig + (e & 1))];
 #pragma unroll
                     for (int h = 0; h < MT; ++h) {
                         const int r = h * 16 + (e >> 1) * 8 + gid, t = t0 + r;
@@ -906,7 +912,7 @@ struct Attend {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int col = col_of(nt, 2 * tig + e) - c0;
-                const float sum = w.sum[nt][e], by = sum == 0.0f ? 0.0f : (kF32 ? 0x1p-6f : 0x1p-3f) / kValueUnit / sum;
+                const float sum = w.sum[nt][e], by = sum == 0.0f ? 0.0f : __frcp_rn(sum) * ((kF32 ? 0x1p-6f : 0x1p-3f) / kValueUnit);
 #pragma unroll
                 for (int u = 0; u < NG; ++u) {
                     float x[4];
@@ -955,8 +961,8 @@ __device__ __forceinline__ int tiles_of(const AttendParams& p, int b) {  // at l
 
 // How the tiles of all (sequence, head, column tile) pairs, laid end to end, are cut into pieces of the same cost.  A pair costs what kPairCost tiles do on
 // top of its tiles: the units before its first tile are nobody's work, but count.  (Without them a CTA whose sequences are short had several times
-// the work of one whose sequences are long: 359 -> 307 us for 64 sequences of 512 .. 8192 tokens.)
-constexpr uint32_t kPairCost = 12;
+// the work of one whose sequences are long: 359 -> 286 us for 64 sequences of 512 .. 8192 tokens.)
+constexpr uint32_t kPairCost = 24;
 struct Cut {
     uint32_t total, each, more;  // units; of a piece (the first `more` have one more)
     __device__ __forceinline__ Cut(uint32_t units, uint32_t pieces) : total(units), each(units / pieces), more(units - units / pieces * pieces) {}
@@ -1056,13 +1062,13 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
     extern __shared__ __align__(128) uint8_t smem[];
     float* const ml = reinterpret_cast<float*>(smem + A::kRing);
     uint32_t* const left_at = reinterpret_cast<uint32_t*>(smem + A::kRing + A::kMl);
-    __shared__ typename A::Column columns[A::kCols];
-    uint4* const queries = reinterpret_cast<uint4*>(smem + A::kRing + A::kMl + 16 * ((W * 4 + 15) / 16));
+    auto& prepared = *reinterpret_cast<typename A::Prepared*>(smem + A::kRing + A::kMl + 16 * ((W * 4 + 15) / 16));
     __shared__ Place<kTok> now[W], ahead[W];
     __shared__ uint32_t there[W][S];  // which tokens of a stage are there
     __shared__ int pieces[3];
     const int warp = threadIdx.x >> 5;
     const uint32_t ring = smem_u32(smem) + warp * S * A::kStage;
+    if (p.cluster > 0) grid_launch_dependents();  // (a launch of long runs fills the SMs to its end)
     grid_dependency_wait();
 
     // This CTA's run of tiles, and which of a pair's tokens are this warp's: kTok from `skip` on, `step` further on the next ones.
@@ -1139,12 +1145,12 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
     for (;;) {
         int t = now[warp].first + now[warp].tile * kTok + skip;
         const int end = now[warp].first + now[warp].end * kTok;
-        A::begin(p, q, raw, queries, columns, now[warp].g, now[warp].ct, now[warp].n);
+        A::begin(p, q, raw, prepared, now[warp].g, now[warp].ct, now[warp].n);
         for (; t < end; t += step) {
             copy_wait<S - 2>();
             __syncwarp();
             copy(slot == 0 ? S - 1 : slot - 1);
-            A::fold(p, l, q, queries, columns, ring + slot * A::kStage, t, there[warp][slot]);
+            A::fold(p, l, q, prepared, ring + slot * A::kStage, t, there[warp][slot]);
             slot = slot == S - 1 ? 0 : slot + 1;
         }
         if (p.cluster > 1) {
@@ -1209,7 +1215,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
             constexpr int kRoom = (S - 1) * A::kStage / 16;  // quads in a warp's ring
             static_assert(A::kCols * D / 4 <= W * kRoom && 8 * A::kCols * 4 <= NG * NT * 512, "");
             const auto where = [](int quad) { return static_cast<uint32_t>(quad / kRoom * (S * A::kStage) + A::kStage + quad % kRoom * 16); };
-            const uint32_t their_lse = smem_u32(queries);
+            const uint32_t their_lse = smem_u32(prepared.queries);
             const int rank = static_cast<int>(cluster_rank()), each = (A::kCols * D / 4 + p.cluster - 1) / p.cluster;
             cluster_wait();
 #pragma unroll
@@ -1223,7 +1229,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
                 }
             }
             cluster_sync();
-            const float* const lse = reinterpret_cast<const float*>(queries);
+            const float* const lse = reinterpret_cast<const float*>(prepared.queries);
             for (int i = threadIdx.x; i * p.cluster + rank < used * (D / 4); i += kThreads) {
                 const int quad = i * p.cluster + rank, col = quad / (D / 4), d = (quad - col * (D / 4)) * 4;
                 float top = kNegInf, total = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
