@@ -269,14 +269,13 @@ def linear_options(group_x_rows: int, x_rows: int, flags: int):
     return _structure(LinearOptions, _LINEAR_OPTIONS.pack(group_x_rows, x_rows, flags))
 
 
-def qcache(*fields):
-    """``b2kv_qcache`` for ``lib``; the fields in order, pointers as integers (0: none)."""
-    return _structure(QCache, _QCACHE.pack(*fields))
+def _packer(cls, packed: struct.Struct):
+    """The structure for ``lib`` from its fields in order, pointers as integers (0: none)."""
+    return packed.pack if calls is not None else lambda *fields: ctypes.byref(cls.from_buffer_copy(packed.pack(*fields)))
 
 
-def qcache_attend_args(*fields):
-    """``b2kv_qcache_attend_args`` for ``lib``, likewise."""
-    return _structure(QCacheAttendArgs, _QCACHE_ATTEND_ARGS.pack(*fields))
+qcache = _packer(QCache, _QCACHE)
+qcache_attend_args = _packer(QCacheAttendArgs, _QCACHE_ATTEND_ARGS)
 
 
 def check(status: int) -> None:

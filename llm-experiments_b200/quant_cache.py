@@ -86,25 +86,33 @@ def quant_cache_set_lengths(cache: QuantKVCache, lens) -> None:
 
 
 def _layer(cache: QuantKVCache, layer_idx: int):
-    if layer_idx < 0 or layer_idx >= len(cache.layers):
-        raise ValueError(f"layer_idx {layer_idx} out of range [0, {len(cache.layers)})")
-    layer = cache.layers[layer_idx]
+    """``b2kv_qcache`` of a layer.  (Asking a tensor for its address costs 0.2 us, a step of a decoding loop would ask four for each call.)"""
+    layers = cache.layers
+    if layer_idx < 0 or layer_idx >= len(layers):
+        raise ValueError(f"layer_idx {layer_idx} out of range [0, {len(layers)})")
+    layer = layers[layer_idx]
+    kc, vc, ks, vs, kept = layer.k_codes.buffer, layer.v_codes.buffer, layer.k_scales.buffer, layer.v_scales.buffer, layer.pointers
+    if kept is None or kept[0] is not kc or kept[1] is not vc or kept[2] is not ks or kept[3] is not vs:
+        kept = layer.pointers = (kc, vc, ks, vs, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr())
     table, lens = cache.block_table, cache.seq_lens
     return _native.qcache(
-        layer.k_codes.buffer.data_ptr(), layer.v_codes.buffer.data_ptr(), layer.k_scales.buffer.data_ptr(), layer.v_scales.buffer.data_ptr(),
-        0 if table is None else table.data_ptr(), 0 if lens is None else lens.data_ptr(), cache.current_len, cache.batch_size, cache.n_kv_heads,
-        cache.head_dim, cache.max_seq_len, 0 if table is None else table.shape[1], cache.block_size, cache.n_blocks, cache.k_bits, cache.v_bits,
-        dtype_code(cache.dtype))
+        kept[4], kept[5], kept[6], kept[7], 0 if table is None else table.data_ptr(), 0 if lens is None else lens.data_ptr(), cache.current_len,
+        cache.batch_size, cache.n_kv_heads, cache.head_dim, cache.max_seq_len, 0 if table is None else table.shape[1], cache.block_size,
+        cache.n_blocks, cache.k_bits, cache.v_bits, dtype_code(cache.dtype))
 
 
 def _rows(buffer: GPUBuffer2D, shape, dtype: torch.dtype, name: str) -> int:
     """Checks a buffer of rows; its row pitch."""
-    validate_buffer_shape_2d(buffer, shape, name)
-    if buffer.buffer.dtype != dtype:
+    t = buffer.buffer
+    if buffer.shape != shape:
+        validate_buffer_shape_2d(buffer, shape, name)
+    if t.dtype != dtype:
         raise ValueError(f"{name} dtype must match the cache dtype {dtype}")
-    if buffer.buffer.dim() != 2 or buffer.buffer.stride(1) != 1:
+    if t.is_contiguous():
+        return shape[1]
+    if t.dim() != 2 or t.stride(1) != 1:
         raise ValueError(f"the elements of a row of {name} must lie next to one another")
-    return buffer.buffer.stride(0)
+    return t.stride(0)
 
 
 @reference_op("quant_cache_update")
@@ -158,20 +166,20 @@ def attention_with_quant_cache(ctx: GPUContext, cache: QuantKVCache, layer_idx: 
     described = _layer(cache, layer_idx)
     if not 1 <= tokens <= MAX_TOKENS:
         raise ValueError(f"tokens must lie in [1, {MAX_TOKENS}], got {tokens}")
-    if pending < 0 or cache.current_len + pending > cache.max_seq_len:
-        raise ValueError(f"pending must lie in [0, {cache.max_seq_len - cache.current_len}], got {pending}")
     held = cache.current_len + pending
+    if pending < 0 or held > cache.max_seq_len:
+        raise ValueError(f"pending must lie in [0, {cache.max_seq_len - cache.current_len}], got {pending}")
     if held == 0 and cache.seq_lens is None:  # (with lengths of their own, sequences may be empty)
         raise ValueError("Cache is empty: current_len=0")
     if window < 0:
         raise ValueError(f"window must be >= 0, got {window}")
     if not (math.isfinite(softcap) and softcap >= 0) or (scale is not None and not math.isfinite(scale)):
         raise ValueError(f"softcap must be finite and >= 0 and scale finite, got {softcap} and {scale}")
-    D = cache.head_dim
-    heads = q_new.shape[1] // D
-    if heads * D != q_new.shape[1] or heads == 0 or heads % cache.n_kv_heads != 0:
-        raise ValueError(f"q_new has {q_new.shape[1]} columns, not a multiple of {cache.n_kv_heads} heads of {D}")
-    shape = (cache.batch_size * tokens, heads * D)
+    D, columns = cache.head_dim, q_new.shape[1]
+    heads = columns // D
+    if heads * D != columns or heads == 0 or heads % cache.n_kv_heads != 0:
+        raise ValueError(f"q_new has {columns} columns, not a multiple of {cache.n_kv_heads} heads of {D}")
+    shape = (cache.batch_size * tokens, columns)
     ld_q, ld_out = _rows(q_new, shape, cache.dtype, "q_new"), _rows(output, shape, cache.dtype, "output")
     if slopes is not None:
         validate_buffer_shape_1d(slopes, heads, "slopes")
@@ -179,8 +187,10 @@ def attention_with_quant_cache(ctx: GPUContext, cache: QuantKVCache, layer_idx: 
             raise ValueError("slopes must be contiguous float32")
     args = _native.qcache_attend_args(q_new.buffer.data_ptr(), output.buffer.data_ptr(), 0 if slopes is None else slopes.buffer.data_ptr(),
                                       ld_q, ld_out, heads, tokens, held, pending, window, D ** -0.5 if scale is None else scale, softcap)
-    stream = batch_op_begin(ctx)
-    nbytes = _native.lib.b2kv_qcache_attend_workspace_bytes(described, args)
+    stream, lib = batch_op_begin(ctx), _native.lib
+    nbytes = lib.b2kv_qcache_attend_workspace_bytes(described, args)
     # Scratch of this call alone, from the stream's (or the capture's) own memory: nothing is shared by calls that run at the same time.
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q_new.buffer.device) if nbytes else None
-    _native.check(_native.lib.b2kv_qcache_attend(described, args, None if ws is None else ws.data_ptr(), nbytes, dev_status_ptr(ctx), stream))
+    rc = lib.b2kv_qcache_attend(described, args, None if ws is None else ws.data_ptr(), nbytes, dev_status_ptr(ctx), stream)
+    if rc != 0:
+        _native.check(rc)
