@@ -38,19 +38,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Quotients by a divisor that the host knows, of numbers below 2^31: m / 2^(31 + l) is above 1 / d by less than 2^-31 / d.
-struct Divisor {
-    uint32_t d, m;
-    int shift;
-    explicit Divisor(uint32_t by) : d(by) {
-        int l = 0;
-        while ((1ull << l) < by) ++l;
-        shift = 31 + l;
-        m = static_cast<uint32_t>(((1ull << shift) + by - 1) / by);
-    }
-    __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> shift); }
-};
-
 // Eight elements as they lie in memory.
 template <typename T>
 struct Octet {
@@ -196,7 +183,7 @@ __device__ __forceinline__ void write_row(const b2kv_qcache& c, const T* src, in
 // Thread = (row of a head, octet); grid.y 0 keys, 1 values.
 template <typename T, int NG, int KB, int VB>
 __global__ void __launch_bounds__(kThreads) write_kernel(const b2kv_qcache c, const T* k, int64_t ld_k, const T* v, int64_t ld_v, int n, Divisor by_heads,
-                                                         Divisor by_rows, uint32_t rows, int32_t* dev_status) {
+                                                         Divisor by_rows, Divisor by_block, uint32_t rows, int32_t* dev_status) {
     grid_launch_dependents();
     grid_dependency_wait();
     const uint32_t at = blockIdx.x * (kThreads / 4) + threadIdx.x / 4, o = threadIdx.x & 3;
@@ -207,7 +194,7 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const b2kv_qcache c, co
     if (place < 0 || place >= c.T_max)
         report_status(dev_status, B2KV_DEV_BAD_POSITION);
     else
-        row = row_of(c, b, g, static_cast<int>(place), dev_status);
+        row = row_of(c, by_block, b, g, static_cast<int>(place), dev_status);
     if (at >= rows) row = -1;
     if (blockIdx.y == 0)
         write_row<T, NG, KB, false>(c, k + src * ld_k + static_cast<int64_t>(g) * (NG * kGroup), o, row);
@@ -218,7 +205,7 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const b2kv_qcache c, co
 // Thread = (row of a head of the output, octet).
 template <typename T, int NG, int BITS, bool kValues>
 __global__ void __launch_bounds__(kThreads) read_kernel(const b2kv_qcache c, T* out, int n, int last, int len_bias, Divisor by_heads, Divisor by_rows,
-                                                        uint32_t rows, int32_t* dev_status) {
+                                                        Divisor by_block, uint32_t rows, int32_t* dev_status) {
     grid_launch_dependents();
     grid_dependency_wait();
     const uint32_t i = blockIdx.x * (kThreads / 4) + threadIdx.x / 4, o = threadIdx.x & 3;
@@ -226,7 +213,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const b2kv_qcache c, T* 
     const uint32_t dst = by_heads.quotient(i), g = i - dst * by_heads.d, b = by_rows.quotient(dst);
     const int64_t held = min(static_cast<int64_t>(tokens_held(c, b)) + len_bias, static_cast<int64_t>(c.T_max));
     const int64_t place = static_cast<int64_t>(dst - b * by_rows.d) + (last ? held - n : 0);
-    const int64_t row = place >= 0 && place < held ? row_of(c, b, g, static_cast<int>(place), dev_status) : -1;
+    const int64_t row = place >= 0 && place < held ? row_of(c, by_block, b, g, static_cast<int>(place), dev_status) : -1;
     Codes<NG, BITS> codes;
     uint32_t scales[scale_row(NG) / 2] = {};
     if (row >= 0) {
@@ -258,7 +245,7 @@ int launch_write(const b2kv_qcache& c, const void* k, int64_t ld_k, const void* 
     if (rows > 0x7fffffff) return B2KV_ERR_UNSUPPORTED;
     OverlapLaunch launch(dim3(static_cast<unsigned>((rows + kThreads / 4 - 1) / (kThreads / 4)), 2), kThreads, 0, stream);
     B2KV_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, write_kernel<T, NG, KB, VB>, c, static_cast<const T*>(k), ld_k, static_cast<const T*>(v), ld_v, n,
-                                     Divisor(c.G), Divisor(n), static_cast<uint32_t>(rows), dev_status));
+                                     Divisor(c.G), Divisor(n), by_block(c), static_cast<uint32_t>(rows), dev_status));
     return B2KV_OK;
 }
 
@@ -268,7 +255,7 @@ int launch_read(const b2kv_qcache& c, void* out, int n, int last, int len_bias, 
     if (rows > 0x7fffffff) return B2KV_ERR_UNSUPPORTED;
     OverlapLaunch launch(static_cast<unsigned>((rows + kThreads / 4 - 1) / (kThreads / 4)), kThreads, 0, stream);
     B2KV_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, read_kernel<T, NG, BITS, kValues>, c, static_cast<T*>(out), n, last, len_bias, Divisor(c.G), Divisor(n),
-                                     static_cast<uint32_t>(rows), dev_status));
+                                     by_block(c), static_cast<uint32_t>(rows), dev_status));
     return B2KV_OK;
 }
 

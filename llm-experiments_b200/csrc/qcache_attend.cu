@@ -94,6 +94,7 @@ int b2kv_qcache_attend(const b2kv_qcache* cache, const b2kv_qcache_attend_args* 
     }
     AttendParams p{};
     p.c = c;
+    p.by_block = by_block(c);
     p.q = a.q, p.out = a.out, p.slopes = a.slopes, p.dev_status = dev_status;
     p.ld_q = a.ld_q, p.ld_out = a.ld_out;
     p.R = a.H / c.G, p.m = a.m, p.col_tiles = plan.col_tiles, p.T_upper = a.T_upper, p.len_bias = a.len_bias, p.window = a.window;

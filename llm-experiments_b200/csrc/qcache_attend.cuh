@@ -38,6 +38,7 @@ namespace qcache {
 
 struct AttendParams {
     b2kv_qcache c;
+    Divisor by_block;
     const void* q;
     void* out;
     const float* slopes;
@@ -401,7 +402,7 @@ struct Attend {
     // Where a lane's token of a tile lies: its row, -1 where there is none or no query sees it.
     __device__ static __forceinline__ int64_t find(const AttendParams& p, int b, int g, int t0, int seen, int n) {
         const int lane = lane_id(), t = t0 + (lane & (kTok - 1));
-        return t < n && t >= seen ? row_of(p.c, b, g, t, p.dev_status) : -1;
+        return t < n && t >= seen ? row_of(p.c, p.by_block, b, g, t, p.dev_status) : -1;
     }
 
     // Starts the copies of a tile whose rows `find` gave (zeros where there is none); a bit for each token that is there.
@@ -414,9 +415,28 @@ struct Attend {
             copy_small<kSRow>(ks + lane * kSRow, static_cast<const uint8_t*>(p.c.k_scales) + at * kSRow, row >= 0);
             copy_small<kSRow>(ks + kSBytes + lane * kSRow, static_cast<const uint8_t*>(p.c.v_scales) + at * kSRow, row >= 0);
         }
-        pieces_paged<kKRow>(stage + l.put_k, static_cast<const uint8_t*>(p.c.k_codes), at, there, [](int) { return 0u; });
-        pieces_paged<kVRow>(stage + l.put_v, static_cast<const uint8_t*>(p.c.v_codes), at, there, moved_v);
+        const uint8_t* const k = static_cast<const uint8_t*>(p.c.k_codes);
+        const uint8_t* const v = static_cast<const uint8_t*>(p.c.v_codes);
+        if (there == ~0u && p.c.block_size % 16 == 0) {  // tiles begin at multiples of 16: every 16 tokens lie one behind the other
+            const int64_t first = __shfl_sync(~0u, at, 0), second = kTok == 32 ? __shfl_sync(~0u, at, 16) - 16 : first;
+            pieces_halves<kKRow>(stage + l.put_k, k + first * kKRow, k + second * kKRow, [](int) { return 0u; });
+            pieces_halves<kVRow>(stage + l.put_v, v + first * kVRow, v + second * kVRow, moved_v);
+        } else {
+            pieces_paged<kKRow>(stage + l.put_k, k, at, there, [](int) { return 0u; });
+            pieces_paged<kVRow>(stage + l.put_v, v, at, there, moved_v);
+        }
         return there;
+    }
+    // first, second: where row 0 would lie for the first 16 rows and for the others
+    template <int ROW, typename F>
+    __device__ static __forceinline__ void pieces_halves(uint32_t dst, const uint8_t* first, const uint8_t* second, F&& moved) {
+        constexpr int kCh = ROW / 16, kPieces = kCh * kTok, kPer = (kPieces + 31) / 32, kHalf = kCh * 16;
+        const int lane = lane_id();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const bool front = i * 32 + 31 < kHalf || (i * 32 < kHalf && i * 32 + lane < kHalf);
+            if (kPieces % 32 == 0 || i * 32 + lane < kPieces) copy16((dst ^ moved(i)) + i * 512, (front ? first : second) + (i * 32 + lane) * 16);
+        }
     }
     template <int ROW, typename F>
     __device__ static __forceinline__ void pieces_paged(uint32_t dst, const uint8_t* src, int64_t mine, uint32_t there, F&& moved) {
@@ -1113,7 +1133,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
         copy_end = at.first + at.end * kTok;
         held = at.n;
         seen = first_seen(p, held);
-        if (!paged) row = row_of(p.c, at.b, at.g, 0, nullptr);
+        if (!paged) row = row_of(p.c, p.by_block, at.b, at.g, 0, nullptr);
     };
     const auto look = [&] {
         while (copy_t >= copy_end) {
