@@ -172,7 +172,9 @@ struct Words {
 // The first token that any query of a sequence of n tokens sees.
 __device__ __forceinline__ int first_seen(const AttendParams& p, int n) { return p.window > 0 ? max(n - p.m + 1 - p.window, 0) : 0; }
 
-// What a warp's ring holds: stages of 16 or 32 tokens, as many as fit with two CTAs per SM.
+// What a warp's ring holds with two CTAs per SM: at least two stages, one in the arithmetic and one on its way, of 32 tokens where that many fit, else 16.
+// What a stage costs beside its products (copies, masks, references, the scales' exponents) is a quarter of 32 tokens' time, so two long stages beat
+// four short ones (8 and 4 bits, heads of 128, the benchmark's batch: 286 against 340 us); 64 tokens run out of registers (4 bits: 292 against 276 us).
 template <int NG, int KB, int VB, int NT>
 struct Ring {
     static constexpr int kWarps = NT == 1 && NG <= 4 ? 6 : 4;  // of 168 or 255 registers per thread
@@ -180,10 +182,10 @@ struct Ring {
     static constexpr int kToken = NG * 4 * (KB + VB) + 4 * scale_row(NG);
     // Half of what an SM has for two CTAs, less the queries, what is kept per column, and 1 KB of small things.
     static constexpr int kRoom = (113 * 1024 - 1024 - NG * NT * 512 - NT * (640 + kWarps * 64) - 64) / kWarps;
-    static constexpr int kTokens = 3 * 32 * kToken <= kRoom ? 32 : 16;
+    static constexpr int kTokens = 2 * 32 * kToken <= kRoom ? 32 : 16;
     static constexpr int kFit = kRoom / (kTokens * kToken);
-    static constexpr int kStages = kFit > 6 ? 6 : kFit;
-    static_assert(kStages >= 3, "");
+    static constexpr int kStages = kFit > 4 ? 4 : kFit;
+    static_assert(kStages >= 2, "");
 };
 
 // T: type of queries and outputs; NG groups of 32 elements; KB, VB bits; NT tiles of 8 columns (fp32: 2, the second for what fp16 leaves
