@@ -36,7 +36,7 @@ bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& pla
     // Columns (new token, query head) of a key / value head that are taken together: 16 share the widening of the codes (4 sequences of 131072
     // tokens, 16 heads to one: 198 against 242 us), 8 make more pairs where there are few tokens to a CTA (40 columns over 2048 tokens: 22.1 against 25.5 us).
     const bool wide = c.dtype != B2KV_DTYPE_F32 && columns > 8 && heads * ((columns + 15) / 16) * most >= at_once * 1024ll;
-    plan.cols = wide ? 16 : 8;
+    plan.cols = c.dtype == B2KV_DTYPE_F32 ? 4 : wide ? 16 : 8;
     plan.col_tiles = (columns + plan.cols - 1) / plan.cols;
     plan.pairs = heads * plan.col_tiles;
     if (plan.pairs > 0x7fffffff) return false;

@@ -20,7 +20,7 @@
 //   * A probability is rounded to fp16, multiplied by its value scale there and rounded again (11 bits; the output has 8).  To keep that in range
 //     whatever the scales are, they are taken relative to the largest exponent so far, and the accumulators are rescaled when that
 //     grows: products stay below 2^15, and scales down to 2^-17 of the largest keep all their bits.
-//   * fp32 queries and weights are sums of two fp16 numbers (22 bits), in columns of their own; keys are centred like values; and only 16 tokens'
+//   * fp32 queries and weights are sums of two fp16 numbers (22 bits), in columns of their own (four pairs of them to a tile of eight); keys are centred like values; and only 16 tokens'
 //     products are added up in the tensor core, whose sums are cut off and not rounded.
 //   * Softmax: scores in the log2 domain, references that move only when a score has outgrown its own by more than 2^8 (one vote per stage), sums per
 //     lane until the end, all in fp32.
@@ -70,24 +70,24 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // d = the product alone
 __device__ __forceinline__ void mma_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ uint32_t half_sub(uint32_t a, uint32_t b) {
@@ -188,15 +188,14 @@ struct Ring {
     static_assert(kStages >= 2, "");
 };
 
-// T: type of queries and outputs; NG groups of 32 elements; KB, VB bits; NT tiles of 8 columns (fp32: 2, the second for what fp16 leaves
-// of the first).
+// T: type of queries and outputs; NG groups of 32 elements; KB, VB bits; NT tiles of 8 columns (fp32: one, of 4 columns and of what fp16 leaves of each).
 template <typename T, int NG, int KB, int VB, int NT>
 struct Attend {
     using R = Ring<NG, KB, VB, NT>;
     static constexpr int WARPS = R::kWarps, STAGES = R::kStages, kTok = R::kTokens, MT = kTok / 16;
     static constexpr bool kF32 = std::is_same<T, float>::value;
-    static_assert(!kF32 || NT == 2, "");
-    static constexpr int D = NG * kGroup, kCols = kF32 ? 8 : 8 * NT, kThreads = WARPS * 32;
+    static_assert(!kF32 || NT == 1, "");
+    static constexpr int D = NG * kGroup, kCols = kF32 ? 4 : 8 * NT, kThreads = WARPS * 32;
     static constexpr int kKRow = D * KB / 8, kVRow = D * VB / 8, kSRow = scale_row(NG) * 2;
     static constexpr int kKBytes = kTok * kKRow, kVBytes = kTok * kVRow, kSBytes = kTok * kSRow;
     static constexpr int kStage = (kKBytes + kVBytes + 2 * kSBytes + 15) / 16 * 16;
@@ -269,11 +268,11 @@ struct Attend {
         bool fresh;                // some column may not have seen anything yet
     };
 
-    // fp32: both tiles are the same columns.
-    __device__ static __forceinline__ int col_of(int nt, int c) { return kF32 ? c : nt * 8 + c; }
+    // fp32: the second half of a tile is for the same columns as the first, and lanes 2 apart (in tig) have the same scores.
+    __device__ static __forceinline__ int col_of(int nt, int c) { return kF32 ? c & 3 : nt * 8 + c; }
 
     // The queries of a pair are prepared by the CTA's warps together: unit i, group i % NG of the columns of tile i / NG, is warp i % WARPS's.
-    static constexpr int kUnits = (kF32 ? 1 : NT) * NG, kUnitsEach = (kUnits + WARPS - 1) / WARPS;
+    static constexpr int kUnits = NT * NG, kUnitsEach = (kUnits + WARPS - 1) / WARPS;
     struct Prepared {
         uint32_t most[kUnits / NG][8][NG];  // largest magnitude of a column's group, as a whole number (NaN above infinity above all others)
         float sum[kUnits / NG][8][kSG];     // what the centre of its keys comes to
@@ -328,7 +327,7 @@ struct Attend {
             const int unit = warp + i * WARPS, nt = unit / NG, u = unit - nt * NG;
             if (kUnits % WARPS != 0 && unit >= kUnits) break;  // (a warp's lanes all the same)
             const float down = __int_as_float((254 + 14 - exponent(nt, gid)) << 23);
-            uint32_t high[4], low[4];
+            uint32_t high[4], low[4] = {};
             float sum = 0.0f;  // of what the products see
             // elements in the order of the codes in a word's halves: 4 bits (0,4) (1,5) (2,6) (3,7), the odd ones 16 times too
             // large there; 8 bits (0,1) (2,3) (4,5) (6,7)
@@ -341,8 +340,9 @@ struct Attend {
                 sum += (got.x + got.y) * (1.0f / by);
                 if constexpr (kF32) low[j] = pack_half(a - got.x, c - got.y);
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) high[j] = kF32 && gid >= 4 ? low[j] : high[j];
             q.queries[unit * 32 + lane] = make_uint4(high[0], high[1], high[2], high[3]);
-            if constexpr (kF32) q.queries[(NG + u) * 32 + lane] = make_uint4(low[0], low[1], low[2], low[3]);
             sum += __shfl_xor_sync(~0u, sum, 1);
             sum += __shfl_xor_sync(~0u, sum, 2);
             if (tig == 0) {
@@ -367,7 +367,7 @@ struct Attend {
         w.all_lo = __reduce_max_sync(~0u, is ? c.lo : 0);
         const bool plain = p.softcap == 0.0f && p.slopes == nullptr;
 #pragma unroll
-        for (int nt = 0; nt < (kF32 ? 1 : NT); ++nt) {
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) w.f[nt][e] = plain ? q.columns[col_of(nt, 2 * tig + e)].f : 1.0f;
             if constexpr (!kF32) {
@@ -534,8 +534,7 @@ struct Attend {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         const uint32_t ks = stage + kKBytes + kVBytes, vs = ks + kSBytes;
         constexpr int kKPiece = NG * KB;   // bytes of a row that a lane reads
-        constexpr int NS = kF32 ? 1 : NT;  // tiles of scores
-        float s[MT][NS][4];
+        float s[MT][NT][4];
         {
             Words<kKPiece> k[MT][2];
             Words<kSRow> scales[MT][2];
@@ -593,13 +592,13 @@ struct Attend {
 #pragma unroll
             for (int h = 0; h < MT; ++h)
 #pragma unroll
-                for (int nt = 0; nt < NS; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[h][nt][e] = kF32 ? acc[h][0][e] + acc[h][NT - 1][e] : acc[h][nt][e];
+                    for (int e = 0; e < 4; ++e) s[h][nt][e] = kF32 ? acc[h][nt][e] + __shfl_xor_sync(~0u, acc[h][nt][e], 2) : acc[h][nt][e];
         }
         if (p.softcap > 0.0f || p.slopes != nullptr) {
 #pragma unroll
-            for (int nt = 0; nt < NS; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float f = prepared.columns[col_of(nt, 2 * tig + (e & 1))].f;
@@ -611,13 +610,13 @@ struct Attend {
 #pragma unroll
                 for (int h = 0; h < MT; ++h)
 #pragma unroll
-                    for (int nt = 0; nt < NS; ++nt)
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[h][nt][e] = tanhf(s[h][nt][e] * down) * up;
             }
             if (p.slopes != nullptr) {
 #pragma unroll
-                for (int nt = 0; nt < NS; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const Column c = prepared.columns[col_of(nt, 2 * tig + (e & 1))];
@@ -633,7 +632,7 @@ struct Attend {
         if (!move) {
             float most = kNegInf;
 #pragma unroll
-            for (int nt = 0; nt < NS; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -646,13 +645,13 @@ struct Attend {
 #pragma unroll
                 for (int h = 0; h < MT; ++h)
 #pragma unroll
-                    for (int nt = 0; nt < NS; ++nt)
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[h][nt][e] += w.ref[nt][e & 1];
             }
         } else {
 #pragma unroll
-            for (int nt = 0; nt < NS; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const Column c = prepared.columns[col_of(nt, 2 * tig + (e & 1))];
@@ -662,7 +661,7 @@ struct Attend {
                         s[h][nt][e] *= w.f[nt][e & 1];
                         if (!((there >> r) & 1u) || t < c.lo || t >= c.lim) {
                             s[h][nt][e] = kNegInf;
-                            hidden |= 1u << ((h * NS + nt) * 4 + e);
+                            hidden |= 1u << ((h * NT + nt) * 4 + e);
                         }
                     }
                 }
@@ -670,7 +669,7 @@ struct Attend {
         }
         if (move) {
 #pragma unroll
-            for (int nt = 0; nt < NS; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     float top = kNegInf;
@@ -683,16 +682,13 @@ struct Attend {
                     w.ref[nt][e] = top;
                     w.sum[nt][e] *= by;
 #pragma unroll
-                    for (int k = 0; k < (kF32 ? 2 : 1); ++k) {
-#pragma unroll
-                        for (int j = 0; j < NG * 2; ++j) w.o[nt + k][j][e] *= by, w.o[nt + k][j][e + 2] *= by;
-                    }
+                    for (int j = 0; j < NG * 2; ++j) w.o[nt][j][e] *= by, w.o[nt][j][e + 2] *= by;
 #pragma unroll
                     for (int h = 0; h < MT; ++h) s[h][nt][e] -= top, s[h][nt][e + 2] -= top;
                 }
         }
 #pragma unroll
-        for (int nt = 0; nt < NS; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -714,9 +710,9 @@ struct Attend {
             for (int u = 0; u < NG; ++u) {
                 const uint32_t y = u & 1 ? mine.w[u >> 1] >> 16 : mine.w[u >> 1] & 0xffffu;
                 const uint32_t bad = __ballot_sync(~0u, y >= 0x7f80u);  // a bit per token
-                if (y >= 0x7f80u) mine.w[u >> 1] &= u & 1 ? 0x0000ffffu : 0xffff0000u;
+                mine.w[u >> 1] &= y < 0x7f80u ? ~0u : u & 1 ? 0x0000ffffu : 0xffff0000u;
 #pragma unroll
-                for (int nt = 0; nt < NS; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         bool spoilt = false;
@@ -724,12 +720,11 @@ struct Attend {
                         for (int h = 0; h < MT; ++h)
 #pragma unroll
                             for (int i = 0; i < 2; ++i)
-                                spoilt = spoilt || (((bad >> (h * 16 + i * 8 + gid)) & 1u) && !((hidden >> ((h * NS + nt) * 4 + i * 2 + e)) & 1u));
+                                spoilt = spoilt || (((bad >> (h * 16 + i * 8 + gid)) & 1u) && !((hidden >> ((h * NT + nt) * 4 + i * 2 + e)) & 1u));
                         const uint32_t lanes = __ballot_sync(~0u, spoilt);
-                        if ((lanes >> tig) & 0x11111111u) {
+                        const float add = ((lanes >> tig) & 0x11111111u) != 0 ? __int_as_float(0x7fc00000) : 0.0f;
 #pragma unroll
-                            for (int j = 2 * u; j < 2 * u + 2; ++j) w.o[nt][j][e] = w.o[nt][j][e + 2] = __int_as_float(0x7fc00000);
-                        }
+                        for (int j = 2 * u; j < 2 * u + 2; ++j) w.o[nt][j][e] += add, w.o[nt][j][e + 2] += add;
                     }
             }
             most = mine.w[0];
@@ -755,10 +750,11 @@ struct Attend {
     }
 
     // O += V^T P for fp32: weights times value scales in 32 bits, then as two fp16 numbers.
-    template <int NS>
-    __device__ static __forceinline__ void values_f32(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NS][4], const Words<kSRow>& mine) {
+    __device__ static __forceinline__ void values_f32(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NT][4], const Words<kSRow>& mine) {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         const float vf = __int_as_float((260 - w.scale_exp) << 23);  // 2^(6 - exponent)
+        // (A number, and no branch on the lane: the compiler may lay such a branch around what follows, and instructions of the whole warp are among it.)
+        const float rest = tig >= 2 ? 1.0f : 0.0f;
         __syncwarp();
         mine.store(stage + kKBytes + kVBytes + kSBytes + (lane & (kTok - 1)) * kSRow);  // (without the groups of NaN)
         __syncwarp();
@@ -778,29 +774,26 @@ struct Attend {
                 const float f0 = vf * __uint_as_float(u & 1 ? s0.w[u >> 1] & 0xffff0000u : s0.w[u >> 1] << 16);
                 const float f1 = vf * __uint_as_float(u & 1 ? s1.w[u >> 1] & 0xffff0000u : s1.w[u >> 1] << 16);
                 float x[4] = {weight[h][0][0] * f0, weight[h][0][1] * f0, weight[h][0][2] * f1, weight[h][0][3] * f1};
-                const uint32_t p0 = pack_half(x[0], x[1]), p1 = pack_half(x[2], x[3]);
-                const float2 g0 = unpack_half(p0), g1 = unpack_half(p1);
-                const uint32_t b[2][2] = {{transpose8x8(p0), transpose8x8(p1)},
-                                          {transpose8x8(pack_half(x[0] - g0.x, x[1] - g0.y)), transpose8x8(pack_half(x[2] - g1.x, x[3] - g1.y))}};
+                // lanes of the second half have what fp16 leaves: less `rest` times the rounded number, and rounded again
+                const float2 g0 = unpack_half(pack_half(x[0], x[1])), g1 = unpack_half(pack_half(x[2], x[3]));
+                const uint32_t b0 = transpose8x8(pack_half(fmaf(-rest, g0.x, x[0]), fmaf(-rest, g0.y, x[1])));
+                const uint32_t b1 = transpose8x8(pack_half(fmaf(-rest, g1.x, x[2]), fmaf(-rest, g1.y, x[3])));
                 uint32_t a[2][4];
                 v_pieces(v, u, a);
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
+                for (int j = 0; j < 2; ++j) {
+                    float d[4];
+                    mma_new(d, a[j][0], a[j][1], a[j][2], a[j][3], b0, b1);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float d[4];
-                        mma_new(d, a[j][0], a[j][1], a[j][2], a[j][3], b[nt][0], b[nt][1]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w.o[nt][2 * u + j][e] += d[e];
-                    }
+                    for (int e = 0; e < 4; ++e) w.o[0][2 * u + j][e] += d[e];
+                }
             }
         }
     }
 
     // O += V^T P for bfloat16: weights go to the operand's layout as fp16 numbers and meet the value scales there, two per instruction.  The scales
     // are made fp16 (relative to the largest exponent) and brought into that order by the lane that has the token, in place.
-    template <int NS>
-    __device__ static __forceinline__ void values_bf16(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NS][4], const Words<kSRow>& mine) {
+    __device__ static __forceinline__ void values_bf16(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NT][4], const Words<kSRow>& mine) {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         constexpr int kWords = kSG / 2;
         const uint32_t vs = stage + kKBytes + kVBytes + kSBytes;
@@ -843,16 +836,16 @@ struct Attend {
             Words<NG * VB / 2> v[4];  // tokens 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9
 #pragma unroll
             for (int i = 0; i < 4; ++i) load_v(v[i], values_at[i & 1], h * 16 + (i >> 1) * 8);
-            uint32_t weights[NS][2];
+            uint32_t weights[NT][2];
 #pragma unroll
-            for (int nt = 0; nt < NS; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) weights[nt][i] = transpose8x8(pack_half(weight[h][nt][2 * i], weight[h][nt][2 * i + 1]));
 #pragma unroll
             for (int u = 0; u < NG; ++u) {
-                uint32_t b[NS][2];
+                uint32_t b[NT][2];
 #pragma unroll
-                for (int nt = 0; nt < NS; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) b[nt][i] = half_mul(weights[nt][i], sv.w[i * kSG + u]);
                 uint32_t a[2][4];
@@ -913,12 +906,12 @@ struct Attend {
     __device__ static __forceinline__ void leave_sums(Warp& w, float* ml) {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
 #pragma unroll
-        for (int nt = 0; nt < (kF32 ? 1 : NT); ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int d = 4; d <= 16; d <<= 1) w.sum[nt][e] += __shfl_xor_sync(~0u, w.sum[nt][e], d);
-                if (gid == 0) {
+                if (gid == 0 && (!kF32 || tig < 2)) {
                     float* const to = ml + col_of(nt, 2 * tig + e) * 2;
                     to[0] = w.ref[nt][e], to[1] = w.sum[nt][e];
                 }
@@ -930,7 +923,7 @@ struct Attend {
         // the accumulators are in units of 2^(exponent - 6) kValueUnit, the sums in units of 2^-kShift
         const float up = __int_as_float(w.scale_exp << 23);
 #pragma unroll
-        for (int nt = 0; nt < (kF32 ? 1 : NT); ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int col = col_of(nt, 2 * tig + e) - c0;
@@ -942,10 +935,10 @@ struct Attend {
                     for (int i = 0; i < 4; ++i) {
                         const int j = 2 * u + (i >> 1), at = (i & 1) * 2 + e;
                         const float times = VB == 4 && (i & 1) ? 16.0f : 1.0f;
-                        const float y = kF32 ? w.o[0][j][at] + w.o[NT - 1][j][at] : w.o[nt][j][at];
+                        const float y = kF32 ? w.o[nt][j][at] + __shfl_xor_sync(~0u, w.o[nt][j][at], 2) : w.o[nt][j][at];
                         x[i] = y * (by / times) * up;
                     }
-                    if (col >= 0 && col < kRoundCols)
+                    if (col >= 0 && col < kRoundCols && (!kF32 || tig < 2))
                         asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(o + (col * D + u * kGroup + gid * 4) * 4), "f"(x[0]), "f"(x[1]),
                                      "f"(x[2]), "f"(x[3])
                                      : "memory");
@@ -1359,7 +1352,7 @@ int launch_attend(const AttendParams& p, const Plan& plan, void* stream) {
 
 template <int NG, int KB, int VB>
 int attend_sized(const AttendParams& p, const Plan& plan, void* stream) {
-    if (p.c.dtype == B2KV_DTYPE_F32) return launch_attend<float, NG, KB, VB, 2>(p, plan, stream);
+    if (p.c.dtype == B2KV_DTYPE_F32) return launch_attend<float, NG, KB, VB, 1>(p, plan, stream);
     return plan.cols == 8 ? launch_attend<__nv_bfloat16, NG, KB, VB, 1>(p, plan, stream) : launch_attend<__nv_bfloat16, NG, KB, VB, 2>(p, plan, stream);
 }
 
