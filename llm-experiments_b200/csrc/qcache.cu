@@ -47,6 +47,7 @@ struct Octet {
         for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
     }
     __device__ __forceinline__ void widen(float (&f)[8]) const;
+    __device__ __forceinline__ uint32_t largest() const;  // magnitude, as a whole number: in the same order, NaN above infinity above all others
 };
 template <>
 __device__ __forceinline__ void Octet<float>::widen(float (&f)[8]) const {
@@ -57,6 +58,41 @@ template <>
 __device__ __forceinline__ void Octet<__nv_bfloat16>::widen(float (&f)[8]) const {
     Elt<__nv_bfloat16>::widen(w[0], f);
 }
+template <>
+__device__ __forceinline__ uint32_t Octet<float>::largest() const {
+    const uint32_t a = max(max(w[0].x & 0x7fffffffu, w[0].y & 0x7fffffffu), max(w[0].z & 0x7fffffffu, w[0].w & 0x7fffffffu));
+    const uint32_t b = max(max(w[1].x & 0x7fffffffu, w[1].y & 0x7fffffffu), max(w[1].z & 0x7fffffffu, w[1].w & 0x7fffffffu));
+    return max(a, b);
+}
+template <>
+__device__ __forceinline__ uint32_t Octet<__nv_bfloat16>::largest() const {
+    const uint32_t x = __vmaxu2(__vmaxu2(w[0].x & 0x7fff7fffu, w[0].y & 0x7fff7fffu), __vmaxu2(w[0].z & 0x7fff7fffu, w[0].w & 0x7fff7fffu));
+    return max(x & 0xffff0000u, x << 16);
+}
+
+// Two numbers in one instruction.
+struct Two {
+    unsigned long long v;
+    __device__ __forceinline__ Two() {}
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+    __device__ __forceinline__ Two operator*(const Two& o) const {
+        Two r;
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(v), "l"(o.v));
+        return r;
+    }
+    __device__ __forceinline__ Two operator+(const Two& o) const {
+        Two r;
+        asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(v), "l"(o.v));
+        return r;
+    }
+    __device__ __forceinline__ static Two fma(const Two& a, const Two& b, const Two& c) {
+        Two r;
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+        return r;
+    }
+};
+
 __device__ __forceinline__ void store4(float* p, const float* f) { *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]); }
 __device__ __forceinline__ void store4(__nv_bfloat16* p, const float* f) {
     __nv_bfloat162 h[2] = {__floats2bfloat162_rn(f[0], f[1]), __floats2bfloat162_rn(f[2], f[3])};
@@ -70,14 +106,12 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float* f) {
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
 }
 
-// Eight codes as numbers code + 8 or code + 128, lowest first, of a group's elements; all four lanes of the group get its scale.
+// Eight codes as numbers code + 8 or code + 128, lowest first, of a group's elements, `most` their largest magnitude; all four lanes of the group get
+// its scale.
 template <int BITS>
-__device__ __forceinline__ uint2 quantise(const float (&f)[8], uint32_t& scale) {
+__device__ __forceinline__ uint2 quantise(const float (&f)[8], uint32_t most, uint32_t& scale) {
     constexpr int kTop = BITS == 4 ? 7 : 127;
     constexpr uint32_t kTimes = BITS == 4 ? 16 : 256;
-    uint32_t most = 0;  // magnitudes as whole numbers: in the same order, NaN above infinity above all others
-#pragma unroll
-    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(f[e]) & 0x7fffffffu);
     most = max(most, __shfl_xor_sync(~0u, most, 1));
     most = max(most, __shfl_xor_sync(~0u, most, 2));
     const __nv_bfloat16 rounded = __float2bfloat16_rn(most < 0x7f800000u ? __uint_as_float(most) / kTop : __int_as_float(0x7fc00000));
@@ -85,12 +119,15 @@ __device__ __forceinline__ uint2 quantise(const float (&f)[8], uint32_t& scale) 
     const float s = __bfloat162float(rounded);
     uint32_t n[8];
     if (s >= 0x1p-100f) {
-        const float inverse = 1.0f / s;
+        const float inverse = 1.0f / s, magic = 12582912.0f + (kTop + 1);  // 1.5 * 2^23: the sum's last bits are the rounded number's
+        const Two by(inverse, inverse), less(-s, -s), up(magic, magic);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float q = f[e] * inverse;
-            const float right = fmaf(fmaf(-q, s, f[e]), inverse, q);
-            n[e] = __float_as_uint(right + (12582912.0f + (kTop + 1)));  // 1.5 * 2^23: the sum's last bits are the rounded number's
+        for (int e = 0; e < 8; e += 2) {
+            const Two x(f[e], f[e + 1]), q = x * by;
+            const Two right = Two::fma(Two::fma(q, less, x), by, q) + up;
+            float a, b;
+            right.get(a, b);
+            n[e] = __float_as_uint(a), n[e + 1] = __float_as_uint(b);
         }
     } else {  // (no scale, or a NaN, or one so small that remainders would be cut off)
 #pragma unroll
@@ -167,7 +204,7 @@ __device__ __forceinline__ void write_row(const b2kv_qcache& c, const T* src, in
         float f[8];
         in[u].widen(f);
         uint32_t scale;
-        codes.template put<kValues>(u, quantise<BITS>(f, scale));
+        codes.template put<kValues>(u, quantise<BITS>(f, in[u].largest(), scale));
         scales[u / 2] |= u & 1 ? scale << 16 : scale;
     }
     if (row < 0) return;
