@@ -623,7 +623,7 @@ int b2kv_moe_combine(float* x, int64_t ld_x, const void* y, int64_t ld_y, const 
  *   values  element 32 u + 4 o + i is code i of unit o * (D / 32) + u, units of 4 codes;
  *   codes   lowest bits first, stored as code + 8 or code + 128; units of 4-bit codes (32 bits of keys, 16 of values) are turned left by two bits;
  *   scales  scale of group u at u of b2kv_qcache_scale_row(D) bfloat16 per row, the rest is zeros.
- * D is 32, 64, 96, 128 or 256.  (k_bits, v_bits) is (4, 4), (8, 4) or (8, 8): keys are what suffers from few bits.
+ * D is 32, 64, 96, 128 or 256, T_max at most 2^30.  (k_bits, v_bits) is (4, 4), (8, 4) or (8, 8): keys are what suffers from few bits.
  * dtype is the type of the rows that are written, read back and attended with.  seq_lens (device, B entries) or len are the tokens
  * that each sequence holds; T_max bounds them (through a block table too).
  */
@@ -656,7 +656,7 @@ int b2kv_qcache_read(const b2kv_qcache* cache, int which, void* out, int n, int 
  * Attention of the last m tokens of every sequence over its n_b = min(max(len_b + len_bias, 0), T_upper) tokens, T_upper <= T_max a bound that the
  * host knows.  q and out are [B * m, H * D] (ld elements between rows), row b * m + i stands at place p = n_b - m + i; head h reads
  * key / value head h / (H / G) and sees the tokens t <= p, with window > 0 only those with p - t < window:
- *   score = cap(scale * q . k) - slopes[h] * (p - t),  cap(x) = softcap * tanh(x / softcap) where softcap > 0,  out = softmax(score) v.
+ *   score = cap(scale * q . k) - slopes[h] * (p - t),  cap(x) = softcap * tanh(x / softcap) where softcap > 0 (1e-30 at least),  out = softmax(score) v.
  * A row that sees nothing (an empty sequence, p < 0) is zeros.  slopes (fp32, H) may be NULL.  1 <= m <= B2KV_QCACHE_MAX_ROWS.
  * `workspace` takes b2kv_qcache_attend_workspace_bytes bytes (16-byte aligned), needs no initialisation and carries nothing between
  * calls; calls that may run at the same time need one each.
@@ -686,6 +686,8 @@ int b2kv_qcache_attend(const b2kv_qcache* cache, const b2kv_qcache_attend_args* 
  * behave as if their first bounded wait had run out (the launch then ends after about two seconds with
  * B2KV_DEV_WAIT_TIMEOUT in dev_status), "linear_test_expire": 1 = the same for the warps that take sums out in fp32 products of more
  * than 16 rows, "matmul_splits": ranges of input features per tile in b2kv_matmul_rows,
+ * "qcache_cluster": 1, 2, 4 or 8 CTAs per (sequence, key / value head) in b2kv_qcache_attend, -1 = all tokens end to end in even pieces,
+ * "qcache_columns": 8 or 16 (new token, query head) pairs taken together there in bf16,
  * "serial_launches": 1 = plain stream order for every launch (see "overlap" at the top),
  * "gemm_variant": 1 = one CTA per output tile, 2 / 3 = CTA pairs with 64 / 128 input features per
  * ring stage in b2kv_matmul);

@@ -26,6 +26,7 @@ int check(const b2kv_qcache* c) {
     if (!bits) return B2KV_ERR_UNSUPPORTED;
     if (!c->k_codes || !c->v_codes || !c->k_scales || !c->v_scales) return B2KV_ERR_BAD_ARG;
     if (c->B <= 0 || c->G <= 0 || c->T_max <= 0) return B2KV_ERR_BAD_ARG;
+    if (c->T_max > 1 << 30) return B2KV_ERR_UNSUPPORTED;  // (places are counted in 32 bits)
     if (c->block_table != nullptr) {
         if (c->max_blocks <= 0 || c->block_size <= 0 || c->n_blocks <= 0) return B2KV_ERR_BAD_ARG;
         if (static_cast<int64_t>(c->max_blocks) * c->block_size < c->T_max) return B2KV_ERR_BAD_ARG;

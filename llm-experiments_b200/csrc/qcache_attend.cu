@@ -17,7 +17,7 @@ int check_attend(const b2kv_qcache* c, const b2kv_qcache_attend_args* a) {
     if (a == nullptr || !a->q || !a->out) return B2KV_ERR_BAD_ARG;
     if (a->H <= 0 || a->H % c->G != 0 || a->m <= 0 || a->T_upper < 0 || a->T_upper > c->T_max || a->window < 0) return B2KV_ERR_BAD_ARG;
     if (a->m > B2KV_QCACHE_MAX_ROWS) return B2KV_ERR_UNSUPPORTED;
-    if (!isfinite(a->scale) || !(a->softcap >= 0.0f) || !isfinite(a->softcap)) return B2KV_ERR_BAD_ARG;
+    if (!isfinite(a->scale) || !isfinite(a->softcap) || !(a->softcap == 0.0f || a->softcap >= 1e-30f)) return B2KV_ERR_BAD_ARG;  // (its reciprocal is taken)
     const int64_t cols = static_cast<int64_t>(a->H) * c->D;
     if (a->ld_q < cols || a->ld_out < cols) return B2KV_ERR_BAD_ARG;
     const int es = elt_bytes(c->dtype);
@@ -30,12 +30,14 @@ size_t tickets_at(const Plan& plan, const b2kv_qcache& c) { return static_cast<s
 
 bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& plan) {
     const int columns = a.m * (a.H / c.G);
-    const int most = a.window > 0 ? std::min(a.T_upper, a.window + a.m - 1) : a.T_upper;
+    const int most = a.window > 0 ? static_cast<int>(std::min<int64_t>(a.T_upper, static_cast<int64_t>(a.window) + a.m - 1)) : a.T_upper;
     const int64_t heads = static_cast<int64_t>(c.B) * c.G;
     const int at_once = device_sm_count() * 2;  // CTAs that run at the same time
     // Columns (new token, query head) of a key / value head that are taken together: 16 share the widening of the codes (4 sequences of 131072
     // tokens, 16 heads to one: 198 against 242 us), 8 make more pairs where there are few tokens to a CTA (40 columns over 2048 tokens: 22.1 against 25.5 us).
-    const bool wide = c.dtype != B2KV_DTYPE_F32 && columns > 8 && heads * ((columns + 15) / 16) * most >= at_once * 1024ll;
+    const int forced_columns = tune_get("qcache_columns");
+    const bool wide = c.dtype != B2KV_DTYPE_F32 &&
+                      (forced_columns != 0 ? forced_columns == 16 : columns > 8 && heads * ((columns + 15) / 16) * most >= at_once * 1024ll);
     plan.cols = c.dtype == B2KV_DTYPE_F32 ? 4 : wide ? 16 : 8;
     plan.col_tiles = (columns + plan.cols - 1) / plan.cols;
     plan.pairs = heads * plan.col_tiles;
@@ -97,7 +99,8 @@ int b2kv_qcache_attend(const b2kv_qcache* cache, const b2kv_qcache_attend_args* 
     p.by_block = by_block(c);
     p.q = a.q, p.out = a.out, p.slopes = a.slopes, p.dev_status = dev_status;
     p.ld_q = a.ld_q, p.ld_out = a.ld_out;
-    p.R = a.H / c.G, p.m = a.m, p.col_tiles = plan.col_tiles, p.T_upper = a.T_upper, p.len_bias = a.len_bias, p.window = a.window;
+    p.R = a.H / c.G, p.m = a.m, p.col_tiles = plan.col_tiles, p.T_upper = a.T_upper, p.len_bias = a.len_bias;
+    p.window = static_cast<int>(std::min<int64_t>(a.window, static_cast<int64_t>(a.T_upper) + a.m));  // (no sum with it overflows)
     p.cluster = plan.cluster;
     p.scale = a.scale, p.softcap = a.softcap;
     p.ws_o = static_cast<float*>(workspace);

@@ -39,6 +39,8 @@ def quant_cache_create(ctx: GPUContext, config: QuantKVCacheConfig) -> QuantKVCa
     if (config.k_bits, config.v_bits) not in BITS:
         raise ValueError(f"(k_bits, v_bits) = ({config.k_bits}, {config.v_bits}) is not one of {BITS}")
     dtype_code(config.dtype)
+    if config.max_seq_len > 1 << 30:
+        raise ValueError(f"max_seq_len must be at most {1 << 30}, got {config.max_seq_len}")
     if config.block_size < 0 or config.n_blocks < 0:
         raise ValueError("block_size and n_blocks must be >= 0")
     B, T, G, D = config.batch_size, config.max_seq_len, config.n_kv_heads, config.head_dim
@@ -150,7 +152,7 @@ def quant_cache_gather(ctx: GPUContext, cache: QuantKVCache, layer_idx: int, whi
         raise ValueError(f"length must be > 0 and pending >= 0, got {n} and {pending}")
     out = torch.empty((cache.batch_size, n, cache.n_kv_heads, cache.head_dim), dtype=cache.dtype, device=cache.layers[layer_idx].k_codes.buffer.device)
     stream = batch_op_begin(ctx)
-    _native.check(_native.lib.b2kv_qcache_read(described, 0 if which == "k" else 1, out.data_ptr(), n, int(last), pending, dev_status_ptr(ctx), stream))
+    _native.check(_native.lib.b2kv_qcache_read(described, 0 if which == "k" else 1, out.data_ptr(), n, int(last), min(pending, cache.max_seq_len), dev_status_ptr(ctx), stream))
     return out
 
 
@@ -173,8 +175,8 @@ def attention_with_quant_cache(ctx: GPUContext, cache: QuantKVCache, layer_idx: 
         raise ValueError("Cache is empty: current_len=0")
     if window < 0:
         raise ValueError(f"window must be >= 0, got {window}")
-    if not (math.isfinite(softcap) and softcap >= 0) or (scale is not None and not math.isfinite(scale)):
-        raise ValueError(f"softcap must be finite and >= 0 and scale finite, got {softcap} and {scale}")
+    if not (math.isfinite(softcap) and (softcap == 0 or softcap >= 1e-30)) or (scale is not None and not math.isfinite(scale)):
+        raise ValueError(f"softcap must be 0 or finite and at least 1e-30 and scale finite, got {softcap} and {scale}")
     D, columns = cache.head_dim, q_new.shape[1]
     heads = columns // D
     if heads * D != columns or heads == 0 or heads % cache.n_kv_heads != 0:
@@ -186,7 +188,7 @@ def attention_with_quant_cache(ctx: GPUContext, cache: QuantKVCache, layer_idx: 
         if slopes.buffer.dtype != torch.float32 or not slopes.buffer.is_contiguous():
             raise ValueError("slopes must be contiguous float32")
     args = _native.qcache_attend_args(q_new.buffer.data_ptr(), output.buffer.data_ptr(), 0 if slopes is None else slopes.buffer.data_ptr(),
-                                      ld_q, ld_out, heads, tokens, held, pending, window, D ** -0.5 if scale is None else scale, softcap)
+                                      ld_q, ld_out, heads, tokens, held, pending, min(window, held + tokens), D ** -0.5 if scale is None else scale, softcap)
     stream, lib = batch_op_begin(ctx), _native.lib
     nbytes = lib.b2kv_qcache_attend_workspace_bytes(described, args)
     # Scratch of this call alone, from the stream's (or the capture's) own memory: nothing is shared by calls that run at the same time.

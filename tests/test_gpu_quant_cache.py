@@ -254,6 +254,59 @@ def test_windows(pkg, ctx, window, dtype, bits):
     check(attend(pkg, ctx, cache, q, window=window), q, held, lens, 1, window=window)
 
 
+@pytest.fixture()
+def tune(pkg):
+    knobs = {}
+
+    def set_knob(name, value):
+        knobs[name] = 0
+        pkg._native.tune(name, value)
+
+    yield set_knob
+    for name in knobs:
+        pkg._native.tune(name, 0)
+
+
+@pytest.mark.parametrize("cluster", [1, 2, 4, 8, -1])
+@pytest.mark.parametrize("dtype,D,bits,block,m,R,window", [(BF, 128, (4, 4), 0, 1, 4, 0), (BF, 64, (8, 8), 16, 3, 5, 100), (F32, 96, (8, 4), 24, 2, 3, 0),
+                                                           (BF, 256, (8, 4), 0, 1, 1, 0), (F32, 32, (4, 4), 64, 1, 9, 0)])
+def test_every_way_to_cut(pkg, ctx, tune, cluster, dtype, D, bits, block, m, R, window):
+    """CTAs in clusters and runs of tiles over many sequences: pairs cut once, several times and not at all, runs that begin anywhere."""
+    tune("qcache_cluster", cluster)
+    lens = [700, 0, 1, 33, 64, 1999, 5, 310, 96, 2, 0, 1024, 31, 32, 500]
+    cache, held = filled(pkg, ctx, lens, 2000, 3, D, dtype, bits, block)
+    q = rnd((len(lens) * m, 3 * R * D), dtype, 9, 1.5)
+    check(attend(pkg, ctx, cache, q, tokens=m, window=window), q, held, lens, m, window=window)
+
+
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("cluster,m,R", [(-1, 1, 16), (2, 5, 5), (1, 1, 3)])
+def test_sixteen_columns(pkg, ctx, tune, D, bits, cluster, m, R):
+    tune("qcache_columns", 16)
+    tune("qcache_cluster", cluster)
+    lens = [700, 0, 33, 64, 311, 5]
+    cache, held = filled(pkg, ctx, lens, 700, 2, D, BF, bits, 16)
+    q = rnd((len(lens) * m, 2 * R * D), BF, 9, 1.5)
+    check(attend(pkg, ctx, cache, q, tokens=m), q, held, lens, m)
+
+
+def test_more_sequences_than_threads(pkg, ctx, tune):
+    """Runs over 500 sequences: every thread of a CTA adds up several."""
+    lens = [(7 * i) % 61 for i in range(500)]
+    for cluster in (-1, 1):
+        tune("qcache_cluster", cluster)
+        cache, held = filled(pkg, ctx, lens, 61, 1, 64)
+        q = rnd((len(lens), 2 * 64), BF, 9, 1.5)
+        check(attend(pkg, ctx, cache, q), q, held, lens, 1)
+
+
+def test_a_window_longer_than_any_number(pkg, ctx):
+    cache, held = filled(pkg, ctx, [90, 300], 300, 1, 64)
+    q = rnd((2, 128), BF, 9)
+    assert torch.equal(attend(pkg, ctx, cache, q, window=2 ** 31 - 1), attend(pkg, ctx, cache, q))
+
+
 @pytest.mark.parametrize("softcap,biased", [(30.0, False), (0.5, True), (0.0, True)])
 @pytest.mark.parametrize("dtype,m", [(BF, 1), (F32, 1), (BF, 3)])
 def test_capped_and_biased_scores(pkg, ctx, softcap, biased, dtype, m):

@@ -82,6 +82,8 @@ def test_create_refuses_what_no_kernel_takes(pkg, ctx):
         make(pkg, ctx, dtype=torch.float16)
     with pytest.raises(ValueError, match="n_blocks"):
         make(pkg, ctx, block_size=16, n_blocks=5)
+    with pytest.raises(ValueError, match="max_seq_len must be at most"):
+        make(pkg, ctx, max_seq_len=(1 << 30) + 1)
     with pytest.raises(ValueError, match="block_size"):
         make(pkg, ctx, block_size=-16)
 
@@ -147,6 +149,7 @@ def test_attention_refusals(pkg, ctx):
     refused("window", window=-1)
     refused("softcap", softcap=-1.0)
     refused("softcap", softcap=float("inf"))
+    refused("softcap", softcap=1e-40)
     refused("scale", scale=float("nan"))
     refused("columns", q=two(pkg, 2, 192))
     refused("columns", q=two(pkg, 2, 100))
@@ -173,6 +176,7 @@ def test_entry_points_check_before_any_launch(pkg):
 
     assert write(dt=7) == -3 and write(D=80) == -3 and write(kb=4, vb=8) == -3 and write(kb=2) == -3
     assert write(k=None) == -1 and write(ks=0) == -1 and write(B=0) == -1 and write(n=0) == -1 and write(n=5) == -1 and write(ld=64) == -1
+    assert write(T=(1 << 30) + 1) == -3
     assert write(len=-1) == -1 and write(len=8) == -1
     assert write(k=A + 8) == -2 and write(ld=132) == -2 and write(v=A + 4) == -2
     assert write(table=A) == -1 and write(table=A, max_blocks=1, block=4, n_blocks=1) == -1  # a table that does not hold T_max
@@ -186,7 +190,7 @@ def test_entry_points_check_before_any_launch(pkg):
 
     assert attend(q=0) == -1 and attend(H=3) == -1 and attend(m=0) == -1 and attend(T=9) == -1 and attend(window=-1) == -1
     assert attend(m=65) == -3 and attend(c=dict(D=80)) == -3
-    assert attend(scale=float("nan")) == -1 and attend(cap=-1.0) == -1 and attend(ld_q=128) == -1
+    assert attend(scale=float("nan")) == -1 and attend(cap=-1.0) == -1 and attend(cap=1e-35) == -1 and attend(ld_q=128) == -1
     assert attend(ld_out=260) == -2 and attend(q=A + 2) == -2
     big, long_args = dict(T=1 << 20), dict(T=1 << 20)
     need = lib.b2kv_qcache_attend_workspace_bytes(cache(**big), native.qcache_attend_args(*{**args, **long_args}.values()))
