@@ -19,19 +19,23 @@ and waits inside the kernel for that one to complete; the weight-streaming kerne
 tiles before that wait.  Every
 layer owns its own ``KVCache`` object (``n_layers=1``), so that the lengths advance once per layer
 step; a ragged (per-sequence length) cache works like a shared-length one.
+
+A layer whose cache is a ``QuantKVCache`` (4 or 8 bits) projects Q, K and V by three products, quantises the new rows into
+the cache and attends over it as it is; a prompt attends over its own rows in full width.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
 from .attention import flash_attention
 from .kv_cache import attention_with_kv_cache
 from .projection import matmul, qkv_project_append
+from .quant_cache import attention_with_quant_cache, quant_cache_reset, quant_cache_update
 from .step_tail import layernorm
-from .types import GPUBuffer1D, GPUBuffer2D, GPUContext, KVCache
+from .types import GPUBuffer1D, GPUBuffer2D, GPUContext, KVCache, QuantKVCache
 
 
 @dataclass
@@ -61,6 +65,8 @@ class DecoderLayerScratch:
     a: GPUBuffer2D     # attention output
     x2: GPUBuffer2D
     m: GPUBuffer2D     # MLP hidden rows [B, 4E]
+    k: Optional[GPUBuffer2D] = None  # new rows for a quantised cache
+    v: Optional[GPUBuffer2D] = None
 
 
 def _buf(ctx: GPUContext, rows: int, cols: int) -> GPUBuffer2D:
@@ -68,21 +74,28 @@ def _buf(ctx: GPUContext, rows: int, cols: int) -> GPUBuffer2D:
     return GPUBuffer2D(buffer=t, shape=(rows, cols), size=rows * cols)
 
 
-def decoder_layer_scratch(ctx: GPUContext, batch_size: int, embedding_dim: int, hidden_dim: Optional[int] = None) -> DecoderLayerScratch:
+def decoder_layer_scratch(ctx: GPUContext, batch_size: int, embedding_dim: int, hidden_dim: Optional[int] = None,
+                          quantised: bool = False) -> DecoderLayerScratch:
     hidden_dim = hidden_dim or 4 * embedding_dim
     mk = lambda c: _buf(ctx, batch_size, c)  # noqa: E731
     return DecoderLayerScratch(h=mk(embedding_dim), q=mk(embedding_dim), a=mk(embedding_dim), x2=mk(embedding_dim),
-                               m=mk(hidden_dim))
+                               m=mk(hidden_dim), k=mk(embedding_dim) if quantised else None, v=mk(embedding_dim) if quantised else None)
 
 
-def decoder_layer_step(ctx: GPUContext, cache: KVCache, x: GPUBuffer2D, w: DecoderLayerWeights, s: DecoderLayerScratch,
+def decoder_layer_step(ctx: GPUContext, cache: Union[KVCache, QuantKVCache], x: GPUBuffer2D, w: DecoderLayerWeights, s: DecoderLayerScratch,
                        y: GPUBuffer2D) -> None:
     """Writes the layer's output rows for one new token per sequence into ``y`` and appends the token's
     K / V to ``cache`` (layer 0 of that cache object).  To be called between ``batch_begin`` and
-    ``batch_commit``; seven operations are recorded."""
+    ``batch_commit``; seven operations are recorded (ten with a quantised cache, whose scratch has ``k`` and ``v``)."""
     layernorm(ctx, x, w.ln1_gamma, w.ln1_beta, s.h)
-    qkv_project_append(ctx, cache, 0, s.h, w.wq, w.wk, w.wv, s.q)
-    attention_with_kv_cache(ctx, cache, 0, s.q, s.a)
+    if isinstance(cache, QuantKVCache):
+        for weights, rows in ((w.wq, s.q), (w.wk, s.k), (w.wv, s.v)):
+            matmul(ctx, s.h, weights, rows)
+        quant_cache_update(ctx, cache, 0, s.k, s.v)
+        attention_with_quant_cache(ctx, cache, 0, s.q, s.a)
+    else:
+        qkv_project_append(ctx, cache, 0, s.h, w.wq, w.wk, w.wv, s.q)
+        attention_with_kv_cache(ctx, cache, 0, s.q, s.a)
     matmul(ctx, s.a, w.wo, s.x2, residual=x)
     layernorm(ctx, s.x2, w.ln2_gamma, w.ln2_beta, s.h)
     matmul(ctx, s.h, w.w1, s.m, bias=w.b1, activation="gelu")
@@ -109,7 +122,7 @@ def prompt_layer_scratch(ctx: GPUContext, rows: int, embedding_dim: int, hidden_
                               a=mk(embedding_dim), x2=mk(embedding_dim), m=mk(hidden_dim))
 
 
-def prompt_layer_step(ctx: GPUContext, cache: KVCache, x: GPUBuffer2D, w: DecoderLayerWeights, s: PromptLayerScratch,
+def prompt_layer_step(ctx: GPUContext, cache: Union[KVCache, QuantKVCache], x: GPUBuffer2D, w: DecoderLayerWeights, s: PromptLayerScratch,
                       y: GPUBuffer2D, batch_size: int, seq_len: int) -> None:
     """The same layer for a whole prompt: ``x`` and ``y`` are ``[batch_size * seq_len, E]``.  The reference's
     block as it stands (simple-llm/src/wgpu_backend.py:794-935: three projections, causal
@@ -120,8 +133,13 @@ def prompt_layer_step(ctx: GPUContext, cache: KVCache, x: GPUBuffer2D, w: Decode
     matmul(ctx, s.h, w.wq, s.q)
     matmul(ctx, s.h, w.wk, s.k)
     matmul(ctx, s.h, w.wv, s.v)
-    flash_attention(ctx, s.q, s.k, s.v, s.a, None, None, batch_size, seq_len, cache.n_heads, cache.head_dim,
-                    cache=cache, layer_idx=0)
+    if isinstance(cache, QuantKVCache):
+        flash_attention(ctx, s.q, s.k, s.v, s.a, None, None, batch_size, seq_len, cache.n_kv_heads, cache.head_dim)
+        quant_cache_reset(cache)
+        quant_cache_update(ctx, cache, 0, s.k, s.v, tokens=seq_len)
+    else:
+        flash_attention(ctx, s.q, s.k, s.v, s.a, None, None, batch_size, seq_len, cache.n_heads, cache.head_dim,
+                        cache=cache, layer_idx=0)
     matmul(ctx, s.a, w.wo, s.x2, residual=x)
     layernorm(ctx, s.x2, w.ln2_gamma, w.ln2_beta, s.h)
     matmul(ctx, s.h, w.w1, s.m, bias=w.b1, activation="gelu")

@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass, field
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
@@ -27,9 +27,10 @@ from .batch import batch_begin, batch_commit
 from .decode_layer import DecoderLayerScratch, DecoderLayerWeights, PromptLayerScratch
 from .kv_cache import kv_cache_create, kv_cache_reset
 from .projection import matmul
+from .quant_cache import quant_cache_create
 from .registry import register_model
 from .step_tail import argmax, embedding, extract_last_tokens, layernorm
-from .types import GPUBuffer1D, GPUBuffer2D, GPUContext, KVCache, KVCacheConfig
+from .types import GPUBuffer1D, GPUBuffer2D, GPUContext, KVCache, KVCacheConfig, QuantKVCache, QuantKVCacheConfig
 
 
 @dataclass
@@ -64,7 +65,7 @@ class DecoderState:
     cfg: DecoderConfig
     weights: DecoderWeights
     batch_size: int
-    caches: List[KVCache]
+    caches: List[Union[KVCache, QuantKVCache]]
     x: GPUBuffer2D
     y: GPUBuffer2D
     h: GPUBuffer2D
@@ -127,20 +128,27 @@ def random_weights(ctx: GPUContext, cfg: DecoderConfig, seed: int = 0) -> Decode
 
 
 def decoder_state_create(ctx: GPUContext, cfg: DecoderConfig, weights: DecoderWeights, batch_size: int,
-                         max_seq_len: Optional[int] = None, ragged: bool = False) -> DecoderState:
+                         max_seq_len: Optional[int] = None, ragged: bool = False,
+                         kv_bits: Optional[Tuple[int, int]] = None) -> DecoderState:
+    """``kv_bits``: bits of cached keys and of values, (4, 4), (8, 4) or (8, 8); ``None``: bfloat16 caches."""
     if cfg.embedding_dim % cfg.n_heads != 0:
         raise ValueError(f"embedding_dim {cfg.embedding_dim} is not divisible by n_heads {cfg.n_heads}")
     T = cfg.context_size if max_seq_len is None else max_seq_len
     if T > cfg.context_size:
         raise ValueError(f"Sequence length {T} exceeds context size {cfg.context_size}")
     E, dev = cfg.embedding_dim, ctx.device
-    caches = [kv_cache_create(ctx, KVCacheConfig(batch_size=batch_size, max_seq_len=T, n_layers=1, n_heads=cfg.n_heads,
-                                                 head_dim=cfg.head_dim, dtype=torch.bfloat16, layout="bhtd",
-                                                 ragged=ragged)) for _ in range(cfg.n_layers)]
+    if kv_bits is not None:
+        caches = [quant_cache_create(ctx, QuantKVCacheConfig(batch_size=batch_size, max_seq_len=T, n_layers=1, n_kv_heads=cfg.n_heads,
+                                                             head_dim=cfg.head_dim, k_bits=kv_bits[0], v_bits=kv_bits[1],
+                                                             ragged=ragged)) for _ in range(cfg.n_layers)]
+    else:
+        caches = [kv_cache_create(ctx, KVCacheConfig(batch_size=batch_size, max_seq_len=T, n_layers=1, n_heads=cfg.n_heads,
+                                                     head_dim=cfg.head_dim, dtype=torch.bfloat16, layout="bhtd",
+                                                     ragged=ragged)) for _ in range(cfg.n_layers)]
     mk = lambda cols: _b2(torch.empty((batch_size, cols), dtype=torch.bfloat16, device=dev))  # noqa: E731
     ctx.config.flash_attn_max_head_dim = max(ctx.config.flash_attn_max_head_dim, cfg.head_dim)
     return DecoderState(cfg=cfg, weights=weights, batch_size=batch_size, caches=caches, x=mk(E), y=mk(E), h=mk(E),
-                        logits=mk(cfg.vocab_size), scratch=decode_layer.decoder_layer_scratch(ctx, batch_size, E),
+                        logits=mk(cfg.vocab_size), scratch=decode_layer.decoder_layer_scratch(ctx, batch_size, E, quantised=kv_bits is not None),
                         last=mk(E))
 
 
@@ -302,9 +310,9 @@ class CachedDecoder:
     """Batch-of-one adapter with the interface ``generate_text`` drives: ``cache``, ``context``,
     ``prefill(tokens) -> logits [1, vocab]`` and ``decode_step(token) -> logits [1, vocab]`` (float32)."""
 
-    def __init__(self, ctx: GPUContext, cfg: DecoderConfig, weights: DecoderWeights):
+    def __init__(self, ctx: GPUContext, cfg: DecoderConfig, weights: DecoderWeights, kv_bits: Optional[Tuple[int, int]] = None):
         self.ctx, self.cfg = ctx, cfg
-        self.state = decoder_state_create(ctx, cfg, weights, batch_size=1)
+        self.state = decoder_state_create(ctx, cfg, weights, batch_size=1, kv_bits=kv_bits)
         self.context = cfg.context_size
         self.cache = _CacheGroup(self.state)
         self._tok = _b1(torch.zeros(1, dtype=torch.int32, device=ctx.device))
@@ -343,7 +351,8 @@ class _CacheGroup:
 
 @register_model("GPTDecoder")
 def _build(ctx: GPUContext, config: dict, weights: dict, dtype: torch.dtype, batch_size: int, max_tokens: int) -> CachedDecoder:
-    """The decoder of a model folder: ``config`` holds the fields of ``DecoderConfig``, the checkpoint ``embedding``,
+    """The decoder of a model folder: ``config`` holds the fields of ``DecoderConfig`` and, for a cache in 4 or 8 bits, ``kv_bits`` (of keys and of
+    values), the checkpoint ``embedding``,
     ``out_proj``, ``lnf_gamma``, ``lnf_beta`` and ``layers.<i>.<name>`` for the fields of ``DecoderLayerWeights``."""
     if dtype != torch.bfloat16:
         raise ValueError("this decoder runs in bfloat16 only")
@@ -354,4 +363,5 @@ def _build(ctx: GPUContext, config: dict, weights: dict, dtype: torch.dtype, bat
     layers = [{k: get(f"layers.{i}.{k}") for k in DecoderLayerWeights.__dataclass_fields__} for i in range(cfg.n_layers)]
     params = dict(embedding=get("embedding"), pos_encoding=positional_encoding(cfg.context_size, cfg.embedding_dim), layers=layers,
                   lnf_gamma=get("lnf_gamma"), lnf_beta=get("lnf_beta"), out_proj=get("out_proj"))
-    return CachedDecoder(ctx, cfg, weights_from_numpy(ctx, cfg, params))
+    bits = config.get("kv_bits")
+    return CachedDecoder(ctx, cfg, weights_from_numpy(ctx, cfg, params), None if bits is None else (int(bits[0]), int(bits[1])))

@@ -21,14 +21,17 @@ def bf16_round(a):
     return u.astype(np.uint32).view(np.float32).reshape(a.shape)
 
 
-def decoder_layer_step(x, w, k_rows, v_rows, lens, n_heads):
+def decoder_layer_step(x, w, k_rows, v_rows, lens, n_heads, hold=None):
     """x [B, E] float32 (bf16 values); w: dict of float32 arrays (bf16 values); k_rows / v_rows:
     per sequence, float32 [len_b, E] of the cached K / V rows (bf16 values); returns
-    (y [B, E], new K rows [B, E], new V rows [B, E]) as float32 arrays of bf16 values."""
+    (y [B, E], new K rows [B, E], new V rows [B, E]) as float32 arrays of bf16 values.  hold(rows, "k" or "v"): what a
+    quantised cache holds for new rows."""
     B, E = x.shape
     D = E // n_heads
     h1 = bf16_round(layernorm(x, w["ln1_gamma"], w["ln1_beta"]))
     q, k_new, v_new = (bf16_round(t) for t in kv_oracle.qkv_project(h1, w["wq"], w["wk"], w["wv"]))
+    if hold is not None:
+        k_new, v_new = hold(k_new, "k"), hold(v_new, "v")
     a = np.zeros((B, E), dtype=np.float32)
     for b in range(B):
         K = np.concatenate([k_rows[b][: lens[b]], k_new[b : b + 1]], axis=0).reshape(-1, n_heads, D)
