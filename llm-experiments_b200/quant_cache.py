@@ -88,17 +88,13 @@ def quant_cache_set_lengths(cache: QuantKVCache, lens) -> None:
 
 
 def _layer(cache: QuantKVCache, layer_idx: int):
-    """``b2kv_qcache`` of a layer.  (Asking a tensor for its address costs 0.2 us, a step of a decoding loop would ask four for each call.)"""
+    """``b2kv_qcache`` of a layer."""
     layers = cache.layers
     if layer_idx < 0 or layer_idx >= len(layers):
         raise ValueError(f"layer_idx {layer_idx} out of range [0, {len(layers)})")
-    layer = layers[layer_idx]
-    kc, vc, ks, vs, kept = layer.k_codes.buffer, layer.v_codes.buffer, layer.k_scales.buffer, layer.v_scales.buffer, layer.pointers
-    if kept is None or kept[0] is not kc or kept[1] is not vc or kept[2] is not ks or kept[3] is not vs:
-        kept = layer.pointers = (kc, vc, ks, vs, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr())
-    table, lens = cache.block_table, cache.seq_lens
+    layer, table, lens = layers[layer_idx], cache.block_table, cache.seq_lens
     return _native.qcache(
-        kept[4], kept[5], kept[6], kept[7], 0 if table is None else table.data_ptr(), 0 if lens is None else lens.data_ptr(), cache.current_len,
+        layer.k_codes.buffer.data_ptr(), layer.v_codes.buffer.data_ptr(), layer.k_scales.buffer.data_ptr(), layer.v_scales.buffer.data_ptr(), 0 if table is None else table.data_ptr(), 0 if lens is None else lens.data_ptr(), cache.current_len,
         cache.batch_size, cache.n_kv_heads, cache.head_dim, cache.max_seq_len, 0 if table is None else table.shape[1], cache.block_size,
         cache.n_blocks, cache.k_bits, cache.v_bits, dtype_code(cache.dtype))
 

@@ -175,7 +175,6 @@ class QuantKVCacheLayer:
     v_codes: GPUBuffer2D
     k_scales: GPUBuffer2D
     v_scales: GPUBuffer2D
-    pointers: Optional[Tuple] = None  # the four tensors and where they lie, as the last call found them
 
 
 @dataclass

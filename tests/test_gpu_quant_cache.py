@@ -407,6 +407,34 @@ def test_the_same_call_gives_the_same_bits(pkg, ctx):
         assert torch.equal(attend(pkg, ctx, cache, q), first)
 
 
+@pytest.mark.parametrize("dtype,m,R,lens", [(BF, 1, 4, [40, 0, 300]), (BF, 3, 7, [2500, 33, 900]), (F32, 2, 3, [700, 5, 64])])
+@pytest.mark.parametrize("cluster", [1, 4, -1])
+def test_outputs_in_the_queries_place(pkg, ctx, tune, dtype, m, R, lens, cluster):
+    """Several tiles of columns and several CTAs to a pair, which write where others read their queries."""
+    tune("qcache_cluster", cluster)
+    cache, _ = filled(pkg, ctx, lens, max(lens), 2, 128, dtype)
+    q = rnd((len(lens) * m, 2 * R * 128), dtype, 5, 1.5)
+    want, both = attend(pkg, ctx, cache, q, tokens=m), two(pkg, q.clone())
+    pkg.gpu.batch_begin(ctx)
+    pkg.gpu.attention_with_quant_cache(ctx, cache, 0, both, both, tokens=m)
+    pkg.gpu.batch_commit(ctx)
+    assert torch.equal(both.buffer, want)
+
+
+def test_buffers_that_lie_elsewhere_between_calls(pkg, ctx):
+    """A layer's tensors may be given other memory; the next call goes there."""
+    cache, _ = filled(pkg, ctx, [40, 7], 64, 2, 64)
+    q = rnd((2, 4 * 64), BF, 5)
+    want, layer = attend(pkg, ctx, cache, q), cache.layers[0]
+    for name in ("k_codes", "v_codes", "k_scales", "v_scales"):
+        t = getattr(layer, name).buffer
+        moved = t.clone()
+        old = t.detach().view_as(t)  # (keeps the old memory, which holds nothing of use any more)
+        t.set_(moved)
+        old.zero_()
+    assert torch.equal(attend(pkg, ctx, cache, q), want)
+
+
 def test_rows_whose_offsets_pass_32_bits(pkg, ctx):
     """The last sequence's rows lie beyond 4 GB of codes."""
     B, G, D, T = 3, 8, 128, 3_000_000
