@@ -138,6 +138,8 @@ def decoder_state_create(ctx: GPUContext, cfg: DecoderConfig, weights: DecoderWe
         raise ValueError(f"Sequence length {T} exceeds context size {cfg.context_size}")
     E, dev = cfg.embedding_dim, ctx.device
     if kv_bits is not None:
+        if len(kv_bits) != 2:
+            raise ValueError(f"kv_bits must be the bits of keys and of values, got {kv_bits!r}")
         caches = [quant_cache_create(ctx, QuantKVCacheConfig(batch_size=batch_size, max_seq_len=T, n_layers=1, n_kv_heads=cfg.n_heads,
                                                              head_dim=cfg.head_dim, k_bits=kv_bits[0], v_bits=kv_bits[1],
                                                              ragged=ragged)) for _ in range(cfg.n_layers)]
@@ -364,4 +366,4 @@ def _build(ctx: GPUContext, config: dict, weights: dict, dtype: torch.dtype, bat
     params = dict(embedding=get("embedding"), pos_encoding=positional_encoding(cfg.context_size, cfg.embedding_dim), layers=layers,
                   lnf_gamma=get("lnf_gamma"), lnf_beta=get("lnf_beta"), out_proj=get("out_proj"))
     bits = config.get("kv_bits")
-    return CachedDecoder(ctx, cfg, weights_from_numpy(ctx, cfg, params), None if bits is None else (int(bits[0]), int(bits[1])))
+    return CachedDecoder(ctx, cfg, weights_from_numpy(ctx, cfg, params), None if bits is None else tuple(int(b) for b in bits))

@@ -88,6 +88,13 @@ def test_create_refuses_what_no_kernel_takes(pkg, ctx):
         make(pkg, ctx, block_size=-16)
 
 
+@pytest.mark.parametrize("bits", [(4,), (8, 8, 8), (4, 8), (5, 5)])
+def test_a_decoder_refuses_other_bits(pkg, ctx, bits):
+    from llm_experiments_b200 import model
+    with pytest.raises(ValueError, match="bits"):
+        model.decoder_state_create(ctx, model.DecoderConfig(vocab_size=64, context_size=32, embedding_dim=64, n_heads=1, n_layers=1), None, 1, kv_bits=bits)
+
+
 def test_create_sizes(pkg, ctx):
     c = make(pkg, ctx, head_dim=128, k_bits=8, n_layers=2)
     lay = c.layers[1]
