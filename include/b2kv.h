@@ -686,7 +686,7 @@ int b2kv_qcache_attend(const b2kv_qcache* cache, const b2kv_qcache_attend_args* 
  * behave as if their first bounded wait had run out (the launch then ends after about two seconds with
  * B2KV_DEV_WAIT_TIMEOUT in dev_status), "linear_test_expire": 1 = the same for the warps that take sums out in fp32 products of more
  * than 16 rows, "matmul_splits": ranges of input features per tile in b2kv_matmul_rows,
- * "qcache_cluster": 1, 2, 4 or 8 CTAs per (sequence, key / value head) in b2kv_qcache_attend, -1 = all tokens end to end in even pieces,
+ * "qcache_cluster": 1 - 8 CTAs per (sequence, key / value head) in b2kv_qcache_attend, -1 = all tokens end to end in even pieces,
  * "qcache_columns": 8 or 16 (new token, query head) pairs taken together there in bf16,
  * "serial_launches": 1 = plain stream order for every launch (see "overlap" at the top),
  * "gemm_variant": 1 = one CTA per output tile, 2 / 3 = CTA pairs with 64 / 128 input features per

@@ -39,7 +39,7 @@ static Knob g_knobs[] = {
     {"serial_launches", 0},  // 1 = no kernel is launched ahead of the end of the kernel before it (plain stream order)
     {"gqa_runs", 0},  // b2kv_gqa_decode_runs in fp32: 0 = rows share keys and values where there are enough of them, 1 = always
     {"gqa_decode_share", 0},  // 128-key tiles per share in b2kv_gqa_decode (0 = by size)
-    {"qcache_cluster", 0},  // b2kv_qcache_attend: CTAs per (sequence, head), 1, 2, 4 or 8; -1 = all tokens end to end, cut evenly; 0 = by size
+    {"qcache_cluster", 0},  // b2kv_qcache_attend: CTAs per (sequence, head), 1 - 8; -1 = all tokens end to end, cut evenly; 0 = by size
     {"qcache_columns", 0},  // b2kv_qcache_attend in bf16: columns of a tile, 8 or 16; 0 = by size
     {"gemm_variant", 0},   // b2kv_matmul: 0 = by shape and device, 1 = one CTA per tile, 2 / 3 = CTA pairs, 64 / 128 features per stage
 };

@@ -28,6 +28,25 @@ int check_attend(const b2kv_qcache* c, const b2kv_qcache_attend_args* a) {
 // Results of two pairs per CTA, their sums, and a ticket per pair.
 size_t tickets_at(const Plan& plan, const b2kv_qcache& c) { return static_cast<size_t>(plan.ctas) * 2 * plan.cols * (c.D + 1) * sizeof(float); }
 
+constexpr int kMostCluster = 8;
+
+// Clusters of that many CTAs that a launch gets going together.  A cluster lies within one group of SMs, so there are fewer than there are places for
+// its CTAs (sizes 2 - 8: 148, 93, 71, 56, 45, 37, 33 for 296 CTAs), and the last of them wait for what an earlier launch leaves behind: one
+// in sixteen is not counted on (1024 tokens, 32 pairs: 8.0 us in clusters of 7, 10.5 of 8; 36 pairs: 8.0 of 6, 9.3 of 7, 14.2 of 8; 73 pairs: 9.5 of 3, 14.9 of 4).
+int64_t cluster_places(int size) {
+    static std::atomic<int> known[64][kMostCluster + 1];
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) device = 64;
+    int count = device < 64 ? known[device][size].load(std::memory_order_relaxed) : 0;
+    if (count == 0) {
+        count = size == 1 ? device_sm_count() * 2 : clusters_at_once(size);
+        if (count <= 0) count = std::max(1, device_sm_count() * 2 / size);
+        if (size > 2) count -= count / 16;
+        if (device < 64) known[device][size].store(count, std::memory_order_relaxed);
+    }
+    return count;
+}
+
 bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& plan) {
     const int columns = a.m * (a.H / c.G);
     const int most = a.window > 0 ? static_cast<int>(std::min<int64_t>(a.T_upper, static_cast<int64_t>(a.window) + a.m - 1)) : a.T_upper;
@@ -42,12 +61,12 @@ bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& pla
     plan.col_tiles = (columns + plan.cols - 1) / plan.cols;
     plan.pairs = heads * plan.col_tiles;
     if (plan.pairs > 0x7fffffff) return false;
-    // A cluster of 1, 2, 4 or 8 CTAs for each pair, or one run of tiles per CTA that is there.  In tokens that a CTA gets through in the time: setting
+    // A cluster of 1 - 8 CTAs for each pair, or one run of tiles per CTA that is there.  In tokens that a CTA gets through in the time: setting
     // up and finishing a CTA is about 430, putting a cluster's results together 150, finding and cutting a run 1000.
     const int64_t runs = 1000 + plan.pairs * most / at_once;
     int64_t best = 0;
-    for (int size = 1; size <= 8; size *= 2) {
-        const int64_t waves = (plan.pairs * size + at_once - 1) / at_once;
+    for (int size = 1; size <= kMostCluster; ++size) {
+        const int64_t places = cluster_places(size), waves = (plan.pairs + places - 1) / places;
         const int64_t cost = waves * (430 + (size > 1 ? 150 : 0) + (most + size - 1) / size);
         if (size == 1 || cost < best) best = cost, plan.cluster = size;
     }
@@ -55,7 +74,7 @@ bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& pla
     const bool countable = plan.pairs * (most / 16 + 1 + kPairCost) < (1ll << 31);
     if (runs < best && countable) plan.cluster = 0;
     const int forced = tune_get("qcache_cluster");
-    if (forced == 1 || forced == 2 || forced == 4 || forced == 8) plan.cluster = forced;
+    if (forced >= 1 && forced <= kMostCluster) plan.cluster = forced;
     if (forced < 0 && countable) plan.cluster = 0;
     plan.workspace = 0;
     if (plan.cluster == 0) {

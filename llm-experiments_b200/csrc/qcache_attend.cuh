@@ -1228,7 +1228,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
             // One pair per cluster.  Every CTA has a share of the columns' elements, quads rank, rank + cluster, ... of them, and gets all CTAs' results for
             // it, each behind the other, into the rings (all but the first stages), and their sums to where the queries were.
             constexpr int kRoom = (S - 1) * A::kStage / 16;  // quads in a warp's ring
-            static_assert(A::kCols * D / 4 <= W * kRoom && 8 * A::kCols * 4 <= NG * NT * 512, "");
+            static_assert(A::kCols * D / 4 + 7 <= W * kRoom && 8 * A::kCols * 4 <= NG * NT * 512, "");
             const auto where = [](int quad) { return static_cast<uint32_t>(quad / kRoom * (S * A::kStage) + A::kStage + quad % kRoom * 16); };
             const uint32_t their_lse = smem_u32(prepared.queries);
             const int rank = static_cast<int>(cluster_rank()), each = (A::kCols * D / 4 + p.cluster - 1) / p.cluster;
@@ -1349,6 +1349,21 @@ int launch_attend(const AttendParams& p, const Plan& plan, void* stream) {
     B2KV_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, kernel, p));
     return B2KV_OK;
 }
+
+// Clusters of `size` CTAs that run at the same time on the current device; 0 without one.
+template <typename T, int NG, int KB, int VB, int NT>
+int count_clusters(int size) {
+    using A = Attend<T, NG, KB, VB, NT>;
+    auto kernel = attend_kernel<T, NG, KB, VB, NT>;
+    int count = 0;
+    OverlapLaunch launch(dim3(static_cast<unsigned>(size)), A::kThreads, A::kSmem, nullptr, static_cast<unsigned>(size));
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, A::kSmem) == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&count, kernel, &launch.cfg) == cudaSuccess)
+        return count;
+    cudaGetLastError();
+    return 0;
+}
+int clusters_at_once(int size);
 
 template <int NG, int KB, int VB>
 int attend_sized(const AttendParams& p, const Plan& plan, void* stream) {

@@ -279,6 +279,18 @@ def test_every_way_to_cut(pkg, ctx, tune, cluster, dtype, D, bits, block, m, R, 
     check(attend(pkg, ctx, cache, q, tokens=m, window=window), q, held, lens, m, window=window)
 
 
+@pytest.mark.parametrize("cluster", [3, 5, 6, 7])
+@pytest.mark.parametrize("dtype,D,bits,m,R,columns", [(BF, 128, (8, 4), 1, 3, 0), (BF, 32, (4, 4), 5, 3, 0), (BF, 256, (8, 8), 4, 4, 16), (F32, 256, (4, 4), 1, 4, 0),
+                                                      (F32, 32, (8, 8), 1, 1, 0), (BF, 96, (4, 4), 2, 5, 16), (F32, 64, (8, 4), 3, 2, 0)])
+def test_clusters_that_do_not_divide_the_elements(pkg, ctx, tune, cluster, dtype, D, bits, m, R, columns):
+    tune("qcache_cluster", cluster)
+    tune("qcache_columns", columns)
+    lens = [700, 0, 1, 33, 64, 1999, 5, 310]
+    cache, held = filled(pkg, ctx, lens, 2000, 3, D, dtype, bits)
+    q = rnd((len(lens) * m, 3 * R * D), dtype, 9, 1.5)
+    check(attend(pkg, ctx, cache, q, tokens=m), q, held, lens, m)
+
+
 @pytest.mark.parametrize("D", [32, 64, 96, 128, 256])
 @pytest.mark.parametrize("bits", BITS)
 @pytest.mark.parametrize("cluster,m,R", [(-1, 1, 16), (2, 5, 5), (1, 1, 3)])
