@@ -62,8 +62,12 @@ bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& pla
     plan.pairs = heads * plan.col_tiles;
     if (plan.pairs > 0x7fffffff) return false;
     // A cluster of 1 - 8 CTAs for each pair, or one run of tiles per CTA that is there.  In tokens that a CTA gets through in the time: setting
-    // up and finishing a CTA is about 430, putting a cluster's results together 150, finding and cutting a run 1000.
-    const int64_t runs = 1000 + plan.pairs * most / at_once;
+    // up and finishing a CTA is about 430, putting a cluster's results together 150, finding and cutting a run 1000 and each piece of a pair, which one CTA
+    // puts together, another 10: so few pairs are cut into no more pieces than pay (one pair of 131072 tokens: 27 us in 115 pieces, 43 in 296; of
+    // 8192: 12.5 in 29, 35.6 in 296; 320 pairs of 400: 18.8 in runs, 14.4 as they are).
+    const int64_t pieces = static_cast<int64_t>(sqrt(most / 10.0)) + 1;
+    const int run_ctas = static_cast<int>(std::min<int64_t>(at_once, plan.pairs * pieces));
+    const int64_t runs = 1000 + plan.pairs * (most + 16 * kPairCost) / run_ctas + 10 * run_ctas / plan.pairs;
     int64_t best = 0;
     for (int size = 1; size <= kMostCluster; ++size) {
         const int64_t places = cluster_places(size), waves = (plan.pairs + places - 1) / places;
@@ -78,7 +82,7 @@ bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& pla
     if (forced < 0 && countable) plan.cluster = 0;
     plan.workspace = 0;
     if (plan.cluster == 0) {
-        plan.ctas = at_once;
+        plan.ctas = run_ctas;
         plan.workspace = tickets_at(plan, c) + static_cast<size_t>(plan.pairs) * sizeof(unsigned long long);
     } else {
         if (plan.pairs * plan.cluster > 0x7fffffff) return false;

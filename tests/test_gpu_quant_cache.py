@@ -303,6 +303,16 @@ def test_sixteen_columns(pkg, ctx, tune, D, bits, cluster, m, R):
     check(attend(pkg, ctx, cache, q, tokens=m), q, held, lens, m)
 
 
+@pytest.mark.parametrize("lens", [[5000], [7001, 3], [0, 1], [16]])
+@pytest.mark.parametrize("dtype,bits,D", [(BF, (4, 4), 128), (F32, (8, 4), 64)])
+def test_few_pairs_in_even_pieces(pkg, ctx, tune, lens, dtype, bits, D):
+    """Fewer pieces than CTAs that are there."""
+    tune("qcache_cluster", -1)
+    cache, held = filled(pkg, ctx, lens, max(lens) + 1, 1, D, dtype, bits)
+    q = rnd((len(lens), 3 * D), dtype, 9, 2.0)
+    check(attend(pkg, ctx, cache, q), q, held, lens, 1)
+
+
 def test_more_sequences_than_threads(pkg, ctx, tune):
     """Runs over 500 sequences: every thread of a CTA adds up several."""
     lens = [(7 * i) % 61 for i in range(500)]
