@@ -1199,19 +1199,22 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
                 x[0] = x[1] = x[2] = x[3] = 0.0f;
                 kept_lse[r * kPer + k] = kNegInf;
                 if ((kQuads % kThreads == 0 || i < kQuads) && col < used) {
-                    float top = kNegInf, total = 0.0f;
+                    // (shares of 1 are what results are multiplied by: sums of exponentials times the type's largest values are not finite)
+                    float top = kNegInf, total = 0.0f, share[W];
 #pragma unroll
                     for (int j = 0; j < W; ++j) top = fmaxf(top, ml[(j * A::kCols + col) * 2]);
 #pragma unroll
                     for (int j = 0; j < W; ++j) {
-                        const float l = ml[(j * A::kCols + col) * 2 + 1] * ex2(ml[(j * A::kCols + col) * 2] - top);
-                        const float4 y = *reinterpret_cast<const float4*>(smem + left_at[j] + (in_round * D + d) * 4);
-                        total += l;
-                        x[0] += l * y.x, x[1] += l * y.y, x[2] += l * y.z, x[3] += l * y.w;
+                        share[j] = ml[(j * A::kCols + col) * 2 + 1] * ex2(ml[(j * A::kCols + col) * 2] - top);
+                        total += share[j];
                     }
                     const float by = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] *= by;
+                    for (int j = 0; j < W; ++j) {
+                        const float l = share[j] * by;
+                        const float4 y = *reinterpret_cast<const float4*>(smem + left_at[j] + (in_round * D + d) * 4);
+                        x[0] += l * y.x, x[1] += l * y.y, x[2] += l * y.z, x[3] += l * y.w;
+                    }
                     kept_lse[r * kPer + k] = total == 0.0f ? kNegInf : top + log2f(total);
                     if (whole) {
                         A::store(A::out_row(p, b, g, ct * A::kCols + col) + d, x);
@@ -1249,7 +1252,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
                 const int quad = i * p.cluster + rank, col = quad / (D / 4), d = (quad - col * (D / 4)) * 4;
                 float top = kNegInf, total = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 for (int j = 0; j < p.cluster; ++j) top = fmaxf(top, lse[j * A::kCols + col]);
-                const float ref = top == kNegInf ? 0.0f : top;
+                const float ref = (top == kNegInf ? 0.0f : top) + 3.0f;  // (weights of 1 / 8 at most: sums of up to 8 results are finite)
                 for (int j = 0; j < p.cluster; ++j) {
                     const float l = ex2(lse[j * A::kCols + col] - ref);
                     const float4 y = *reinterpret_cast<const float4*>(smem + where(j * each + i));
@@ -1289,7 +1292,9 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
             if (n > 0) {
                 for (int i = threadIdx.x; i < used * (D / 4); i += kThreads) {
                     const int col = i / (D / 4), d = (i - col * (D / 4)) * 4;
-                    // the pieces' results in the order of the tokens, each taken relative to the largest so far
+                    // the pieces' results in the order of the tokens, each taken relative to the largest so far; weights are 2^-kDown at most, so that sums
+                    // of up to 2^kDown results are finite
+                    constexpr float kDown = 12.0f;
                     float top = kLowest, total_weight = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     for (int j0 = 0; j0 < n; j0 += 4) {
                         float lse[4];
@@ -1309,7 +1314,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
                         for (int e = 0; e < 4; ++e) x[e] *= by;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const float l = ex2(lse[j] - top);
+                            const float l = ex2(lse[j] - top - kDown);
                             total_weight += l;
                             if (j0 + j < n) x[0] += l * y[j].x, x[1] += l * y[j].y, x[2] += l * y[j].z, x[3] += l * y[j].w;
                         }
