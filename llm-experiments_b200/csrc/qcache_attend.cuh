@@ -17,12 +17,17 @@
 //     layout gives a lane the codes that it needs as one piece, the query is permuted to match, and P goes from the accumulator's
 //     layout to the operand's by an 8 x 8 transpose within the warp.  The rows go through tcgen05 only if they were first widened into
 //     shared memory at 16 bits per element, which is four times the traffic of reading them; as register operands they are widened in place.
-//   * A probability is rounded to fp16, multiplied by its value scale there and rounded again (11 bits; the output has 8).  To keep that in range
-//     whatever the scales are, they are taken relative to the largest exponent so far, and the accumulators are rescaled when that
-//     grows: products stay below 2^15, and scales down to 2^-17 of the largest keep all their bits.
+//   * A probability is rounded to fp16, multiplied by its value scale there and rounded again (11 bits; the output has 8).  fp16 has room for that as
+//     long as a group's scales are of a size: each group (of a warp's tokens of a pair) has a reference exponent, and a scale goes this way if it lies within
+//     2^-8 .. 2 of it.  The weight is 2^14 at most and 2^10 where it is the largest, so that products stay below 2^15, and a product below 2^-14, where
+//     bits are lost, is one whose weight is below 2^-16 of the largest.
+//   * What lies outside (a group whose tokens differ by more, a large value that no query gives any weight) is seldom there and goes another way: weight times
+//     scale in fp32, as a sum of bfloat16 parts, which have fp32's range, by as many more products.  So no element depends on what lies in other groups, nor on
+//     tokens that it does not see.  The reference moves, and the accumulators with it, where more than half of a group's scales in a stage lie outside; it
+//     stays within 2^64 of the largest, so that sums are finite.
 //   * fp32 queries and weights are sums of two fp16 numbers (22 bits), in columns of their own (four pairs of them to a tile of eight); keys are centred like values; and only 16 tokens'
 //     products are added up in the tensor core, whose sums are cut off and not rounded.
-//   * Softmax: scores in the log2 domain, references that move only when a score has outgrown its own by more than 2^8 (one vote per stage), sums per
+//   * Softmax: scores in the log2 domain, references that move only when a score has outgrown its own by more than 2^4 (one vote per stage), sums per
 //     lane until the end, all in fp32.
 #pragma once
 
@@ -56,7 +61,6 @@ struct AttendParams {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLowest = -3.0e38f;  // a reference where nothing was seen yet: any score has outgrown it, and differences stay finite
-constexpr int kScaleExpMin = 17;  // (biased) smaller exponents of value scales are taken for this one: 2^-110
 
 __device__ __forceinline__ int lane_id() {
     int lane;
@@ -210,8 +214,12 @@ struct Attend {
     static constexpr int kSG = scale_row(NG), kOffs = kF32 ? 1 : kSG == 8 ? 4 : 2;
     static constexpr int kKOff = KB == 4 ? 8 : 128;  // what is added to a key's code
     static constexpr float kKeyUnit = (KB == 4 ? 4.0f : 1.0f) * (kF32 ? 1.0f : 0x1p-24f);
-    // Weights are probabilities times 2^kShift, up to 2^(8 + kShift); times a value scale, 2^(6 - exponent) times that at most: below 2^15.
-    static constexpr int kShift = kF32 ? 0 : 3;
+    // Weights are probabilities (relative to the largest) times 2^kShift, up to 2^(kLag + kShift); value scales relative to their reference are below 2: products
+    // below 2^15.
+    static constexpr int kShift = 10, kLag = 4;
+    // Scales from 2^-kSpan of the reference to twice the reference go through fp16; a new reference is kHeadroom above the scales that it was made for; one
+    // is never more than kReach below the largest scale: sums stay below 2^(kReach + 15 + kHeadroom) * 127 * 2^30 tokens.
+    static constexpr int kSpan = 8, kHeadroom = 2, kReach = 64;
     static constexpr float kValueUnit = VB == 4 ? 4.0f : 1.0f;  // of a code of one; every other row of 4 bits has 16 times that
 
     // Where 16-byte piece ch of row r lies in a stage: moved about so that the lanes that read together meet different banks.
@@ -264,8 +272,16 @@ struct Attend {
         float o[NT][NG * 2][4];    // elements 32 (j / 2) + 4 gid + 2 (j & 1) (+1 in the last two), columns 2 tig, 2 tig + 1
         float ref[NT][2];          // scores are taken relative to this: what was the largest so far, less kShift
         float sum[NT][2];          // of 2^(score - ref), this lane's tokens
-        int scale_exp;
         bool fresh;                // some column may not have seen anything yet
+    };
+
+    // What value scales of the warp's present pair are relative to, in shared memory: one over the reference of each group (a power of two; 0 where no stage has
+    // been seen yet), and the largest (biased) exponent that has gone into the accumulators.
+    struct Refs {
+        float by[kSG];
+        int most[kSG];
+        __device__ __forceinline__ int exponent(int u) const { return 254 - (__float_as_int(by[u]) >> 23); }
+        __device__ __forceinline__ void set(int u, int e, int m) { by[u] = __int_as_float((254 - e) << 23), most[u] = m; }
     };
 
     // fp32: the second half of a tile is for the same columns as the first, and lanes 2 apart (in tig) have the same scores.
@@ -299,7 +315,7 @@ struct Attend {
     }
 
     // The CTA's part in it (two barriers), then the warp's own.  n: tokens of the sequence.
-    __device__ static __forceinline__ void begin(const AttendParams& p, Warp& w, const Query& raw, Prepared& q, int g, int ct, int n) {
+    __device__ static __forceinline__ void begin(const AttendParams& p, Warp& w, Refs& refs, const Query& raw, Prepared& q, int g, int ct, int n) {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3, warp = threadIdx.x >> 5;
         float x[kUnitsEach][8];
 #pragma unroll
@@ -398,7 +414,7 @@ struct Attend {
             for (int e = 0; e < 2; ++e) w.ref[nt][e] = kLowest, w.sum[nt][e] = 0.0f;
         }
         w.fresh = true;
-        w.scale_exp = kScaleExpMin;
+        if (lane < kSG) refs.by[lane] = 0.0f;
     }
 
     // Where a lane's token of a tile lies: its row, -1 where there is none or no query sees it.
@@ -530,7 +546,8 @@ struct Attend {
     }
 
     // The tokens of a stage, t0 the first.
-    __device__ static __forceinline__ void fold(const AttendParams& p, const Lane& l, Warp& w, const Prepared& prepared, uint32_t stage, int t0, uint32_t there) {
+    __device__ static __forceinline__ void fold(const AttendParams& p, const Lane& l, Warp& w, Refs& refs, const Prepared& prepared, uint32_t stage, int t0,
+                                                uint32_t there) {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         const uint32_t ks = stage + kKBytes + kVBytes, vs = ks + kSBytes;
         constexpr int kKPiece = NG * KB;   // bytes of a row that a lane reads
@@ -640,7 +657,7 @@ struct Attend {
                         s[h][nt][e] = fmaf(s[h][nt][e], w.f[nt][e & 1], -w.ref[nt][e & 1]);
                         most = fmaxf(most, s[h][nt][e]);
                     }
-            move = __any_sync(~0u, most > 8.0f + kShift);
+            move = __any_sync(~0u, most > static_cast<float>(kLag + kShift));
             if (move) {
 #pragma unroll
                 for (int h = 0; h < MT; ++h)
@@ -697,66 +714,191 @@ struct Attend {
                     s[h][nt][e + 2] = ex2(s[h][nt][e + 2]);
                     w.sum[nt][e] += s[h][nt][e] + s[h][nt][e + 2];
                 }
-        // The largest exponent of a value scale so far (NaN groups have none).
+        // Value scales relative to their references; a vote on whether all lie where fp16 holds them (zeros do).
         Words<kSRow> mine;
         mine.load(vs + (lane & (kTok - 1)) * kSRow);
-        uint32_t most = mine.w[0];
+        float x[kSG];
+        if (refs.by[0] == 0.0f) first_refs(refs, mine);
+        if (__any_sync(~0u, relative(refs, mine, x))) {
+            far_scales(w, refs, stage, s, hidden, mine);
+            relative(refs, mine, x);
+        }
+        if constexpr (kF32)
+            values_f32(l, w, stage, s, x);
+        else
+            values_bf16(l, w, stage, s, x);
+    }
+
+    // x = a token's scales relative to their references (exact); whether one lies outside 2^-kSpan .. 2 and is not zero.
+    __device__ static __forceinline__ bool relative(const Refs& refs, const Words<kSRow>& mine, float (&x)[kSG]) {
+        constexpr uint32_t kLeast = (127 - kSpan) << 23, kMost = 128 << 23;
+        uint32_t least = ~0u, most = 0;
 #pragma unroll
-        for (int i = 1; i < kSG / 2; ++i) most = __vmaxu2(most, mine.w[i]);
-        most = __reduce_max_sync(~0u, max(most >> 16, most & 0xffffu));
-        if (most >= 0x7f80u) {
-            // Groups of NaN spoil their elements of the columns that see their token, and take no part in the products, which know neither.
+        for (int u = 0; u < kSG; ++u) {
+            x[u] = __uint_as_float(u & 1 ? mine.w[u >> 1] & 0xffff0000u : mine.w[u >> 1] << 16) * refs.by[u];
+            least = min(least, __float_as_uint(x[u]) - 1);
+            most = max(most, __float_as_uint(x[u]));
+        }
+        return least < kLeast - 1 || most >= kMost;
+    }
+
+    // The references of a pair's first stage: a little above its largest scales.  (All lanes write the same.)
+    __device__ static __forceinline__ void first_refs(Refs& refs, const Words<kSRow>& mine) {
+        __syncwarp();
 #pragma unroll
-            for (int u = 0; u < NG; ++u) {
-                const uint32_t y = u & 1 ? mine.w[u >> 1] >> 16 : mine.w[u >> 1] & 0xffffu;
-                const uint32_t bad = __ballot_sync(~0u, y >= 0x7f80u);  // a bit per token
-                mine.w[u >> 1] &= y < 0x7f80u ? ~0u : u & 1 ? 0x0000ffffu : 0xffff0000u;
+        for (int u = 0; u < kSG; ++u) {
+            const uint32_t y = u & 1 ? mine.w[u >> 1] >> 16 : mine.w[u >> 1] & 0xffffu;
+            const int e = static_cast<int>(__reduce_max_sync(~0u, y < 0x7f80u ? y : 0u) >> 7) + kHeadroom;
+            refs.set(u, min(max(e, 1), 253), e);
+        }
+        __syncwarp();
+    }
+
+    // A stage with scales outside their references' range, or NaN ones.  References move where most of a group's scales lie outside; what lies outside all
+    // the same is multiplied here, and `mine` keeps the rest.  Groups of NaN spoil their elements of the columns that see their token.
+    // (A loop over the groups that is not unrolled: it is run seldom, and should take neither registers nor instruction cache.)
+    __device__ static __forceinline__ void far_scales(Warp& w, Refs& refs, uint32_t stage, const float (&weight)[MT][NT][4], uint32_t hidden, Words<kSRow>& mine) {
+        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
+#pragma unroll 1
+        for (int u = 0; u < NG; ++u) {
+            uint32_t y = mine.w[0];
+#pragma unroll
+            for (int i = 1; i < kSG / 2; ++i) y = (u >> 1) == i ? mine.w[i] : y;
+            y = u & 1 ? y >> 16 : y & 0xffffu;
+            const uint32_t bad = __ballot_sync(~0u, y >= 0x7f80u);  // a bit per token, like those below
+            y = y >= 0x7f80u ? 0u : y;
+            const int e = y != 0 ? max(static_cast<int>(y >> 7), 1) : 0, old = refs.exponent(u);
+            const auto outside = [&](int ref) { return e != 0 && (e > ref || e + kSpan < ref); };
+            const int largest = static_cast<int>(__reduce_max_sync(~0u, static_cast<uint32_t>(e)));
+            const int largest_outside = static_cast<int>(__reduce_max_sync(~0u, outside(old) ? static_cast<uint32_t>(e) : 0u));
+            const bool moves = 2 * __popc(__ballot_sync(~0u, outside(old))) > __popc(__ballot_sync(~0u, e != 0));
+            const int most = max(max(refs.most[u], old), largest);
+            const int now = max(moves ? min(largest_outside + kHeadroom, 253) : old, most - kReach);
+            const uint32_t far = __ballot_sync(~0u, outside(now));
+            const float x = outside(now) ? __uint_as_float(y << 16) * __int_as_float((254 - now) << 23) : 0.0f;
+            __syncwarp();
+            refs.set(u, now, most);
+            __syncwarp();
+            float add[NT][2][4] = {};
+            if (far != 0) far_products(stage, weight, u, x, add);
+            if (bad != 0) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
+                    for (int c = 0; c < 2; ++c) {
                         bool spoilt = false;
 #pragma unroll
                         for (int h = 0; h < MT; ++h)
 #pragma unroll
                             for (int i = 0; i < 2; ++i)
-                                spoilt = spoilt || (((bad >> (h * 16 + i * 8 + gid)) & 1u) && !((hidden >> ((h * NT + nt) * 4 + i * 2 + e)) & 1u));
+                                spoilt = spoilt || (((bad >> (h * 16 + i * 8 + gid)) & 1u) && !((hidden >> ((h * NT + nt) * 4 + i * 2 + c)) & 1u));
                         const uint32_t lanes = __ballot_sync(~0u, spoilt);
-                        const float add = ((lanes >> tig) & 0x11111111u) != 0 ? __int_as_float(0x7fc00000) : 0.0f;
+                        const float nan = ((lanes >> tig) & 0x11111111u) != 0 ? __int_as_float(0x7fc00000) : 0.0f;
 #pragma unroll
-                        for (int j = 2 * u; j < 2 * u + 2; ++j) w.o[nt][j][e] += add, w.o[nt][j][e + 2] += add;
+                        for (int j = 0; j < 2; ++j) add[nt][j][c] += nan, add[nt][j][c + 2] += nan;
                     }
             }
-            most = mine.w[0];
-#pragma unroll
-            for (int i = 1; i < kSG / 2; ++i) most = __vmaxu2(most, mine.w[i]);
-            most = __reduce_max_sync(~0u, max(most >> 16, most & 0xffffu));
-        }
-        const int now = static_cast<int>(most >> 7);
-        if (now > w.scale_exp) {
-            const float by = w.scale_exp - now < -126 ? 0.0f : __int_as_float((127 + w.scale_exp - now) << 23);
-            w.scale_exp = now;
+            // 2^(old - now) in two factors, each of them a normal number
+            const int half = (old - now) / 2;
+            const float by0 = __int_as_float((127 + half) << 23), by1 = __int_as_float((127 + old - now - half) << 23);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < NG * 2; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) w.o[nt][j][e] *= by;
+                    for (int c = 0; c < 4; ++c) w.o[nt][j][c] = (j >> 1) == u ? fmaf(w.o[nt][j][c] * by0, by1, add[nt][j & 1][c]) : w.o[nt][j][c];
+            y = outside(now) ? 0u : y;
+#pragma unroll
+            for (int i = 0; i < kSG / 2; ++i)
+                mine.w[i] = (u >> 1) != i ? mine.w[i] : u & 1 ? (mine.w[i] & 0xffffu) | y << 16 : (mine.w[i] & 0xffff0000u) | y;
         }
-        if constexpr (kF32)
-            values_f32(l, w, stage, s, mine);
-        else
-            values_bf16(l, w, stage, s, mine);
+    }
+
+    // add = the products of group u's codes with weights times x, a scale per lane's token (0: no part in this): bfloat16 numbers, which hold codes as they
+    // are, and weights times scales as sums of two (fp32: three, the second in the tile's other half and the third in a product of its own).
+    __device__ static __forceinline__ void far_products(uint32_t stage, const float (&weight)[MT][NT][4], int u, float x, float (&add)[NT][2][4]) {
+        const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
+        const float rest = kF32 && tig >= 2 ? 1.0f : 0.0f;  // (a number and no branch, as below)
+        const auto pack = [](float lo, float hi) {
+            const __nv_bfloat162 both = __floats2bfloat162_rn(lo, hi);
+            return *reinterpret_cast<const uint32_t*>(&both);
+        };
+        const auto less = [](uint32_t y, float by, float& lo, float& hi) {
+            lo = fmaf(-by, __uint_as_float(y << 16), lo), hi = fmaf(-by, __uint_as_float(y & 0xffff0000u), hi);
+        };
+        const int at = gid * (NG * VB / 2) + u * (VB / 2);
+#pragma unroll
+        for (int h = 0; h < MT; ++h) {
+            struct Piece {
+                uint32_t w[1];
+            } v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = h * 16 + (i >> 1) * 8 + 2 * tig + (i & 1);
+                const uint32_t from = stage + kKBytes + (NG == 3 ? r * kVRow + at : v_place(r, at / 16) + at % 16);
+                if constexpr (VB == 4) {
+                    uint16_t y;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(from) : "memory");
+                    v[i].w[0] = y;
+                } else {
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[i].w[0]) : "r"(from) : "memory");
+                }
+            }
+            uint32_t a[2][4];
+            v_pieces(v, 0, a);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 y = unpack_half(a[j][i]);
+                    a[j][i] = pack(y.x, y.y);
+                }
+            const float f0 = __shfl_sync(~0u, x, h * 16 + gid), f1 = __shfl_sync(~0u, x, h * 16 + 8 + gid);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float y[4] = {weight[h][nt][0] * f0, weight[h][nt][1] * f0, weight[h][nt][2] * f1, weight[h][nt][3] * f1};
+                uint32_t b[2][2];  // [part][tokens gid or gid + 8]
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t first = pack(y[2 * i], y[2 * i + 1]);
+                    if constexpr (kF32) {
+                        less(first, rest, y[2 * i], y[2 * i + 1]);
+                        b[0][i] = pack(y[2 * i], y[2 * i + 1]);
+                        less(first, 1.0f - rest, y[2 * i], y[2 * i + 1]);
+                        less(pack(y[2 * i], y[2 * i + 1]), 1.0f, y[2 * i], y[2 * i + 1]);
+                        b[1][i] = pack(y[2 * i] * (1.0f - rest), y[2 * i + 1] * (1.0f - rest));
+                    } else {
+                        b[0][i] = first;
+                        less(first, 1.0f, y[2 * i], y[2 * i + 1]);
+                        b[1][i] = pack(y[2 * i], y[2 * i + 1]);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    b[k][0] = transpose8x8(b[k][0]), b[k][1] = transpose8x8(b[k][1]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float d[4] = {};
+                        mma_bf16(d, a[j][0], a[j][1], a[j][2], a[j][3], b[k][0], b[k][1]);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) add[nt][j][c] += d[c];
+                    }
+                }
+            }
+        }
     }
 
     // O += V^T P for fp32: weights times value scales in 32 bits, then as two fp16 numbers.
-    __device__ static __forceinline__ void values_f32(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NT][4], const Words<kSRow>& mine) {
+    __device__ static __forceinline__ void values_f32(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NT][4], const float (&x)[kSG]) {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
-        const float vf = __int_as_float((260 - w.scale_exp) << 23);  // 2^(6 - exponent)
         // (A number, and no branch on the lane: the compiler may lay such a branch around what follows, and instructions of the whole warp are among it.)
         const float rest = tig >= 2 ? 1.0f : 0.0f;
+        // scales relative to their references, bfloat16 numbers as before, in place
+        Words<kSRow> mine;
+#pragma unroll
+        for (int i = 0; i < kSG / 2; ++i) mine.w[i] = __byte_perm(__float_as_uint(x[2 * i]), __float_as_uint(x[2 * i + 1]), 0x7632);
         __syncwarp();
-        mine.store(stage + kKBytes + kVBytes + kSBytes + (lane & (kTok - 1)) * kSRow);  // (without the groups of NaN)
+        mine.store(stage + kKBytes + kVBytes + kSBytes + (lane & (kTok - 1)) * kSRow);
         __syncwarp();
         const uint32_t vs = stage + kKBytes + kVBytes + kSBytes;
         const uint32_t values_at[2] = {stage + kKBytes + l.v, stage + kKBytes + l.v_next()};
@@ -771,13 +913,13 @@ struct Attend {
             for (int i = 0; i < 4; ++i) load_v(v[i], values_at[i & 1], h * 16 + (i >> 1) * 8);
 #pragma unroll
             for (int u = 0; u < NG; ++u) {
-                const float f0 = vf * __uint_as_float(u & 1 ? s0.w[u >> 1] & 0xffff0000u : s0.w[u >> 1] << 16);
-                const float f1 = vf * __uint_as_float(u & 1 ? s1.w[u >> 1] & 0xffff0000u : s1.w[u >> 1] << 16);
-                float x[4] = {weight[h][0][0] * f0, weight[h][0][1] * f0, weight[h][0][2] * f1, weight[h][0][3] * f1};
+                const float f0 = __uint_as_float(u & 1 ? s0.w[u >> 1] & 0xffff0000u : s0.w[u >> 1] << 16);
+                const float f1 = __uint_as_float(u & 1 ? s1.w[u >> 1] & 0xffff0000u : s1.w[u >> 1] << 16);
+                const float y[4] = {weight[h][0][0] * f0, weight[h][0][1] * f0, weight[h][0][2] * f1, weight[h][0][3] * f1};
                 // lanes of the second half have what fp16 leaves: less `rest` times the rounded number, and rounded again
-                const float2 g0 = unpack_half(pack_half(x[0], x[1])), g1 = unpack_half(pack_half(x[2], x[3]));
-                const uint32_t b0 = transpose8x8(pack_half(fmaf(-rest, g0.x, x[0]), fmaf(-rest, g0.y, x[1])));
-                const uint32_t b1 = transpose8x8(pack_half(fmaf(-rest, g1.x, x[2]), fmaf(-rest, g1.y, x[3])));
+                const float2 g0 = unpack_half(pack_half(y[0], y[1])), g1 = unpack_half(pack_half(y[2], y[3]));
+                const uint32_t b0 = transpose8x8(pack_half(fmaf(-rest, g0.x, y[0]), fmaf(-rest, g0.y, y[1])));
+                const uint32_t b1 = transpose8x8(pack_half(fmaf(-rest, g1.x, y[2]), fmaf(-rest, g1.y, y[3])));
                 uint32_t a[2][4];
                 v_pieces(v, u, a);
 #pragma unroll
@@ -792,17 +934,16 @@ struct Attend {
     }
 
     // O += V^T P for bfloat16: weights go to the operand's layout as fp16 numbers and meet the value scales there, two per instruction.  The scales
-    // are made fp16 (relative to the largest exponent) and brought into that order by the lane that has the token, in place.
-    __device__ static __forceinline__ void values_bf16(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NT][4], const Words<kSRow>& mine) {
+    // are made fp16 (relative to their references, which is exact) and brought into that order by the lane that has the token, in place.
+    __device__ static __forceinline__ void values_bf16(const Lane& l, Warp& w, uint32_t stage, const float (&weight)[MT][NT][4], const float (&x)[kSG]) {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
         constexpr int kWords = kSG / 2;
         const uint32_t vs = stage + kKBytes + kVBytes + kSBytes;
         const uint32_t values_at[2] = {stage + kKBytes + l.v, stage + kKBytes + l.v_next()};
         {
-            const float vf = __int_as_float((257 - w.scale_exp) << 23);  // 2^(6 - kShift - exponent)
             uint32_t c[kWords];
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) c[i] = pack_half(__uint_as_float(mine.w[i] << 16) * vf, __uint_as_float(mine.w[i] & 0xffff0000u) * vf);
+            for (int i = 0; i < kWords; ++i) c[i] = pack_half(x[2 * i], x[2 * i + 1]);
             const bool odd = lane & 1;
             const int r = lane & (kTok - 1);
             const uint32_t to = vs + (((r >> 4) * 4 + ((r & 7) >> 1)) * 2 + ((r >> 3) & 1)) * (kSG * 4);
@@ -918,18 +1059,18 @@ struct Attend {
             }
     }
     // Its normalised result for columns c0 .. c0 + kRoundCols - 1 into o [kRoundCols][D].
-    __device__ static __forceinline__ void leave(const Warp& w, uint32_t o, int c0) {
+    __device__ static __forceinline__ void leave(const Warp& w, const Refs& refs, uint32_t o, int c0) {
         const int lane = lane_id(), gid = lane >> 2, tig = lane & 3;
-        // the accumulators are in units of 2^(exponent - 6) kValueUnit, the sums in units of 2^-kShift
-        const float up = __int_as_float(w.scale_exp << 23);
+        // the accumulators are in units of their group's reference times kValueUnit, and of 2^-kShift like the sums
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int col = col_of(nt, 2 * tig + e) - c0;
-                const float sum = w.sum[nt][e], by = sum == 0.0f ? 0.0f : __frcp_rn(sum) * ((kF32 ? 0x1p-6f : 0x1p-3f) / kValueUnit);
+                const float sum = w.sum[nt][e], by = sum == 0.0f ? 0.0f : __frcp_rn(sum) * (1.0f / kValueUnit);
 #pragma unroll
                 for (int u = 0; u < NG; ++u) {
+                    const float up = __int_as_float(refs.exponent(u) << 23);
                     float x[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -1080,6 +1221,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
     auto& prepared = *reinterpret_cast<typename A::Prepared*>(smem + A::kRing + A::kMl + 16 * ((W * 4 + 15) / 16));
     __shared__ Place<kTok> now[W], ahead[W];
     __shared__ uint32_t there[W][S];  // which tokens of a stage are there
+    __shared__ typename A::Refs refs[W];
     __shared__ int pieces[3];
     const int warp = threadIdx.x >> 5;
     const uint32_t ring = smem_u32(smem) + warp * S * A::kStage;
@@ -1160,12 +1302,12 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
     for (;;) {
         int t = now[warp].first + now[warp].tile * kTok + skip;
         const int end = now[warp].first + now[warp].end * kTok;
-        A::begin(p, q, raw, prepared, now[warp].g, now[warp].ct, now[warp].n);
+        A::begin(p, q, refs[warp], raw, prepared, now[warp].g, now[warp].ct, now[warp].n);
         for (; t < end; t += step) {
             copy_wait<S - 2>();
             __syncwarp();
             copy(slot == 0 ? S - 1 : slot - 1);
-            A::fold(p, l, q, prepared, ring + slot * A::kStage, t, there[warp][slot]);
+            A::fold(p, l, q, refs[warp], prepared, ring + slot * A::kStage, t, there[warp][slot]);
             slot = slot == S - 1 ? 0 : slot + 1;
         }
         if (p.cluster > 1) {
@@ -1189,7 +1331,7 @@ __global__ void __launch_bounds__(Ring<NG, KB, VB, NT>::kWarps * 32, Ring<NG, KB
         float kept_lse[A::kRounds * kPer];
 #pragma unroll
         for (int r = 0; r < A::kRounds; ++r) {
-            A::leave(q, smem_u32(smem) + mine, r * A::kRoundCols);
+            A::leave(q, refs[warp], smem_u32(smem) + mine, r * A::kRoundCols);
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < kPer; ++k) {

@@ -80,3 +80,24 @@ def tolerance(out, mean, size, n, dtype: str, extra: float = 0.0, largest: float
     score = 34 * (2.0 ** -20 * 15 / 7 if bf16 else 2.0 ** -24) * size + extra
     summed = 2.0 ** -23 * (n / 16 + 32) * mean
     return half * np.abs(out) + (held_in + 2 * score) * mean + summed + n * 2.0 ** -31 * largest
+
+
+def largest_seen(v, m, H, window=0):
+    """Per query and head, of each element's group: the largest magnitude held among the tokens that the query sees.  v [n, G, D] -> [m, H, D]."""
+    n, G, D = v.shape
+    most = np.repeat(np.abs(np.nan_to_num(v)).reshape(n, G, -1, GROUP).max(-1), GROUP, axis=-1)
+    out = np.zeros((m, H, D))
+    for i in range(m):
+        p = n - m + i
+        if p >= 0:
+            out[i] = np.repeat(most[max(0, p + 1 - window) if window else 0:p + 1].max(0), H // G, axis=0)
+    return out
+
+
+def tolerance_seen(out, mean, size, n, dtype: str, largest, extra: float = 0.0):
+    """`tolerance` with nothing allowed for groups and tokens that an element has nothing to do with: `largest` is what `largest_seen` gives.
+    Where fp16 numbers are used for a token, its value scale lies within 2^9 of its group's reference 2^E, and its weight is relative to a sum of
+    2^10 at least.  Below 2^-14 weight and product are each off by up to 2^-25, the weight's times a scale below 2: 3 * 2^-25 * 2^-10 * 2^E * L,
+    and a token that is seen makes L 2^E at most 2^8 * largest: 3 * 2^-27 = 48 * 2^-31 of it per token.  Other tokens' products are sums of 16 bits
+    (fp32: 24), which the relative terms cover."""
+    return tolerance(out, mean, size, n, dtype, extra, 48.0 * largest)
