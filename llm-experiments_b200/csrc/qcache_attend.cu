@@ -125,7 +125,8 @@ int b2kv_qcache_attend(const b2kv_qcache* cache, const b2kv_qcache_attend_args* 
     p.R = a.H / c.G, p.m = a.m, p.col_tiles = plan.col_tiles, p.T_upper = a.T_upper, p.len_bias = a.len_bias;
     p.window = static_cast<int>(std::min<int64_t>(a.window, static_cast<int64_t>(a.T_upper) + a.m));  // (no sum with it overflows)
     p.cluster = plan.cluster;
-    p.scale = a.scale, p.softcap = a.softcap;
+    p.scale = static_cast<float>(frexp(static_cast<double>(a.scale) * M_LOG2E, &p.scale_exp));
+    p.softcap = a.softcap;
     p.ws_o = static_cast<float*>(workspace);
     p.ws_lse = p.ws_o + static_cast<size_t>(plan.ctas) * 2 * plan.cols * c.D;
     p.tickets = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + tickets_at(plan, c));

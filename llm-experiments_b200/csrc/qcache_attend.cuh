@@ -55,7 +55,9 @@ struct AttendParams {
     int64_t ld_q, ld_out;
     int R, m, col_tiles, T_upper, len_bias, window;
     int cluster;      // > 0: a cluster of this many CTAs per (sequence, head, column tile); 0: all tokens laid end to end and cut into gridDim.x pieces
-    float scale, softcap;
+    float scale;        // scale * log2 e = scale * 2^scale_exp
+    int scale_exp;
+    float softcap;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -213,7 +215,10 @@ struct Attend {
     // in three bfloat16 parts (16 places: part k / kSG of group k % kSG; with 8 groups in two products).
     static constexpr int kSG = scale_row(NG), kOffs = kF32 ? 1 : kSG == 8 ? 4 : 2;
     static constexpr int kKOff = KB == 4 ? 8 : 128;  // what is added to a key's code
-    static constexpr float kKeyUnit = (KB == 4 ? 4.0f : 1.0f) * (kF32 ? 1.0f : 0x1p-24f);
+    // A code of one in a score's sum, as a power of two: codes' own (fp16 numbers or subnormals), and in fp32, where that would let sums of large keys
+    // overflow, another 2^-16 that the key scales are multiplied by (a scale of 8 bits stays exact).
+    static constexpr int kKeyUnitExp = (KB == 4 ? 2 : 0) - (kF32 ? 16 : 24);
+    static constexpr float kKeyUnit = (KB == 4 ? 4.0f : 1.0f) * (kF32 ? 0x1p-16f : 0x1p-24f);
     // Weights are probabilities (relative to the largest) times 2^kShift, up to 2^(kLag + kShift); value scales relative to their reference are below 2: products
     // below 2^15.
     static constexpr int kShift = 10, kLag = 4;
@@ -262,12 +267,13 @@ struct Attend {
     struct Column {
         int lo, lim;  // it sees tokens lo <= t < lim
         float slope;  // log2 e times its slope
-        float f;      // a score is the product's sum times this (before a cap and a bias)
+        float f;      // a score is the product's sum times this (before a cap and a bias), and times Prepared::rest
     };
 
     struct Warp {
         uint32_t off[NT][kOffs];   // what the key's centre comes to, as the second operand of a product with the key scales (not for fp32)
-        float f[NT][2];            // the same where there is neither cap nor bias, else 1
+        float f[NT][2];            // Column::f where a score is the product's sum times it, else 1
+        int apart;                 // bits: 1 - scores are made apart from that (a cap, a bias, a factor beyond fp32), 2 - a factor beyond fp32
         int all_lo, all_lim;       // tokens that every used column sees
         float o[NT][NG * 2][4];    // elements 32 (j / 2) + 4 gid + 2 (j & 1) (+1 in the last two), columns 2 tig, 2 tig + 1
         float ref[NT][2];          // scores are taken relative to this: what was the largest so far, less kShift
@@ -293,9 +299,11 @@ struct Attend {
         uint32_t most[kUnits / NG][8][NG];  // largest magnitude of a column's group, as a whole number (NaN above infinity above all others)
         float sum[kUnits / NG][8][kSG];     // what the centre of its keys comes to
         Column columns[kCols];
+        float rest[kCols];                  // what the factor of a column's scores has beyond 2^-100 .. 2^100 (a power of two, nearly always 1)
         uint4 queries[NG * NT * 32];        // the second operand of S = K q, both steps of a group in one
     };
     static constexpr int kSmem = kRing + kMl + 16 * ((WARPS * 4 + 15) / 16) + static_cast<int>(sizeof(Prepared));
+    static_assert(kSmem <= 112 * 1024, "two CTAs per SM, and 1 KB for what has a fixed size");
     // A lane's part of them as they lie in memory: octet tig of its warp's groups, of column gid.
     struct Query {
         uint4 w[kUnitsEach][sizeof(T) / 2];
@@ -336,7 +344,7 @@ struct Attend {
             uint32_t most = q.most[nt][c][0];
 #pragma unroll
             for (int u = 1; u < NG; ++u) most = max(most, q.most[nt][c][u]);
-            return min(max(static_cast<int>(most >> 23), 27), 254);
+            return most == 0 ? 127 : min(max(static_cast<int>(most >> 23), 15), 254);
         };
 #pragma unroll
         for (int i = 0; i < kUnitsEach; ++i) {
@@ -370,8 +378,11 @@ struct Attend {
         if (threadIdx.x < kCols) {
             const int c = threadIdx.x, col = ct * kCols + c, i = col / p.R, place = n - p.m + i;
             const bool is = col < p.m * p.R;
-            // a score is scale * 2^(e - 14) over what a code of one is in the product
-            const float f = p.scale * kLog2e * 0x1p-14f / kKeyUnit * __int_as_float(exponent(c / 8, c % 8) << 23);
+            // a score is scale * 2^(e - 14) over what a code of one is in the product: queries, keys and scales of any size can make scores of an
+            // ordinary one, so this may be no fp32 number
+            const int power = p.scale_exp + exponent(c / 8, c % 8) - 127 - 14 - kKeyUnitExp, within = min(max(power, -100), 100);
+            const float f = p.scale * __int_as_float((127 + within) << 23);
+            q.rest[c] = is ? __int_as_float((127 + min(max(power - within, -126), 127)) << 23) : 1.0f;
             q.columns[c] = Column{is && p.window > 0 ? max(place + 1 - p.window, 0) : 0, is ? place + 1 : 0,
                                   is && p.slopes != nullptr ? p.slopes[g * p.R + col - i * p.R] * kLog2e : 0.0f, f};
         }
@@ -381,11 +392,12 @@ struct Attend {
         const bool is = ct * kCols + (lane & (kCols - 1)) < p.m * p.R;
         w.all_lim = __reduce_min_sync(~0u, is ? c.lim : 0x7fffffff);
         w.all_lo = __reduce_max_sync(~0u, is ? c.lo : 0);
-        const bool plain = p.softcap == 0.0f && p.slopes == nullptr;
+        const bool beyond = __any_sync(~0u, q.rest[lane & (kCols - 1)] != 1.0f);
+        w.apart = (beyond ? 2 : 0) | (beyond || p.softcap > 0.0f || p.slopes != nullptr ? 1 : 0);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) w.f[nt][e] = plain ? q.columns[col_of(nt, 2 * tig + e)].f : 1.0f;
+            for (int e = 0; e < 2; ++e) w.f[nt][e] = w.apart == 0 ? q.columns[col_of(nt, 2 * tig + e)].f : 1.0f;
             if constexpr (!kF32) {
                 // places 2 tig and 2 tig + 1 of every eight: two neighbouring groups, one of their three parts
                 constexpr int kPairs = kSG / 2;
@@ -592,8 +604,9 @@ struct Attend {
                     k_piece<1>(k[h][0].w + u * kW, a[1][0], a[1][2]);
                     k_piece<1>(k[h][1].w + u * kW, a[1][1], a[1][3]);
                     const uint32_t s0 = scales[h][0].w[u >> 1], s1 = scales[h][1].w[u >> 1];
-                    const float f0 = __uint_as_float(u & 1 ? s0 & 0xffff0000u : s0 << 16);
-                    const float f1 = __uint_as_float(u & 1 ? s1 & 0xffff0000u : s1 << 16);
+                    const float down = kF32 ? 0x1p-16f : 1.0f;
+                    const float f0 = __uint_as_float(u & 1 ? s0 & 0xffff0000u : s0 << 16) * down;
+                    const float f1 = __uint_as_float(u & 1 ? s1 & 0xffff0000u : s1 << 16) * down;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float d[4];
@@ -613,7 +626,7 @@ struct Attend {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[h][nt][e] = kF32 ? acc[h][nt][e] + __shfl_xor_sync(~0u, acc[h][nt][e], 2) : acc[h][nt][e];
         }
-        if (p.softcap > 0.0f || p.slopes != nullptr) {
+        if (w.apart != 0) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -622,6 +635,16 @@ struct Attend {
 #pragma unroll
                     for (int h = 0; h < MT; ++h) s[h][nt][e] *= f;
                 }
+            if (w.apart & 2) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float rest = prepared.rest[col_of(nt, 2 * tig + (e & 1))];
+#pragma unroll
+                        for (int h = 0; h < MT; ++h) s[h][nt][e] *= rest;
+                    }
+            }
             if (p.softcap > 0.0f) {
                 const float down = 1.0f / (p.softcap * kLog2e), up = p.softcap * kLog2e;
 #pragma unroll

@@ -1,5 +1,5 @@
 """Attention over a quantised cache at the ends of its inputs' ranges, against float64: values near the type's largest, groups and tokens whose
-values lie far apart, large values that no weight or no query reaches."""
+values lie far apart, large values that no weight or no query reaches, queries and keys at the ends of the type."""
 import numpy as np
 import pytest
 import torch
@@ -140,3 +140,24 @@ def test_values_near_the_largest_number(pkg, ctx, tune, dtype, D, bits, cluster,
     cache, held = holding(pkg, ctx, lens, T, k, v, D, dtype, bits)
     q = rnd((B, 2 * D), dtype, 3)
     check(attend(pkg, ctx, cache, q), q, held, lens, 1)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# queries
+# ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("bits,q_exp,k_exp,scale", [((4, 4), 119, -120, 1.0), ((8, 8), 117, -118, 1.0), ((4, 4), 124, -122, 0.18), ((8, 4), 124, -118, 2.0 ** -6),
+                                                    ((4, 4), -112, 112, 0.18), ((8, 8), -115, 115, 0.18), ((4, 4), 100, 20, 2.0 ** -122), ((8, 8), -90, -25, 2.0 ** 113)])
+@pytest.mark.parametrize("options", [{}, {"softcap": 20.0}, {"window": 40}])
+def test_queries_at_the_ends_of_the_type(pkg, ctx, dtype, bits, q_exp, k_exp, scale, options):
+    """Scores of ordinary size by the definition, from queries, keys and scales that are not."""
+    lens, T, D = [70, 300, 1], 300, 32
+    k, v = rnd((3 * T, D), dtype, 1), rnd((3 * T, D), dtype, 2)
+    k = times(k, torch.full(k.shape, k_exp))
+    cache, held = holding(pkg, ctx, lens, T, k, v, D, dtype, bits)
+    q = rnd((3, 3 * D), dtype, 9)
+    q[:, D:2 * D] = times(q[:, D:2 * D], torch.full((3, D), q_exp))
+    q[:, 2 * D:] = times(q[:, 2 * D:], torch.full((3, D), q_exp - 1))
+    q[:, :D] = 0.0                                                # (a head beside them whose scores are all 0)
+    check(attend(pkg, ctx, cache, q, scale=scale, **options), q, held, lens, 1, scale, extra=2.0 ** -22 * options.get("softcap", 0.0), **options)
