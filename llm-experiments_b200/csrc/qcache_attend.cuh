@@ -57,7 +57,7 @@ struct AttendParams {
     int cluster;      // > 0: a cluster of this many CTAs per (sequence, head, column tile); 0: all tokens laid end to end and cut into gridDim.x pieces
     float scale;        // scale * log2 e = scale * 2^scale_exp
     int scale_exp;
-    float softcap;
+    float cap, cap_inverse;  // the cap times log2 e, one over it; 0 without one
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -393,7 +393,7 @@ struct Attend {
         w.all_lim = __reduce_min_sync(~0u, is ? c.lim : 0x7fffffff);
         w.all_lo = __reduce_max_sync(~0u, is ? c.lo : 0);
         const bool beyond = __any_sync(~0u, q.rest[lane & (kCols - 1)] != 1.0f);
-        w.apart = (beyond ? 2 : 0) | (beyond || p.softcap > 0.0f || p.slopes != nullptr ? 1 : 0);
+        w.apart = (beyond ? 2 : 0) | (beyond || p.cap > 0.0f || p.slopes != nullptr ? 1 : 0);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -645,14 +645,13 @@ struct Attend {
                         for (int h = 0; h < MT; ++h) s[h][nt][e] *= rest;
                     }
             }
-            if (p.softcap > 0.0f) {
-                const float down = 1.0f / (p.softcap * kLog2e), up = p.softcap * kLog2e;
+            if (p.cap > 0.0f) {
 #pragma unroll
                 for (int h = 0; h < MT; ++h)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[h][nt][e] = tanhf(s[h][nt][e] * down) * up;
+                        for (int e = 0; e < 4; ++e) s[h][nt][e] = tanhf(s[h][nt][e] * p.cap_inverse) * p.cap;
             }
             if (p.slopes != nullptr) {
 #pragma unroll

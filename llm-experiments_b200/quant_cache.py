@@ -14,7 +14,6 @@ but not counted yet), and advances with the last layer; a single layer advances 
 """
 from __future__ import annotations
 
-import math
 from typing import List, Optional
 
 import torch
@@ -27,6 +26,7 @@ from .types import GPUBuffer1D, GPUBuffer2D, GPUContext, QuantKVCache, QuantKVCa
 
 HEAD_DIMS = (32, 64, 96, 128, 256)
 BITS = ((4, 4), (8, 4), (8, 8))
+LARGEST = torch.finfo(torch.float32).max
 MAX_TOKENS = 64  # new tokens per sequence that attention takes in one call
 
 
@@ -171,8 +171,8 @@ def attention_with_quant_cache(ctx: GPUContext, cache: QuantKVCache, layer_idx: 
         raise ValueError("Cache is empty: current_len=0")
     if window < 0:
         raise ValueError(f"window must be >= 0, got {window}")
-    if not (math.isfinite(softcap) and (softcap == 0 or softcap >= 1e-30)) or (scale is not None and not math.isfinite(scale)):
-        raise ValueError(f"softcap must be 0 or finite and at least 1e-30 and scale finite, got {softcap} and {scale}")
+    if not (softcap == 0 or 1e-30 <= softcap <= LARGEST) or not (scale is None or -LARGEST <= scale <= LARGEST):
+        raise ValueError(f"softcap must be 0 or at least 1e-30, and it and scale finite float32 numbers, got {softcap} and {scale}")
     D, columns = cache.head_dim, q_new.shape[1]
     heads = columns // D
     if heads * D != columns or heads == 0 or heads % cache.n_kv_heads != 0:

@@ -1,11 +1,11 @@
 """Attention over a quantised cache at the ends of its inputs' ranges, against float64: values near the type's largest, groups and tokens whose
-values lie far apart, large values that no weight or no query reaches, queries and keys at the ends of the type."""
+values lie far apart, large values that no weight or no query reaches, queries, keys and caps at the ends of the type."""
 import numpy as np
 import pytest
 import torch
 
 from oracle import quant_cache_oracle as qo
-from tests.test_gpu_quant_cache import BF, F32, attend, make, np64, rnd, tune, update  # noqa: F401  (tune: a fixture)
+from tests.test_gpu_quant_cache import BF, F32, attend, filled, make, np64, one, rnd, tune, update  # noqa: F401  (tune: a fixture)
 from tests.kv_util import make_ctx
 
 pytestmark = pytest.mark.gpu
@@ -143,7 +143,7 @@ def test_values_near_the_largest_number(pkg, ctx, tune, dtype, D, bits, cluster,
 
 
 # ---------------------------------------------------------------------------------------------------------------------
-# queries
+# queries and caps
 # ---------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [BF, F32])
@@ -161,3 +161,25 @@ def test_queries_at_the_ends_of_the_type(pkg, ctx, dtype, bits, q_exp, k_exp, sc
     q[:, 2 * D:] = times(q[:, 2 * D:], torch.full((3, D), q_exp - 1))
     q[:, :D] = 0.0                                                # (a head beside them whose scores are all 0)
     check(attend(pkg, ctx, cache, q, scale=scale, **options), q, held, lens, 1, scale, extra=2.0 ** -22 * options.get("softcap", 0.0), **options)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("cap", [1e-30, 1e-3, 1e10, 1e30, 1e37, 1e38, 2.4e38, float(torch.finfo(F32).max)])
+@pytest.mark.parametrize("slopes", [False, True])
+def test_every_cap_that_is_taken(pkg, ctx, dtype, cap, slopes):
+    """A cap beyond all scores is none; one below them all leaves the tokens' mean (and the bias)."""
+    lens, D = [1, 40, 500], 64
+    cache, held = filled(pkg, ctx, lens, 500, 1, D, dtype, (8, 4))
+    q = rnd((3, 2 * D), dtype, 9, 3.0)
+    bias = torch.tensor([0.25, 0.01], device="cuda")
+    got = attend(pkg, ctx, cache, q, softcap=cap, slopes=one(pkg, bias) if slopes else None)
+    assert torch.isfinite(got).all()
+    K, V = held
+    got64, q64 = np64(got).reshape(3, 1, 2, D), np64(q).reshape(3, 1, 2, D)
+    for b, n in enumerate(lens):
+        out, mean, size = qo.attention(q64[b], K[b, :n], V[b, :n], D ** -0.5, cap, 0, np64(bias) if slopes else None)
+        # scores (below 40) are rounded a few times on their way through the cap, the bias (up to n / 4) once; a cap near the type's largest number leaves
+        # steps of 2^-149 in what tanh gets, 2^-23 of a score by a cap of 2^126 or less
+        extra = 2.0 ** -22 * (min(cap, 40.0) + (0.25 * n if slopes else 0.0)) + 2.0 ** -22
+        tol = qo.tolerance_seen(out, mean, size, n, "bf16" if dtype == BF else "f32", qo.largest_seen(V[b, :n], 1, 2), extra)
+        assert (np.abs(got64[b] - out) <= tol).all(), (b, n, np.abs(got64[b] - out).max(), tol.min())

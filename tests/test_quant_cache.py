@@ -170,6 +170,15 @@ def test_attention_refusals(pkg, ctx):
         gpu.attention_with_quant_cache(ctx, c, 0, q, q)
 
 
+def test_numbers_beyond_float32_are_refused(pkg, ctx):
+    gpu, c = pkg.gpu, make(pkg, ctx)
+    c.current_len = 30
+    q = two(pkg, 2, 256)
+    for kw in (dict(softcap=1e300), dict(softcap=3.5e38), dict(scale=1e300), dict(scale=-3.5e38), dict(softcap=float("nan")), dict(scale=float("-inf"))):
+        with pytest.raises(ValueError, match="softcap"):
+            gpu.attention_with_quant_cache(ctx, c, 0, q, q, **kw)
+
+
 def test_entry_points_check_before_any_launch(pkg):
     native = pkg._native
     lib, A = native.lib, 0x1000
