@@ -126,12 +126,9 @@ int b2kv_qcache_attend(const b2kv_qcache* cache, const b2kv_qcache_attend_args* 
     p.window = static_cast<int>(std::min<int64_t>(a.window, static_cast<int64_t>(a.T_upper) + a.m));  // (no sum with it overflows)
     p.cluster = plan.cluster;
     p.scale = static_cast<float>(frexp(static_cast<double>(a.scale) * M_LOG2E, &p.scale_exp));
-    if (a.softcap > 0.0f) {
-        // A larger cap is taken for 2^126, whose inverse is a normal number, and the product with log2 e finite.  (Scores that would show the difference lie
-        // above 2^114, where the next fp32 number is 2^91 away.)
-        p.cap = static_cast<float>(std::min(a.softcap * M_LOG2E, 0x1p126));
-        p.cap_inverse = 1.0f / p.cap;
-    }
+    // A cap beyond 2^126 is taken for that, whose inverse is a normal number, and its product with log2 e is finite.  (Scores that would show the difference lie
+    // above 2^114, where the next fp32 number is 2^91 away.)
+    p.cap = static_cast<float>(std::min(a.softcap * M_LOG2E, 0x1p126));
     p.ws_o = static_cast<float*>(workspace);
     p.ws_lse = p.ws_o + static_cast<size_t>(plan.ctas) * 2 * plan.cols * c.D;
     p.tickets = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + tickets_at(plan, c));

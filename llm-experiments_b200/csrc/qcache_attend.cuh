@@ -57,7 +57,7 @@ struct AttendParams {
     int cluster;      // > 0: a cluster of this many CTAs per (sequence, head, column tile); 0: all tokens laid end to end and cut into gridDim.x pieces
     float scale;        // scale * log2 e = scale * 2^scale_exp
     int scale_exp;
-    float cap, cap_inverse;  // the cap times log2 e, one over it; 0 without one
+    float cap;          // times log2 e; 0 without one
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -646,12 +646,13 @@ struct Attend {
                     }
             }
             if (p.cap > 0.0f) {
+                const float down = 1.0f / p.cap;
 #pragma unroll
                 for (int h = 0; h < MT; ++h)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[h][nt][e] = tanhf(s[h][nt][e] * p.cap_inverse) * p.cap;
+                        for (int e = 0; e < 4; ++e) s[h][nt][e] = tanhf(s[h][nt][e] * down) * p.cap;
             }
             if (p.slopes != nullptr) {
 #pragma unroll
@@ -736,13 +737,14 @@ struct Attend {
                     s[h][nt][e + 2] = ex2(s[h][nt][e + 2]);
                     w.sum[nt][e] += s[h][nt][e] + s[h][nt][e + 2];
                 }
-        // Value scales relative to their references; a vote on whether all lie where fp16 holds them (zeros do).
+        // Value scales relative to their references; one vote on whether there are references yet and all scales lie where fp16 holds them (zeros do).
         Words<kSRow> mine;
         mine.load(vs + (lane & (kTok - 1)) * kSRow);
         float x[kSG];
-        if (refs.by[0] == 0.0f) first_refs(refs, mine);
-        if (__any_sync(~0u, relative(refs, mine, x))) {
-            far_scales(w, refs, stage, s, hidden, mine);
+        const bool first = refs.by[0] == 0.0f;
+        if (__builtin_expect(__any_sync(~0u, relative(refs, mine, x) || first), 0)) {
+            if (first) first_refs(refs, mine);
+            if (!first || __any_sync(~0u, relative(refs, mine, x))) far_scales(w, refs, stage, s, hidden, mine);
             relative(refs, mine, x);
         }
         if constexpr (kF32)
