@@ -375,6 +375,7 @@ struct Attend {
                     for (int v = NG; v < kSG; ++v) q.sum[nt][gid][v] = 0.0f;
             }
         }
+        bool beyond = false;
         if (threadIdx.x < kCols) {
             const int c = threadIdx.x, col = ct * kCols + c, i = col / p.R, place = n - p.m + i;
             const bool is = col < p.m * p.R;
@@ -382,17 +383,17 @@ struct Attend {
             // ordinary one, so this may be no fp32 number
             const int power = p.scale_exp + exponent(c / 8, c % 8) - 127 - 14 - kKeyUnitExp, within = min(max(power, -100), 100);
             const float f = p.scale * __int_as_float((127 + within) << 23);
-            q.rest[c] = is ? __int_as_float((127 + min(max(power - within, -126), 127)) << 23) : 1.0f;
+            q.rest[c] = __int_as_float((127 + min(max(power - within, -126), 127)) << 23);
+            beyond = is && power != within;
             q.columns[c] = Column{is && p.window > 0 ? max(place + 1 - p.window, 0) : 0, is ? place + 1 : 0,
                                   is && p.slopes != nullptr ? p.slopes[g * p.R + col - i * p.R] * kLog2e : 0.0f, f};
         }
-        __syncthreads();
+        beyond = __syncthreads_or(beyond);
 
         const Column c = q.columns[lane & (kCols - 1)];
         const bool is = ct * kCols + (lane & (kCols - 1)) < p.m * p.R;
         w.all_lim = __reduce_min_sync(~0u, is ? c.lim : 0x7fffffff);
         w.all_lo = __reduce_max_sync(~0u, is ? c.lo : 0);
-        const bool beyond = __any_sync(~0u, q.rest[lane & (kCols - 1)] != 1.0f);
         w.apart = (beyond ? 2 : 0) | (beyond || p.cap > 0.0f || p.slopes != nullptr ? 1 : 0);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -743,9 +744,15 @@ struct Attend {
         float x[kSG];
         const bool first = refs.by[0] == 0.0f;
         if (__builtin_expect(__any_sync(~0u, relative(refs, mine, x) || first), 0)) {
-            if (first) first_refs(refs, mine);
-            if (!first || __any_sync(~0u, relative(refs, mine, x))) far_scales(w, refs, stage, s, hidden, mine);
-            relative(refs, mine, x);
+            bool far = true;
+            if (first) {
+                first_refs(refs, mine);
+                far = __any_sync(~0u, relative(refs, mine, x));
+            }
+            if (far) {
+                far_scales(w, refs, stage, s, hidden, mine);
+                relative(refs, mine, x);
+            }
         }
         if constexpr (kF32)
             values_f32(l, w, stage, s, x);
