@@ -54,8 +54,11 @@ bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& pla
     const int at_once = device_sm_count() * 2;  // CTAs that run at the same time
     // Columns (new token, query head) of a key / value head that are taken together: 16 share the widening of the codes (4 sequences of 131072
     // tokens, 16 heads to one: 198 against 242 us), 8 make more pairs where there are few tokens to a CTA (40 columns over 2048 tokens: 22.1 against 25.5 us).
+    // Keys of 8 and values of 4 bits in heads of 256 have no form of 16 (kWide): it took 261.5 -> 296.8 us for 4 sequences of 65536 tokens and 16 heads to one,
+    // 212.2 -> 248.0 for 64 of 2048 .. 4096, 108.5 -> 140.9 for 16 columns over 32 of 4096 .. 8192.  With the same bits for both it pays at length
+    // ((4, 4) 227.3 -> 200.4 us and 198.1 -> 183.8, (8, 8) 359.5 -> 275.1 and 257.5 -> 251.6) and costs up to 8 and 18 % in the last case.
     const int forced_columns = tune_get("qcache_columns");
-    const bool wide = c.dtype != B2KV_DTYPE_F32 &&
+    const bool wide = c.dtype != B2KV_DTYPE_F32 && (c.D != 256 || c.k_bits == c.v_bits) &&
                       (forced_columns != 0 ? forced_columns == 16 : columns > 8 && heads * ((columns + 15) / 16) * most >= at_once * 1024ll);
     plan.cols = c.dtype == B2KV_DTYPE_F32 ? 4 : wide ? 16 : 8;
     plan.col_tiles = (columns + plan.cols - 1) / plan.cols;

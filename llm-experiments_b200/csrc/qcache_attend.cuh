@@ -1546,7 +1546,10 @@ int clusters_at_once(int size);
 template <int NG, int KB, int VB>
 int attend_sized(const AttendParams& p, const Plan& plan, void* stream) {
     if (p.c.dtype == B2KV_DTYPE_F32) return launch_attend<float, NG, KB, VB, 1>(p, plan, stream);
-    return plan.cols == 8 ? launch_attend<__nv_bfloat16, NG, KB, VB, 1>(p, plan, stream) : launch_attend<__nv_bfloat16, NG, KB, VB, 2>(p, plan, stream);
+    constexpr bool kWide = NG != 8 || KB == VB;  // tiles of 16 columns (make_plan asks for none elsewhere)
+    if constexpr (kWide)
+        if (plan.cols == 16) return launch_attend<__nv_bfloat16, NG, KB, VB, 2>(p, plan, stream);
+    return launch_attend<__nv_bfloat16, NG, KB, VB, 1>(p, plan, stream);
 }
 
 // One file each, so that they compile side by side.

@@ -215,3 +215,20 @@ def test_entry_points_check_before_any_launch(pkg):
     assert lib.b2kv_qcache_attend_workspace_bytes(cache(D=80), native.qcache_attend_args(*args.values())) == 0
     assert [lib.b2kv_qcache_scale_row(d) for d in (32, 64, 96, 128, 256, 80, 0)] == [2, 2, 4, 4, 8, 0, 0]
     assert ctypes.sizeof(native.QCache) == 96 and ctypes.sizeof(native.QCacheAttendArgs) == 72
+
+
+@pytest.mark.parametrize("D,bits,wide", [(128, (8, 4), True), (256, (4, 4), True), (256, (8, 8), True), (256, (8, 4), False)])
+def test_columns_that_are_taken_together(pkg, D, bits, wide):
+    """Scratch memory tells the tiles apart: results of 16 columns per CTA, or of 8 and a ticket more.  Heads of 256 in 8 and 4 bits have no tiles of 16."""
+    native, need = pkg._native, {}
+    cache = native.qcache(0x1000, 0x1000, 0x1000, 0x1000, 0, 0, 1 << 20, 1, 1, D, 1 << 20, 0, 0, 0, *bits, 1)
+    args = native.qcache_attend_args(0x1000, 0x1000, 0, 16 * D, 16 * D, 16, 1, 1 << 20, 0, 0, 0.125, 0.0)
+    try:
+        native.tune("qcache_cluster", -1)
+        for columns in (8, 16):
+            native.tune("qcache_columns", columns)
+            need[columns] = native.lib.b2kv_qcache_attend_workspace_bytes(cache, args)
+    finally:
+        native.tune("qcache_columns", 0)
+        native.tune("qcache_cluster", 0)
+    assert (need[16] != need[8]) == wide and need[8] > 0
