@@ -122,13 +122,28 @@ def prompt_layer_scratch(ctx: GPUContext, rows: int, embedding_dim: int, hidden_
                               a=mk(embedding_dim), x2=mk(embedding_dim), m=mk(hidden_dim))
 
 
+def _check_prompt(cache: QuantKVCache, x: GPUBuffer2D, batch_size: int, seq_len: int) -> None:
+    """What ``flash_attention`` checks of the cache that it writes into, before any cache is started over."""
+    if cache.batch_size != batch_size or cache.n_kv_heads * cache.head_dim != x.shape[1]:
+        raise ValueError("cache dimensions do not match the prompt's")
+    if seq_len <= 0:
+        raise ValueError(f"seq_len must be > 0, got {seq_len}")
+    if seq_len > cache.max_seq_len:
+        raise ValueError(f"Cache is full: seq_len={seq_len}, max_seq_len={cache.max_seq_len}")
+    if cache.dtype != x.buffer.dtype:
+        raise ValueError(f"cache dtype {cache.dtype} does not match {x.buffer.dtype}")
+
+
 def prompt_layer_step(ctx: GPUContext, cache: Union[KVCache, QuantKVCache], x: GPUBuffer2D, w: DecoderLayerWeights, s: PromptLayerScratch,
                       y: GPUBuffer2D, batch_size: int, seq_len: int) -> None:
     """The same layer for a whole prompt: ``x`` and ``y`` are ``[batch_size * seq_len, E]``.  The reference's
     block as it stands (simple-llm/src/wgpu_backend.py:794-935: three projections, causal
     ``flash_attention``, output projection, MLP), with the prompt's K / V rows written into ``cache``
     (layer 0 of that cache object; its length becomes ``seq_len``) by the attention kernel.  Nine
-    operations are recorded; the projections run on the tiled tensor-core GEMM."""
+    operations are recorded (ten with a quantised cache, which the rows go into behind the attention); the projections run on the tiled
+    tensor-core GEMM."""
+    if isinstance(cache, QuantKVCache):
+        _check_prompt(cache, x, batch_size, seq_len)
     layernorm(ctx, x, w.ln1_gamma, w.ln1_beta, s.h)
     matmul(ctx, s.h, w.wq, s.q)
     matmul(ctx, s.h, w.wk, s.k)

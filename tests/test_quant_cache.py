@@ -232,3 +232,50 @@ def test_columns_that_are_taken_together(pkg, D, bits, wide):
         native.tune("qcache_columns", 0)
         native.tune("qcache_cluster", 0)
     assert (need[16] != need[8]) == wide and need[8] > 0
+
+
+# ---- the decoder ----
+
+def decoder(pkg, ctx, batch_size=2, context_size=32, kv_bits=(8, 4), ragged=True):
+    """(model module, state) of a decoder of zeros with one head of 64 and two layers."""
+    from llm_experiments_b200 import model
+
+    cfg = model.DecoderConfig(vocab_size=64, context_size=context_size, embedding_dim=64, n_heads=1, n_layers=2)
+    z = lambda *shape: np.zeros(shape, dtype=np.float32)  # noqa: E731
+    layer = dict(ln1_gamma=z(64), ln1_beta=z(64), wq=z(64, 64), wk=z(64, 64), wv=z(64, 64), wo=z(64, 64), ln2_gamma=z(64), ln2_beta=z(64),
+                 w1=z(64, 256), b1=z(256), w2=z(256, 64), b2=z(64))
+    weights = model.weights_from_numpy(ctx, cfg, dict(embedding=z(64, 64), pos_encoding=model.positional_encoding(context_size, 64), layers=[layer, layer],
+                                                      lnf_gamma=z(64), lnf_beta=z(64), out_proj=z(64, 64)))
+    return model, model.decoder_state_create(ctx, cfg, weights, batch_size=batch_size, kv_bits=kv_bits, ragged=ragged)
+
+
+@pytest.fixture()
+def no_launches(pkg, monkeypatch):
+    """Operators of a layer that only note that they were called."""
+    from llm_experiments_b200 import decode_layer
+
+    called = []
+    for name in ("layernorm", "matmul", "flash_attention"):
+        monkeypatch.setattr(decode_layer, name, lambda *a, _name=name, **kw: called.append(_name))
+    return called
+
+
+def test_a_prompt_that_is_refused_leaves_the_caches_as_they_were(pkg, ctx, no_launches):
+    model, state = decoder(pkg, ctx)
+    from llm_experiments_b200 import decode_layer
+    for cache in state.caches:
+        pkg.gpu.quant_cache_set_lengths(cache, [7, 20])
+
+    def refused(text, batch, seq_len, width=64, dtype=torch.bfloat16):
+        x = two(pkg, batch * seq_len, width, dtype)
+        scratch = decode_layer.prompt_layer_scratch(ctx, batch * seq_len, width)
+        with pytest.raises(ValueError, match=text):
+            decode_layer.prompt_layer_step(ctx, state.caches[0], x, state.weights.layers[0], scratch, x, batch, seq_len)
+        assert no_launches == []
+        assert all(c.current_len == 20 and c.seq_lens.tolist() == [7, 20] for c in state.caches)
+
+    refused("Cache is full: seq_len=33", 2, 33)
+    refused("dimensions", 3, 10)
+    refused("dimensions", 2, 10, width=128)
+    refused("dtype", 2, 10, dtype=torch.float32)
+    refused("seq_len", 2, 0)
