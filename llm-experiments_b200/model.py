@@ -11,7 +11,9 @@ cached decode steps, and every operation is one of this package's operators (no 
              attention, Wo, MLP) -> layernorm -> matmul (logits) -> argmax
 
 Storage is bfloat16, arithmetic fp32.  Every layer owns a ``KVCache`` object of one layer, so lengths advance
-once per layer step; positions of a decode step come from layer 0's lengths before it advances them.
+once per layer step; positions of a decode step come from layer 0's lengths before it advances them.  With ``kv_bits`` the caches
+are ``QuantKVCache`` objects in 4 or 8 bits: a step's Q, K and V come from three products, new rows are quantised into the
+cache, and attention reads it as it is (``decode_layer.py``).
 """
 from __future__ import annotations
 
@@ -76,6 +78,7 @@ class DecoderState:
     prompt_y: Optional[GPUBuffer2D] = None
     prompt_scratch: Optional[PromptLayerScratch] = None
     last: Optional[GPUBuffer2D] = field(default=None)
+    kv_bits: Optional[Tuple[int, int]] = None  # of the caches' keys and values; None: bfloat16
 
 
 def _b2(t: torch.Tensor) -> GPUBuffer2D:
@@ -151,7 +154,7 @@ def decoder_state_create(ctx: GPUContext, cfg: DecoderConfig, weights: DecoderWe
     ctx.config.flash_attn_max_head_dim = max(ctx.config.flash_attn_max_head_dim, cfg.head_dim)
     return DecoderState(cfg=cfg, weights=weights, batch_size=batch_size, caches=caches, x=mk(E), y=mk(E), h=mk(E),
                         logits=mk(cfg.vocab_size), scratch=decode_layer.decoder_layer_scratch(ctx, batch_size, E, quantised=kv_bits is not None),
-                        last=mk(E))
+                        last=mk(E), kv_bits=None if kv_bits is None else tuple(kv_bits))
 
 
 def decoder_state_reset(state: DecoderState) -> None:
@@ -159,11 +162,12 @@ def decoder_state_reset(state: DecoderState) -> None:
         kv_cache_reset(cache)
 
 
-def launches_per_decode_step(cfg: DecoderConfig) -> int:
+def launches_per_decode_step(cfg: DecoderConfig, kv_bits: Optional[Tuple[int, int]] = None) -> int:
     """Kernels of this library launched by one ``decode_step``: the embedding, eight per layer (seven operations
     and the advance of the layer cache's device-side lengths), the final layernorm, the logits projection and the
-    argmax."""
-    return 1 + 8 * cfg.n_layers + 3
+    argmax.  Over quantised caches (``kv_bits`` of the state) a layer's are eleven: three projections and the write of the
+    new rows stand in the place of the one launch that does both, and attention, advance and the rest as before."""
+    return 1 + (8 if kv_bits is None else 11) * cfg.n_layers + 3
 
 
 def _head(ctx: GPUContext, state: DecoderState, rows: GPUBuffer2D, next_ids: Optional[GPUBuffer1D]) -> None:

@@ -279,3 +279,17 @@ def test_a_prompt_that_is_refused_leaves_the_caches_as_they_were(pkg, ctx, no_la
     refused("dimensions", 2, 10, width=128)
     refused("dtype", 2, 10, dtype=torch.float32)
     refused("seq_len", 2, 0)
+
+
+def test_launches_of_a_step_over_quantised_caches(pkg, ctx, monkeypatch):
+    """Counted where the operators of a layer are called: each is one kernel, and the write with lengths on the device a second one."""
+    from llm_experiments_b200 import decode_layer
+
+    model, state = decoder(pkg, ctx)
+    called = []
+    for name in ("layernorm", "matmul", "quant_cache_update", "attention_with_quant_cache"):
+        monkeypatch.setattr(decode_layer, name, lambda *a, _name=name, **kw: called.append(_name))
+    decode_layer.decoder_layer_step(ctx, state.caches[0], state.x, state.weights.layers[0], state.scratch, state.y)
+    per_layer = len(called) + called.count("quant_cache_update")
+    assert per_layer == 11 and model.launches_per_decode_step(state.cfg, state.kv_bits) == 1 + per_layer * 2 + 3
+    assert model.launches_per_decode_step(state.cfg) == 1 + 8 * 2 + 3
