@@ -141,8 +141,8 @@ def decoder_state_create(ctx: GPUContext, cfg: DecoderConfig, weights: DecoderWe
         raise ValueError(f"Sequence length {T} exceeds context size {cfg.context_size}")
     E, dev = cfg.embedding_dim, ctx.device
     if kv_bits is not None:
-        if len(kv_bits) != 2:
-            raise ValueError(f"kv_bits must be the bits of keys and of values, got {kv_bits!r}")
+        if not isinstance(kv_bits, (tuple, list)) or len(kv_bits) != 2 or not all(type(b) is int for b in kv_bits):
+            raise ValueError(f"kv_bits must be the bits of keys and of values, two whole numbers, got {kv_bits!r}")
         caches = [quant_cache_create(ctx, QuantKVCacheConfig(batch_size=batch_size, max_seq_len=T, n_layers=1, n_kv_heads=cfg.n_heads,
                                                              head_dim=cfg.head_dim, k_bits=kv_bits[0], v_bits=kv_bits[1],
                                                              ragged=ragged)) for _ in range(cfg.n_layers)]
@@ -369,5 +369,4 @@ def _build(ctx: GPUContext, config: dict, weights: dict, dtype: torch.dtype, bat
     layers = [{k: get(f"layers.{i}.{k}") for k in DecoderLayerWeights.__dataclass_fields__} for i in range(cfg.n_layers)]
     params = dict(embedding=get("embedding"), pos_encoding=positional_encoding(cfg.context_size, cfg.embedding_dim), layers=layers,
                   lnf_gamma=get("lnf_gamma"), lnf_beta=get("lnf_beta"), out_proj=get("out_proj"))
-    bits = config.get("kv_bits")
-    return CachedDecoder(ctx, cfg, weights_from_numpy(ctx, cfg, params), None if bits is None else tuple(int(b) for b in bits))
+    return CachedDecoder(ctx, cfg, weights_from_numpy(ctx, cfg, params), config.get("kv_bits"))

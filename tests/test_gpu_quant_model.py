@@ -107,3 +107,25 @@ def test_generation_over_a_quantised_cache(pkg):
     prompt = [int(t) for t in np.random.default_rng(2).integers(0, 512, size=9)]
     first = generate.generate_text(dec, prompt, max_tokens=6, temperature=0.0)
     assert first[:9] == prompt and len(first) == 15 and generate.generate_text(dec, prompt, max_tokens=6, temperature=0.0) == first
+
+
+def test_generation_from_a_model_folder(pkg, tmp_path):
+    """``kv_bits`` of ``config.json``: the same tokens as of a decoder made with them, over caches of those bits."""
+    import json
+
+    from llm_experiments_b200 import checkpoint, generate, model
+
+    ctx = pkg.gpu.context_create(0)
+    cfg = model.DecoderConfig(vocab_size=512, context_size=64, embedding_dim=256, n_heads=2, n_layers=2)
+    params = _params(cfg, model, seed=5)
+    tensors = {k: params[k] for k in ("embedding", "out_proj", "lnf_gamma", "lnf_beta")}
+    tensors.update({f"layers.{i}.{k}": x for i, layer in enumerate(params["layers"]) for k, x in layer.items()})
+    checkpoint.write_safetensors(tmp_path / "model.safetensors", {k: torch.from_numpy(x).to(torch.bfloat16) for k, x in tensors.items()})
+    (tmp_path / "config.json").write_text(json.dumps(dict(architecture="GPTDecoder", vocab_size=512, context_size=64, embedding_dim=256, n_heads=2, n_layers=2,
+                                                          kv_bits=[8, 4])))
+    loaded = pkg.gpu.load_model(ctx, tmp_path)
+    assert all(isinstance(c, pkg.gpu.QuantKVCache) and (c.k_bits, c.v_bits) == (8, 4) for c in loaded.state.caches)
+    prompt = [int(t) for t in np.random.default_rng(2).integers(0, 512, size=9)]
+    made = model.CachedDecoder(ctx, cfg, model.weights_from_numpy(ctx, cfg, params), kv_bits=(8, 4))
+    got = generate.generate_text(loaded, prompt, max_tokens=6, temperature=0.0)
+    assert len(got) == 15 and got == generate.generate_text(made, prompt, max_tokens=6, temperature=0.0)

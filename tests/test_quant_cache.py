@@ -249,6 +249,35 @@ def decoder(pkg, ctx, batch_size=2, context_size=32, kv_bits=(8, 4), ragged=True
     return model, model.decoder_state_create(ctx, cfg, weights, batch_size=batch_size, kv_bits=kv_bits, ragged=ragged)
 
 
+def folder_config():
+    return dict(architecture="GPTDecoder", vocab_size=64, context_size=32, embedding_dim=64, n_heads=1, n_layers=1)
+
+
+def folder_weights():
+    z = lambda *shape: torch.zeros(shape, dtype=torch.bfloat16)  # noqa: E731
+    layer = dict(ln1_gamma=z(64), ln1_beta=z(64), wq=z(64, 64), wk=z(64, 64), wv=z(64, 64), wo=z(64, 64), ln2_gamma=z(64), ln2_beta=z(64),
+                 w1=z(64, 256), b1=z(256), w2=z(256, 64), b2=z(64))
+    return dict(embedding=z(64, 64), out_proj=z(64, 64), lnf_gamma=z(64), lnf_beta=z(64), **{f"layers.0.{k}": t for k, t in layer.items()})
+
+
+@pytest.mark.parametrize("bits", [None, [8, 4], [4, 4]])
+def test_kv_bits_of_a_model_folder(pkg, ctx, tmp_path, bits):
+    """``config.json`` and ``model.safetensors`` through the registry: caches of these bits, or bfloat16 ones without the entry."""
+    import json
+
+    from llm_experiments_b200 import checkpoint
+
+    (tmp_path / "config.json").write_text(json.dumps(folder_config() if bits is None else dict(folder_config(), kv_bits=bits)))
+    checkpoint.write_safetensors(tmp_path / "model.safetensors", folder_weights())
+    dec = pkg.gpu.load_model(ctx, tmp_path)
+    (cache,) = dec.state.caches
+    if bits is None:
+        assert isinstance(cache, pkg.gpu.KVCache) and dec.state.kv_bits is None
+    else:
+        assert isinstance(cache, pkg.gpu.QuantKVCache) and [cache.k_bits, cache.v_bits] == bits and dec.state.kv_bits == tuple(bits)
+        assert (cache.max_seq_len, cache.n_kv_heads, cache.head_dim) == (32, 1, 64)
+
+
 @pytest.fixture()
 def no_launches(pkg, monkeypatch):
     """Operators of a layer that only note that they were called."""
@@ -293,3 +322,13 @@ def test_launches_of_a_step_over_quantised_caches(pkg, ctx, monkeypatch):
     per_layer = len(called) + called.count("quant_cache_update")
     assert per_layer == 11 and model.launches_per_decode_step(state.cfg, state.kv_bits) == 1 + per_layer * 2 + 3
     assert model.launches_per_decode_step(state.cfg) == 1 + 8 * 2 + 3
+
+
+@pytest.mark.parametrize("bits", [8, "84", (8.5, 4), ("8", "4"), (None, 4)])
+def test_kv_bits_that_are_no_pair_of_numbers(pkg, ctx, bits):
+    from llm_experiments_b200 import registry
+
+    with pytest.raises(ValueError, match="kv_bits"):
+        decoder(pkg, ctx, kv_bits=bits)
+    with pytest.raises(ValueError, match="kv_bits"):
+        registry.build_model(ctx, dict(folder_config(), kv_bits=bits), folder_weights())
