@@ -87,6 +87,8 @@ def decoder_layer_step(ctx: GPUContext, cache: Union[KVCache, QuantKVCache], x: 
     """Writes the layer's output rows for one new token per sequence into ``y`` and appends the token's
     K / V to ``cache`` (layer 0 of that cache object).  To be called between ``batch_begin`` and
     ``batch_commit``; seven operations are recorded (ten with a quantised cache, whose scratch has ``k`` and ``v``)."""
+    if isinstance(cache, QuantKVCache) and (s.k is None or s.v is None):
+        raise ValueError("a quantised cache takes scratch with room for its new rows: decoder_layer_scratch(..., quantised=True)")
     layernorm(ctx, x, w.ln1_gamma, w.ln1_beta, s.h)
     if isinstance(cache, QuantKVCache):
         for weights, rows in ((w.wq, s.q), (w.wk, s.k), (w.wv, s.v)):

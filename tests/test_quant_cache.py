@@ -324,6 +324,17 @@ def test_launches_of_a_step_over_quantised_caches(pkg, ctx, monkeypatch):
     assert model.launches_per_decode_step(state.cfg) == 1 + 8 * 2 + 3
 
 
+def test_a_step_without_room_for_the_new_rows_is_refused(pkg, ctx, no_launches):
+    """Scratch made for bfloat16 caches."""
+    from llm_experiments_b200 import decode_layer
+
+    model, state = decoder(pkg, ctx)
+    plain = decode_layer.decoder_layer_scratch(ctx, 2, 64)
+    with pytest.raises(ValueError, match="quantised=True"):
+        decode_layer.decoder_layer_step(ctx, state.caches[0], state.x, state.weights.layers[0], plain, state.y)
+    assert no_launches == [] and state.caches[0].current_len == 0
+
+
 @pytest.mark.parametrize("bits", [8, "84", (8.5, 4), ("8", "4"), (None, 4)])
 def test_kv_bits_that_are_no_pair_of_numbers(pkg, ctx, bits):
     from llm_experiments_b200 import registry
