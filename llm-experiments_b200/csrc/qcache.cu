@@ -220,7 +220,7 @@ __device__ __forceinline__ void write_row(const b2kv_qcache& c, const T* src, in
 
 // Thread = (row of a head, octet); grid.y 0 keys, 1 values.
 template <typename T, int NG, int KB, int VB>
-__global__ void __launch_bounds__(kThreads) write_kernel(const b2kv_qcache c, const T* k, int64_t ld_k, const T* v, int64_t ld_v, int n, Divisor by_heads,
+__global__ void __launch_bounds__(kThreads) write_kernel(const b2kv_qcache c, const T* k, int64_t ld_k, const T* v, int64_t ld_v, Divisor by_heads,
                                                          Divisor by_rows, Divisor by_block, uint32_t rows, int32_t* dev_status) {
     grid_launch_dependents();
     grid_dependency_wait();
@@ -282,7 +282,7 @@ int launch_write(const b2kv_qcache& c, const void* k, int64_t ld_k, const void* 
     const int64_t rows = static_cast<int64_t>(c.B) * n * c.G;
     if (rows > 0x7fffffff) return B2KV_ERR_UNSUPPORTED;
     OverlapLaunch launch(dim3(static_cast<unsigned>((rows + kThreads / 4 - 1) / (kThreads / 4)), 2), kThreads, 0, stream);
-    B2KV_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, write_kernel<T, NG, KB, VB>, c, static_cast<const T*>(k), ld_k, static_cast<const T*>(v), ld_v, n,
+    B2KV_CUDA_TRY(cudaLaunchKernelEx(&launch.cfg, write_kernel<T, NG, KB, VB>, c, static_cast<const T*>(k), ld_k, static_cast<const T*>(v), ld_v,
                                      Divisor(c.G), Divisor(n), by_block(c), static_cast<uint32_t>(rows), dev_status));
     return B2KV_OK;
 }
