@@ -657,7 +657,8 @@ int b2kv_qcache_read(const b2kv_qcache* cache, int which, void* out, int n, int 
  * host knows.  q and out are [B * m, H * D] (ld elements between rows), row b * m + i stands at place p = n_b - m + i; head h reads
  * key / value head h / (H / G) and sees the tokens t <= p, with window > 0 only those with p - t < window:
  *   score = cap(scale * q . k) - slopes[h] * (p - t),  cap(x) = softcap * tanh(x / softcap) where softcap > 0 (1e-30 at least),  out = softmax(score) v.
- * A row that sees nothing (an empty sequence, p < 0) is zeros.  slopes (fp32, H) may be NULL.  1 <= m <= B2KV_QCACHE_MAX_ROWS.
+ * A row that sees nothing (an empty sequence, p < 0) is zeros.  An element depends on its own group of 32 alone and on the tokens that its row sees, whatever
+ * the size of others' values (tokens of a group that differ by more than 2^8 cost time).  slopes (fp32, H) may be NULL.  1 <= m <= B2KV_QCACHE_MAX_ROWS.
  * `workspace` takes b2kv_qcache_attend_workspace_bytes bytes (16-byte aligned), needs no initialisation and carries nothing between
  * calls; calls that may run at the same time need one each.
  */

@@ -64,7 +64,7 @@ bool make_plan(const b2kv_qcache& c, const b2kv_qcache_attend_args& a, Plan& pla
     plan.col_tiles = (columns + plan.cols - 1) / plan.cols;
     plan.pairs = heads * plan.col_tiles;
     if (plan.pairs > 0x7fffffff) return false;
-    // A cluster of 1 - 8 CTAs for each pair, or one run of tiles per CTA that is there.  In tokens that a CTA gets through in the time: setting
+    // A cluster of 1 - 8 CTAs for each pair, or one run of tiles per CTA that is there.  In tokens that a CTA gets through in the time (bf16 rows, heads of 128): setting
     // up and finishing a CTA is about 430, putting a cluster's results together 150, finding and cutting a run 1000 and each piece of a pair, which one CTA
     // puts together, another 10: so few pairs are cut into no more pieces than pay (one pair of 131072 tokens: 27 us in 115 pieces, 43 in 296; of
     // 8192: 12.5 in 29, 35.6 in 296; 320 pairs of 400: 18.8 in runs, 14.4 as they are).

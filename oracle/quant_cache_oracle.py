@@ -71,9 +71,9 @@ def tolerance(out, mean, size, n, dtype: str, extra: float = 0.0, largest: float
       The largest product is at most `size`.  It scales probabilities above and below the line;
     - sums over n tokens, 16 at a time: 2^-23 of the mean magnitude each, and as much for their reunion;
     `extra` is an absolute error of scores beyond that (bias, cap).
-    - fp16 numbers below 2^-14 lie 2^-24 apart.  A probability (relative to a score that was seen, so their sum is at least 1) times a
-      value scale s is held as a multiple p s / 2^(E - 6), 2^E <= the largest scale: off by up to half of 2^-24 * 2^(E - 6) = 2^-31 2^E beyond the
-      relative error, times a code up to L, over a sum of at least 1.  L 2^E <= `largest`, the largest magnitude held: 2^-31 * largest per token.
+    - fp16 numbers below 2^-14 lie 2^-24 apart.  A probability is held as a multiple w of 2^-10 of a score that was seen, so their sum is at least
+      2^10, a value scale s as s / 2^E < 2: beyond the relative error w is off by up to 2^-25, times that scale, and the product by 2^-25, times a code up
+      to L, over that sum: 3 * 2^-35 * 2^E * L.  2^E is at most 4 times the largest scale: 2^-31 * `largest`, the largest magnitude held, per token.
       (It shows where one token has nearly all the weight and a code of zero, and what is left is below 2^-31 of the values.)"""
     bf16 = dtype == "bf16"
     half, held_in = (2.0 ** -8, 2.0 ** -10) if bf16 else (2.0 ** -24, 2.0 ** -21)
