@@ -85,7 +85,7 @@ def tolerance(out, mean, size, n, dtype: str, extra: float = 0.0, largest: float
 def largest_seen(v, m, H, window=0):
     """Per query and head, of each element's group: the largest magnitude held among the tokens that the query sees.  v [n, G, D] -> [m, H, D]."""
     n, G, D = v.shape
-    most = np.repeat(np.abs(np.nan_to_num(v)).reshape(n, G, -1, GROUP).max(-1), GROUP, axis=-1)
+    most = np.repeat(np.abs(np.nan_to_num(v)).reshape(n, G, D // GROUP, GROUP).max(-1), GROUP, axis=-1)
     out = np.zeros((m, H, D))
     for i in range(m):
         p = n - m + i

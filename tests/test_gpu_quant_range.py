@@ -115,6 +115,28 @@ def test_large_values_that_a_query_does_not_see(pkg, ctx, dtype, large, bits, wi
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("cluster", [-1, 1])
+def test_sequences_of_other_sizes_one_after_another(pkg, ctx, tune, dtype, cluster):  # noqa: F811
+    """A CTA that goes through many sequences starts each with references of its own; some sequences are empty, some all zeros, some hold one NaN."""
+    tune("qcache_cluster", cluster)
+    lens, T, D = [(7 * i) % 61 for i in range(700)], 61, 64
+    B, i = len(lens), torch.arange(len(lens))
+    k, v = rnd((B * T, D), dtype, 1), rnd((B * T, D), dtype, 2)
+    v = times(v, ((i * 37) % 161 - 80).repeat_interleave(T)[:, None].expand(-1, D))
+    v.view(B, T, D)[5::50] = 0
+    cache, held = holding(pkg, ctx, lens, T, k, v, D, dtype, (8, 4))
+    q = rnd((B, 2 * D), dtype, 3, 1.5)
+    fine = attend(pkg, ctx, cache, q)
+    check(fine, q, held, lens, 1)
+    v.view(B, T, D)[9::50, 0, 40] = float("nan")
+    got = attend(pkg, ctx, holding(pkg, ctx, lens, T, k, v, D, dtype, (8, 4))[0], q).view(B, 2, D)
+    struck = [b for b in range(9, B, 50) if lens[b] > 0]
+    assert torch.isnan(got[struck][:, :, 32:]).all() and torch.equal(got[struck][:, :, :32], fine.view(B, 2, D)[struck][:, :, :32])
+    others = [b for b in range(B) if b not in struck]
+    assert torch.equal(got[others], fine.view(B, 2, D)[others])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_nan_beside_values_far_apart(pkg, ctx, dtype):
     lens, T, D = [90], 90, 128
     k, v = rnd((T, D), dtype, 1), times(rnd((T, D), dtype, 2), torch.randint(-30, 31, (T, 4), generator=torch.Generator().manual_seed(5)).repeat_interleave(32, 1))
